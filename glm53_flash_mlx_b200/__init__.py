@@ -35,3 +35,11 @@ from .packed import PackedFP8ExpertBank, PackedFP8MoE, packed_decode_moe  # noqa
 from .router import Float32Gate, router_topk  # noqa: F401
 from .hyper_connection import FFNBoundary, HyperConnection, RMSNorm, hc_expand, rms_norm  # noqa: F401
 from .dsa_output import DSAOutputProjection, head_major_to_rows  # noqa: F401
+from .latent_attention import (  # noqa: F401
+    PagePlan,
+    check_latent_status,
+    latent_attention_absorbed,
+    latent_attention_expanded,
+    latent_cache_write,
+    plan_pages,
+)

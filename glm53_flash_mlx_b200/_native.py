@@ -31,6 +31,11 @@ FLAG_F8_MMA = 16
 STATUS_BAD_EXPERT = 1
 STATUS_WAIT_TIMEOUT = 2
 STATUS_BAD_GEOMETRY = 4
+STATUS_BAD_PAGE = 8
+STATUS_NO_PAGES = 16
+
+DTYPE_BF16 = 0
+DTYPE_FP16 = 1
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -159,6 +164,26 @@ SIGNATURES: dict[str, tuple] = {
     "glm53_rms_norm": (_int, [_vp, _i64, _i64, _vp, _f, _vp, _vp]),
     "glm53_hc_expand": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp]),
     "glm53_head_major_to_rows": (_int, [_vp, _i64, _i64, _i64, _vp, _vp]),
+    "glm53_plan_pages": (
+        _int,
+        [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "glm53_latent_cache_write": (
+        _int,
+        [_vp, _i64, _i64, _i64, _i64, _int, _vp, _f, _vp, _vp, _int, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp,
+         _vp, _vp, _vp],
+    ),
+    "glm53_latent_absorbed_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "glm53_latent_absorbed": (
+        _int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+         _i64, _vp, _f, _vp, _vp, _int, _vp, _sz, _vp, _vp, _vp],
+    ),
+    "glm53_latent_expanded": (
+        _int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _int, _vp, _vp, _i64, _f, _int, _vp, _vp, _int, _vp, _vp, _vp],
+    ),
 }
 
 

@@ -1,0 +1,399 @@
+// Page planning and row stores of the paged latent cache.
+//
+// glm53_plan_pages.  With P rows a page, request i holds ceil(cached_i / P)
+// pages and needs ceil((cached_i + new_i) / P); two exclusive prefix sums over
+// the requests (new tokens, new pages) place every token and every page, so
+// token t of request i at position p = cached_i + t - start_i goes to row
+// table[i][p / P] * P + p % P of the cache, and new page j of the batch is
+// free[count - 1 - j].  A few KB are read and 12 bytes a token written: the
+// call is bound by latency, so it is one launch.  Every block scans all
+// requests itself (two loads a request from L2) instead of waiting for
+// another block, and a token on a new page takes its page from the free list
+// rather than from the table another block is writing.
+//
+// glm53_latent_cache_write.  One row a token: [x[:R] * rsqrt(mean(x[:R]^2) +
+// eps) * w | x[R:] turned by position * inv_freq], rounded once, stored at the
+// token's slot; the queries' rotary parts turn by the same angles in the same
+// launch.  Bound by HBM: every value is read and written once, in 16-byte
+// pieces.
+#include <algorithm>
+
+#include "latent.cuh"
+
+namespace glm53 {
+namespace latent {
+namespace {
+
+constexpr int kPlanThreads = 256;
+constexpr int64_t kPlanMaxRequests = 8192;  // two prefix arrays of this length fit shared memory
+constexpr int kWriteThreads = 256;
+constexpr int64_t kMaxLatent = 1024;  // four 16-byte pieces a lane
+constexpr int64_t kMaxRope = 256;
+
+struct PlanArgs {
+  const int32_t* cached;
+  const int32_t* fresh;  // new tokens
+  int B;
+  int32_t* table;
+  int64_t table_stride, table_width;
+  const int32_t* free_pages;
+  int64_t free_capacity;
+  const int32_t* free_count;
+  int page;
+  int64_t tokens;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* query_starts;
+  int32_t* seq_lens;
+  int32_t* free_count_out;
+  uint32_t* status;
+  uint32_t* status_host;
+};
+
+__device__ __forceinline__ int64_t pages_of(int64_t rows, int page) { return (rows + page - 1) / page; }
+
+// Largest i with start[i] <= v, over start[0..n] ascending with start[0] = 0
+// and v < start[n].
+__device__ __forceinline__ int find_run(const int32_t* start, int n, int32_t v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= v)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(PlanArgs a) {
+  extern __shared__ int32_t plan_smem[];
+  int32_t* tok = plan_smem;               // [B + 1] first token of each request
+  int32_t* pgs = plan_smem + (a.B + 1);   // [B + 1] first new page of each request
+  __shared__ int64_t warp_tok[kPlanThreads / 32], warp_pg[kPlanThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
+  const int i0 = min(a.B, tid * per), i1 = min(a.B, i0 + per);
+  const int64_t count = *a.free_count;
+  int64_t ntok = 0, npg = 0;
+  bool bad = count < 0 || count > a.free_capacity;
+  for (int i = i0; i < i1; ++i) {
+    const int64_t c = a.cached[i], n = a.fresh[i];
+    if (c < 0 || n < 0 || c + n > a.table_width * a.page) {
+      bad = true;
+      continue;
+    }
+    ntok += n;
+    npg += pages_of(c + n, a.page) - pages_of(c, a.page);
+  }
+  // block-wide exclusive scan of both sums, in request order
+  int64_t st = ntok, sp = npg;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, st, o), p = __shfl_up_sync(0xffffffffu, sp, o);
+    if (lane >= o) {
+      st += t;
+      sp += p;
+    }
+  }
+  if (lane == 31) {
+    warp_tok[warp] = st;
+    warp_pg[warp] = sp;
+  }
+  __syncthreads();
+  int64_t tok_total = 0, pg_total = 0, tok0 = 0, pg0 = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w == warp) {
+      tok0 = tok_total;
+      pg0 = pg_total;
+    }
+    tok_total += warp_tok[w];
+    pg_total += warp_pg[w];
+  }
+  bad = __syncthreads_or(bad || tok_total > a.tokens || pg_total > count);
+  if (!bad) {
+    int64_t t = tok0 + st - ntok, p = pg0 + sp - npg;
+    for (int i = i0; i < i1; ++i) {
+      tok[i] = (int32_t)t;
+      pgs[i] = (int32_t)p;
+      const int64_t c = a.cached[i], n = a.fresh[i];
+      t += n;
+      p += pages_of(c + n, a.page) - pages_of(c, a.page);
+    }
+    if (tid == kPlanThreads - 1) {
+      tok[a.B] = (int32_t)tok_total;
+      pgs[a.B] = (int32_t)pg_total;
+    }
+  }
+  __syncthreads();
+
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x, first = (int64_t)blockIdx.x * blockDim.x + tid;
+  if (blockIdx.x == 0 && tid == 0) {
+    *a.free_count_out = (int32_t)(bad ? count : count - pg_total);
+    if (bad) report(a.status, a.status_host, kStatusNoPages);
+  }
+  for (int64_t i = first; i <= a.B; i += stride) {
+    a.query_starts[i] = bad ? 0 : tok[i];
+    if (i < a.B) a.seq_lens[i] = bad ? a.cached[i] : a.cached[i] + a.fresh[i];
+  }
+  if (bad) {
+    for (int64_t t = first; t < a.tokens; t += stride) {
+      a.slots[t] = -1;
+      a.positions[t] = 0;
+    }
+    return;
+  }
+  for (int64_t j = first; j < pg_total; j += stride) {
+    const int i = find_run(pgs, a.B, (int32_t)j);
+    a.table[i * a.table_stride + pages_of(a.cached[i], a.page) + (j - pgs[i])] = a.free_pages[count - 1 - j];
+  }
+  for (int64_t t = first; t < a.tokens; t += stride) {
+    int64_t slot = -1;
+    int32_t pos = 0;
+    if (t < tok_total) {
+      const int i = find_run(tok, a.B, (int32_t)t);
+      const int32_t c = a.cached[i];
+      pos = c + (int32_t)t - tok[i];
+      const int64_t held = pages_of(c, a.page), at = pos / a.page;
+      const int32_t id = at < held ? a.table[i * a.table_stride + at]
+                                   : a.free_pages[count - 1 - (pgs[i] + (at - held))];
+      if (id >= 0)
+        slot = (int64_t)id * a.page + (pos - at * a.page);
+      else
+        report(a.status, a.status_host, kStatusBadPage);
+    }
+    a.slots[t] = slot;
+    a.positions[t] = pos;
+  }
+}
+
+struct WriteArgs {
+  const uint16_t* kv;
+  int64_t T, kv_stride;
+  int latent, rope;
+  const uint16_t* weight;  // nullptr: stored unnormalised
+  float eps;
+  const int32_t* positions;  // nullptr: stored unrotated
+  const double* inv_freq;
+  int interleaved;
+  const int64_t* slots;
+  uint16_t* cache;
+  int64_t cache_rows;
+  const uint16_t* q;  // nullptr: no queries
+  int heads;
+  int64_t q_stride_t, q_stride_h;
+  uint16_t* q_out;
+  uint32_t* status;
+  uint32_t* status_host;
+};
+
+// cos and sin of position * inv_freq.  A position of 10^6 leaves a 32-bit
+// angle 0.06 rad off, so the turn count is formed and reduced in 64 bits and
+// only its fraction goes to 32.
+__device__ __forceinline__ float2 turn_of(int32_t position, double inv_freq) {
+  const double turns = (double)position * inv_freq * 0.15915494309189533577;  // 1 / (2 pi)
+  const float f = (float)(turns - rint(turns));
+  float s, c;
+  sincospif(2.0f * f, &s, &c);
+  return make_float2(c, s);
+}
+
+template <typename E>
+__device__ __forceinline__ void write_row(const WriteArgs& a, int64_t t, int lane, const float2* turns) {
+  const int64_t slot = a.slots[t];
+  if (slot < 0) return;
+  if (slot >= a.cache_rows) {
+    if (lane == 0) report(a.status, a.status_host, kStatusBadPage);
+    return;
+  }
+  const uint16_t* x = a.kv + t * a.kv_stride;
+  uint16_t* y = a.cache + slot * (a.latent + a.rope);
+  const int vecs = a.latent >> 3;
+  float f[4][8];
+  float sq = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int v = lane + 32 * i;
+    if (v < vecs) {
+      unpack8<E>(reinterpret_cast<const uint4*>(x)[v], f[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sq = fmaf(f[i][j], f[i][j], sq);
+    }
+  }
+  float r = 1.f;
+  if (a.weight) r = 1.0f / sqrtf(warp_sum(sq) / (float)a.latent + a.eps);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int v = lane + 32 * i;
+    if (v < vecs) {
+      if (a.weight) {
+        float w[8];
+        unpack8<E>(__ldg(reinterpret_cast<const uint4*>(a.weight) + v), w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[i][j] = f[i][j] * r * w[j];
+      }
+      reinterpret_cast<uint4*>(y)[v] = pack8<E>(f[i]);
+    }
+  }
+  const int half = a.rope >> 1;
+  for (int p = lane; p < half; p += 32) {
+    const int e0 = a.latent + (a.interleaved ? 2 * p : p), e1 = e0 + (a.interleaved ? 1 : half);
+    const float u = Elem<E>::to_float(x[e0]), w = Elem<E>::to_float(x[e1]);
+    if (a.positions) {
+      const float2 cs = turns ? turns[p] : turn_of(a.positions[t], a.inv_freq[p]);
+      y[e0] = Elem<E>::from_float(u * cs.x - w * cs.y);
+      y[e1] = Elem<E>::from_float(w * cs.x + u * cs.y);
+    } else {
+      y[e0] = x[e0];
+      y[e1] = x[e1];
+    }
+  }
+}
+
+// Without queries: a warp a token.  With queries: a block a token, the angles
+// computed once for all heads; the last warp stores the row.
+template <typename E, bool QUERIES>
+__global__ void __launch_bounds__(kWriteThreads) latent_write_kernel(WriteArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (!QUERIES) {
+    const int64_t t = (int64_t)blockIdx.x * (kWriteThreads / 32) + warp;
+    if (t < a.T) write_row<E>(a, t, lane, nullptr);
+  } else {
+    __shared__ float2 turns[kMaxRope / 2];
+    const int64_t t = blockIdx.x;
+    const int half = a.rope >> 1;
+    if (threadIdx.x < half) turns[threadIdx.x] = turn_of(a.positions[t], a.inv_freq[threadIdx.x]);
+    __syncthreads();
+    if (warp == kWriteThreads / 32 - 1) write_row<E>(a, t, lane, turns);
+    const int pieces = a.rope >> 4;  // pairs of 8-value pieces a head
+    for (int i = threadIdx.x; i < a.heads * pieces; i += kWriteThreads) {
+      const int h = i / pieces, v = i - h * pieces;
+      const uint16_t* src = a.q + t * a.q_stride_t + h * a.q_stride_h;
+      uint16_t* dst = a.q_out + (t * a.heads + h) * a.rope;
+      const int e0 = a.interleaved ? 16 * v : 8 * v, e1 = a.interleaved ? e0 + 8 : half + 8 * v;
+      float x[8], y[8];
+      unpack8<E>(*reinterpret_cast<const uint4*>(src + e0), x);
+      unpack8<E>(*reinterpret_cast<const uint4*>(src + e1), y);
+      if (a.interleaved) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 c0 = turns[8 * v + j], c1 = turns[8 * v + 4 + j];
+          const float u0 = x[2 * j], w0 = x[2 * j + 1], u1 = y[2 * j], w1 = y[2 * j + 1];
+          x[2 * j] = u0 * c0.x - w0 * c0.y;
+          x[2 * j + 1] = w0 * c0.x + u0 * c0.y;
+          y[2 * j] = u1 * c1.x - w1 * c1.y;
+          y[2 * j + 1] = w1 * c1.x + u1 * c1.y;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float2 cs = turns[8 * v + j];
+          const float u = x[j], w = y[j];
+          x[j] = u * cs.x - w * cs.y;
+          y[j] = w * cs.x + u * cs.y;
+        }
+      }
+      *reinterpret_cast<uint4*>(dst + e0) = pack8<E>(x);
+      *reinterpret_cast<uint4*>(dst + e1) = pack8<E>(y);
+    }
+  }
+}
+
+template <typename E>
+void launch_write(const WriteArgs& a, cudaStream_t st) {
+  if (a.q) {
+    latent_write_kernel<E, true><<<(unsigned)a.T, kWriteThreads, 0, st>>>(a);
+  } else {
+    const int64_t blocks = (a.T + kWriteThreads / 32 - 1) / (kWriteThreads / 32);
+    latent_write_kernel<E, false><<<(unsigned)blocks, kWriteThreads, 0, st>>>(a);
+  }
+}
+
+}  // namespace
+}  // namespace latent
+}  // namespace glm53
+
+using namespace glm53;
+using namespace glm53::latent;
+
+extern "C" int glm53_plan_pages(const int32_t* cached_lens, const int32_t* new_lens, int64_t requests,
+                                int32_t* block_table, int64_t table_stride, int64_t table_width,
+                                const int32_t* free_pages, int64_t free_capacity, const int32_t* free_count,
+                                int64_t page_size, int64_t tokens, int64_t* slots, int32_t* positions,
+                                int32_t* query_starts, int32_t* seq_lens, int32_t* free_count_out, uint32_t* status,
+                                uint32_t* status_host, void* stream) {
+  const char* fn = "glm53_plan_pages";
+  if (requests < 0 || requests > kPlanMaxRequests) {
+    set_last_error("%s: %lld requests are outside [0, %lld]", fn, (long long)requests, (long long)kPlanMaxRequests);
+    return GLM53_ERR_INVALID;
+  }
+  if (page_size < 1 || table_width < 0 || table_stride < table_width || free_capacity < 0 || tokens < 0 ||
+      page_size > INT32_MAX || table_width > INT32_MAX / page_size || tokens > INT32_MAX) {
+    set_last_error("%s: page size %lld, table width %lld, tokens %lld: sizes are non-negative and positions 32-bit", fn,
+                   (long long)page_size, (long long)table_width, (long long)tokens);
+    return GLM53_ERR_INVALID;
+  }
+  if (!query_starts || !free_count || !free_count_out || free_count == free_count_out ||
+      (requests && (!cached_lens || !new_lens || !seq_lens)) || (requests && table_width && !block_table) ||
+      (free_capacity && !free_pages) || (tokens && (!slots || !positions))) {
+    set_last_error("%s: missing tensor, or free_count_out is free_count", fn);
+    return GLM53_ERR_INVALID;
+  }
+  PlanArgs a{cached_lens, new_lens, (int)requests, block_table, table_stride, table_width, free_pages, free_capacity,
+             free_count, (int)page_size, tokens, slots, positions, query_starts, seq_lens, free_count_out, status,
+             status_host};
+  const size_t smem = 2 * (size_t)(requests + 1) * sizeof(int32_t);
+  const int rc = ensure_max_smem((const void*)plan_pages_kernel, 2 * (kPlanMaxRequests + 1) * sizeof(int32_t));
+  if (rc) return rc;
+  // one block a 1,024 tokens or requests, at most one an SM: each block repeats the scan
+  const int64_t items = std::max(tokens, requests);
+  const int64_t blocks = std::min<int64_t>(sm_count(), std::max<int64_t>(1, (items + 1023) / 1024));
+  plan_pages_kernel<<<(unsigned)blocks, kPlanThreads, smem, (cudaStream_t)stream>>>(a);
+  return check_launch(fn);
+}
+
+extern "C" int glm53_latent_cache_write(const void* kv, int64_t tokens, int64_t kv_stride, int64_t latent_dim,
+                                        int64_t rope_dim, int dtype, const void* norm_weight, float eps,
+                                        const int32_t* positions, const double* inv_freq, int interleaved,
+                                        const int64_t* slots, void* cache, int64_t cache_rows, const void* queries,
+                                        int64_t heads, int64_t q_stride_t, int64_t q_stride_h, void* queries_out,
+                                        uint32_t* status, uint32_t* status_host, void* stream) {
+  const char* fn = "glm53_latent_cache_write";
+  if (dtype != GLM53_DTYPE_BF16 && dtype != GLM53_DTYPE_FP16) {
+    set_last_error("%s: unknown element type %d", fn, dtype);
+    return GLM53_ERR_INVALID;
+  }
+  if (tokens < 0 || tokens > INT32_MAX || latent_dim <= 0 || latent_dim % 8 != 0 || latent_dim > kMaxLatent ||
+      rope_dim < 0 || rope_dim % 16 != 0 || rope_dim > kMaxRope || kv_stride < latent_dim + rope_dim ||
+      kv_stride % 8 != 0 || cache_rows < 0) {
+    set_last_error("%s: latent %lld (a multiple of 8, at most %lld), rotary %lld (a multiple of 16, at most %lld), row "
+                   "stride %lld (a multiple of 8)",
+                   fn, (long long)latent_dim, (long long)kMaxLatent, (long long)rope_dim, (long long)kMaxRope,
+                   (long long)kv_stride);
+    return GLM53_ERR_INVALID;
+  }
+  if ((positions != nullptr) != (inv_freq != nullptr) || (positions && rope_dim == 0)) {
+    set_last_error("%s: positions and inv_freq come together, with a rotary part", fn);
+    return GLM53_ERR_INVALID;
+  }
+  if (queries && (!positions || !queries_out || heads < 1 || heads > 4096 || q_stride_h < rope_dim ||
+                  q_stride_t < 0 || q_stride_h % 8 != 0 || q_stride_t % 8 != 0)) {
+    set_last_error("%s: queries need positions, an output, 1 to 4096 heads and strides that are multiples of 8", fn);
+    return GLM53_ERR_INVALID;
+  }
+  if (tokens == 0) return GLM53_OK;
+  if (!kv || !slots || !cache ||
+      (((uintptr_t)kv | (uintptr_t)cache | (uintptr_t)norm_weight | (uintptr_t)queries | (uintptr_t)queries_out) & 15)) {
+    set_last_error("%s: tensors must be non-NULL and 16-byte aligned", fn);
+    return GLM53_ERR_INVALID;
+  }
+  WriteArgs a{(const uint16_t*)kv, tokens, kv_stride, (int)latent_dim, (int)rope_dim, (const uint16_t*)norm_weight,
+              eps, positions, inv_freq, interleaved, slots, (uint16_t*)cache, cache_rows, (const uint16_t*)queries,
+              (int)heads, q_stride_t, q_stride_h, (uint16_t*)queries_out, status, status_host};
+  if (dtype == GLM53_DTYPE_BF16)
+    launch_write<__nv_bfloat16>(a, (cudaStream_t)stream);
+  else
+    launch_write<__half>(a, (cudaStream_t)stream);
+  return check_launch(fn);
+}

@@ -360,6 +360,10 @@ def _raise_status(word: int) -> None:
         raise IndexError("expert id out of range in routed MoE")
     if word & N.STATUS_WAIT_TIMEOUT:
         raise RuntimeError("a bounded device wait gave up")
+    if word & N.STATUS_BAD_PAGE:
+        raise IndexError("page id or slot outside the latent cache")
+    if word & N.STATUS_NO_PAGES:
+        raise RuntimeError("the page plan exceeds its free pages, block table or token capacity")
     if word:
         raise RuntimeError(f"device status 0x{word:x}")
 

@@ -37,6 +37,12 @@ extern "C" {
 #define GLM53_STATUS_BAD_EXPERT 1u
 #define GLM53_STATUS_WAIT_TIMEOUT 2u
 #define GLM53_STATUS_BAD_GEOMETRY 4u
+#define GLM53_STATUS_BAD_PAGE 8u  /* a page id or slot outside the cache */
+#define GLM53_STATUS_NO_PAGES 16u /* a page plan exceeds its free pages, table or token capacity */
+
+/* `dtype` of the latent-attention entry points. */
+#define GLM53_DTYPE_BF16 0
+#define GLM53_DTYPE_FP16 1
 
 /* `flags` bit: the caller guarantees that the E4M3 weights contain no code
  * 0x7F or 0xFF (true of every E4M3FN checkpoint, where those codes are NaN;
@@ -702,6 +708,91 @@ int glm53_hc_expand(const void* moe, const void* residual, const float* post,
  * NativePrefillDSAOutputPlan::execute (native_prefill_dsa_output_plan.cpp:68-106). */
 int glm53_head_major_to_rows(const void* head_major, int64_t heads, int64_t rows,
                              int64_t dim, void* row_major, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Latent attention over a paged cache
+ *
+ * A cache is `pages` pages of `page_size` rows; a row is one token's
+ * [latent_dim latent values | rope_dim rotary values], contiguous.  Row `slot`
+ * of the cache is row slot % page_size of page slot / page_size.  A request's
+ * block table row lists its pages in order.  `status_host`, where given, is a
+ * pinned (device-mapped) word that a kernel which sets a status bit also
+ * writes.  Strides count elements.
+ * --------------------------------------------------------------------- */
+
+/* Block tables and slot maps from request lengths, in one launch.
+ * cached_lens, new_lens int32 [requests] (at most 8192 requests): rows already
+ * in the cache and rows to come.  New pages are taken from the end of
+ * free_pages[0, *free_count) in request order and written into block_table
+ * (int32 [requests, table_width], rows table_stride apart); entries of pages
+ * already held are read, all others left as they were.
+ * Per token (capacity `tokens`): slots int64 and positions int32; behind the
+ * last token slot -1 and position 0.  Per request: query_starts int32
+ * [requests + 1] (prefix sums of new_lens) and seq_lens int32 [requests]
+ * (cached + new).  *free_count_out (another word than free_count) is what is
+ * left.  A plan that does not fit (too few free pages, a table row too short,
+ * more than `tokens` tokens, a negative length) sets GLM53_STATUS_NO_PAGES and
+ * plans nothing: the table is untouched, every slot -1, every start 0,
+ * seq_lens = cached_lens.  A negative page id sets GLM53_STATUS_BAD_PAGE and
+ * gives its tokens slot -1. */
+int glm53_plan_pages(const int32_t* cached_lens, const int32_t* new_lens, int64_t requests, int32_t* block_table,
+                     int64_t table_stride, int64_t table_width, const int32_t* free_pages, int64_t free_capacity,
+                     const int32_t* free_count, int64_t page_size, int64_t tokens, int64_t* slots,
+                     int32_t* positions, int32_t* query_starts, int32_t* seq_lens, int32_t* free_count_out,
+                     uint32_t* status, uint32_t* status_host, void* stream);
+
+/* Store one row a token: the latent part RMS-normalised with norm_weight
+ * (NULL: as given), the rotary part turned by position * inv_freq (NULL: as
+ * given; inv_freq is FP64 [rope_dim / 2], pairs (i, i + rope_dim / 2), or
+ * (2 i, 2 i + 1) when interleaved), computed in FP32 and rounded once.
+ * kv [tokens, latent_dim + rope_dim], rows kv_stride apart; slots int64: < 0
+ * skips the token, >= cache_rows sets GLM53_STATUS_BAD_PAGE and skips it.  Two
+ * tokens with one slot leave either row.  queries (optional)
+ * [tokens, heads, rope_dim]: turned likewise into queries_out (contiguous). */
+int glm53_latent_cache_write(const void* kv, int64_t tokens, int64_t kv_stride, int64_t latent_dim, int64_t rope_dim,
+                             int dtype, const void* norm_weight, float eps, const int32_t* positions,
+                             const double* inv_freq, int interleaved, const int64_t* slots, void* cache,
+                             int64_t cache_rows, const void* queries, int64_t heads, int64_t q_stride_t,
+                             int64_t q_stride_h, void* queries_out, uint32_t* status, uint32_t* status_host,
+                             void* stream);
+
+/* Absorbed form: q_latent [tokens, heads, latent_dim] and q_rope
+ * [tokens, heads, rope_dim] against the cached rows of each token's request;
+ * out [tokens, heads, latent_dim] and lse FP32 [tokens, heads] (natural log of
+ * the softmax denominator; NULL to skip), contiguous.  latent_dim 128, 256,
+ * 384 or 512; rope_dim 0 or 64; page_size a multiple of 8.  query_starts int32
+ * [requests + 1] gives each request's tokens (NULL: one each); the last of a
+ * request's tokens sees all seq_lens rows, each earlier one a row less.  A
+ * token that sees no row gives 0 and lse -inf.  Tokens behind
+ * query_starts[requests] are zeroed when fill_tail is set, else left as they
+ * were.  A page id outside the cache sets GLM53_STATUS_BAD_PAGE, a length
+ * outside the table GLM53_STATUS_BAD_GEOMETRY. */
+size_t glm53_latent_absorbed_workspace_bytes(int64_t tokens, int64_t heads, int64_t latent_dim);
+int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, int64_t ql_stride_h, const void* q_rope,
+                          int64_t qr_stride_t, int64_t qr_stride_h, int64_t tokens, int64_t heads,
+                          int64_t latent_dim, int64_t rope_dim, int dtype, const void* cache, int64_t pages,
+                          int64_t page_size, const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                          const int32_t* seq_lens, int64_t requests, const int32_t* query_starts, float scale,
+                          void* out, float* lse, int fill_tail, void* workspace, size_t workspace_bytes,
+                          uint32_t* status, uint32_t* status_host, void* stream);
+
+/* Expanded form: queries [q_nope_h | q_rope_h] against keys [k_nope_h | k_rope]
+ * and values v_h (k_rope [key_tokens, rope_dim] is shared by the heads).
+ * query_starts and key_starts int32 [requests + 1] bound each request's rows.
+ * causal: query j of nq sees keys 0 .. nk - nq + j.  out
+ * [query_tokens, heads, value_dim] (row-major, as the output projection reads
+ * it) and lse FP32 [query_tokens, heads], contiguous; rows that see no key and
+ * rows outside every request as in glm53_latent_absorbed.  nope_dim, value_dim
+ * multiples of 64, rope_dim 0 or 64, nope_dim + rope_dim and value_dim at most
+ * 256.  Starts outside the rows set GLM53_STATUS_BAD_GEOMETRY. */
+int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, int64_t qn_stride_h, const void* q_rope,
+                          int64_t qr_stride_t, int64_t qr_stride_h, const void* k_nope, int64_t kn_stride_t,
+                          int64_t kn_stride_h, const void* k_rope, int64_t kr_stride_t, const void* values,
+                          int64_t v_stride_t, int64_t v_stride_h, int64_t query_tokens, int64_t key_tokens,
+                          int64_t heads, int64_t nope_dim, int64_t rope_dim, int64_t value_dim, int dtype,
+                          const int32_t* query_starts, const int32_t* key_starts, int64_t requests, float scale,
+                          int causal, void* out, float* lse, int fill_tail, uint32_t* status, uint32_t* status_host,
+                          void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,745 @@
+"""Latent attention over a paged cache: page plans, row stores, the absorbed
+and the expanded form, against plain 64-bit implementations.
+
+Tolerances of the attention results (u = eps / 2 of the element type, the
+largest relative error of one rounding): the result is rounded once (u |o|);
+each softmax weight may be rounded once to the element type before it meets
+its value (u sum p |v|); a score s = scale q . k in FP32 is off by at most
+e = (d + 2) 2^-23 scale sum |q k| (d products, an addition that may truncate,
+two scalings), which changes a weight and the sum by a factor within e^(+-e)
+each, together 2 e sum p |v| (e < 0.01, doubled to cover the second order);
+exp2 and the remaining FP32 steps stay below 2^-18 sum p |v| (2^-22 for the
+exponential of an argument of up to 2^5, and a sum of n weights in 8 or more
+partial sums).  FP16 weights below 2^-14 keep an absolute step of 2^-24: half
+of it per key, where the largest weight is held as 1 or more; the result's own
+smallest step likewise.  Log-sums: e, the sum's error and one FP32 rounding."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+R, r = 512, 64
+
+
+# --- 64-bit forms ----------------------------------------------------------
+
+
+def plan64(cached, new, table, free, count, page, tokens):
+    table = [list(row) for row in table]
+    free = list(free[:count])
+    slots, positions, starts, lens = [], [], [0], []
+    for i, (c, n) in enumerate(zip(cached, new)):
+        held, want = -(-c // page), -(-(c + n) // page)
+        for k in range(held, want):
+            table[i][k] = free.pop()
+        for p in range(c, c + n):
+            slots.append(table[i][p // page] * page + p % page)
+            positions.append(p)
+        starts.append(starts[-1] + n)
+        lens.append(c + n)
+    pad = tokens - len(slots)
+    return table, slots + [-1] * pad, positions + [0] * pad, starts, lens, len(free)
+
+
+def attend64(q, k, v, visible, scale, dtype):
+    """(out, lse, tolerance, lse tolerance) of one head: q [n, d], k [m, d], v [m, dv], visible [n] keys each."""
+    u = torch.finfo(dtype).eps / 2
+    q, k, v = q.double(), k.double(), v.double()
+    n, m = q.shape[0], k.shape[0]
+    if m == 0:
+        z = torch.zeros((n, v.shape[1]), dtype=torch.float64, device=q.device)
+        return z, torch.full((n,), -math.inf, dtype=torch.float64, device=q.device), z, z[:, 0]
+    seen = torch.arange(m, device=q.device)[None, :] < visible[:, None]
+    # what is masked does not enter, whatever it holds
+    s = torch.empty((n, m), dtype=torch.float64, device=q.device)
+    vz = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    kz = torch.where(torch.isfinite(k), k, torch.zeros_like(k))
+    s = torch.where(seen, (q @ kz.T) * scale, torch.full_like(s, -math.inf))
+    lse = torch.logsumexp(s, -1)
+    p = torch.exp(s - torch.where(lse.isinf(), torch.zeros_like(lse), lse)[:, None])
+    out = p @ vz
+    mass = p @ vz.abs()
+    e = ((q.abs() @ kz.abs().T) * abs(scale) * seen).amax(-1) * (q.shape[1] + 2) * 2.0 ** -23
+    tol = u * out.abs() + (u + 4 * e[:, None] + 2.0 ** -18) * mass * (1 + u) + 1e-30
+    if dtype == torch.float16:
+        tol = tol + m * 2.0 ** -25 * vz.abs().amax() * p.amax(-1, keepdim=True) + 2.0 ** -25
+    return out, lse, tol, 2 * e + 2.0 ** -18 + lse.abs().nan_to_num(posinf=0) * 2.0 ** -22
+
+
+def check(got, lse, out64, lse64, tol, lse_tol):
+    err = (got.double() - out64).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{int(bad.sum())} values off, worst {float((err / tol).nan_to_num(nan=1e9).max()):.3f} x tolerance"
+    if lse is not None:
+        empty = lse64 == -math.inf
+        assert torch.equal(lse.double() == -math.inf, empty)
+        assert ((lse.double() - lse64).abs()[~empty] <= lse_tol[~empty]).all()
+
+
+# --- refusals (no device) --------------------------------------------------
+
+
+def lib():
+    from glm53_flash_mlx_b200 import _native as N
+
+    return N.load_library()
+
+
+ONE = 16  # a pointer that is only checked
+
+
+def plan_args(**kw):
+    a = dict(cached=ONE, new=ONE, B=2, table=ONE, stride=4, width=4, free=ONE, cap=8, count=ONE, page=16, tokens=4,
+             slots=ONE, pos=ONE, starts=ONE, lens=ONE, out=2 * ONE, status=None, host=None, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad", [dict(B=-1), dict(B=8193), dict(page=0), dict(width=5), dict(width=1 << 30, stride=1 << 30),
+                                 dict(tokens=-1), dict(tokens=1 << 31), dict(cap=-1), dict(out=ONE), dict(starts=None),
+                                 dict(slots=None), dict(free=None), dict(table=None)])
+def test_plan_refuses(bad):
+    assert lib().glm53_plan_pages(*plan_args(**bad)) == 1
+
+
+def write_args(**kw):
+    a = dict(kv=ONE, T=2, stride=576, R=512, r=64, dtype=0, w=ONE, eps=1e-6, pos=ONE, freq=ONE, inter=0, slots=ONE,
+             cache=ONE, rows=64, q=ONE, heads=4, qt=256, qh=64, qo=ONE, status=None, host=None, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=2), dict(T=-1), dict(R=12), dict(R=1032), dict(r=8), dict(r=272),
+                                 dict(stride=568), dict(stride=580), dict(pos=None), dict(freq=None),
+                                 dict(r=0, stride=512), dict(heads=0), dict(qh=63), dict(qt=4), dict(qo=None),
+                                 dict(pos=None, freq=None), dict(kv=8), dict(cache=24), dict(slots=None), dict(rows=-1)])
+def test_write_refuses(bad):
+    assert lib().glm53_latent_cache_write(*write_args(**bad)) == 1
+
+
+def absorbed_args(**kw):
+    a = dict(ql=ONE, qlt=512, qlh=512, qr=ONE, qrt=64, qrh=64, T=2, H=1, R=512, r=64, dtype=0, cache=ONE, pages=4,
+             page=16, table=ONE, stride=4, width=4, lens=ONE, B=2, starts=None, scale=1.0, out=ONE, lse=None, tail=0,
+             ws=ONE, wsb=1 << 40, status=None, host=None, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=-1), dict(R=64), dict(R=520), dict(R=640), dict(r=32), dict(H=0), dict(H=1025),
+                                 dict(T=-1), dict(T=3), dict(page=4), dict(page=12), dict(pages=1 << 28),
+                                 dict(width=5), dict(qlt=511), dict(qlh=504), dict(qrh=32), dict(scale=math.inf),
+                                 dict(scale=math.nan), dict(ql=None), dict(qr=None), dict(out=8), dict(cache=None),
+                                 dict(lens=None), dict(ws=None), dict(wsb=1)])
+def test_absorbed_refuses(bad):
+    assert lib().glm53_latent_absorbed(*absorbed_args(**bad)) == 1
+
+
+def expanded_args(**kw):
+    a = dict(qn=ONE, qnt=192, qnh=192, qr=ONE, qrt=64, qrh=64, kn=ONE, knt=192, knh=192, kr=ONE, krt=64, v=ONE, vt=256,
+             vh=256, Tq=2, Tk=2, H=1, dn=192, dr=64, dv=256, dtype=0, qs=ONE, ks=ONE, B=1, scale=1.0, causal=1, out=ONE,
+             lse=None, tail=0, status=None, host=None, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=3), dict(dn=0), dict(dn=96), dict(dn=256), dict(dr=16), dict(dv=32), dict(dv=320),
+                                 dict(Tq=-1), dict(Tk=-1), dict(H=0), dict(B=-1), dict(B=70000), dict(scale=math.nan),
+                                 dict(qnt=1), dict(knh=4), dict(vt=-8), dict(qn=None), dict(kr=None), dict(v=8),
+                                 dict(qs=None)])
+def test_expanded_refuses(bad):
+    assert lib().glm53_latent_expanded(*expanded_args(**bad)) == 1
+
+
+def test_python_refuses_before_the_device():
+    import glm53_flash_mlx_b200 as G
+
+    i32 = torch.int32
+    lens, table, free = torch.zeros(2, dtype=i32), torch.zeros((2, 4), dtype=i32), torch.zeros(8, dtype=i32)
+    one = torch.ones(1, dtype=i32)
+    for args in [(lens.long(), lens, table, free, one), (lens, lens[:1], table, free, one),
+                 (lens, lens, table[:1], free, one), (lens, lens, table.long(), free, one),
+                 (lens, lens, table.t().contiguous().t(), free, one), (lens, lens, table[:1].expand(2, 4), free, one),
+                 (lens, lens, table, free, lens)]:
+        with pytest.raises(ValueError):
+            G.plan_pages(*args, page_size=16, tokens=4)
+    with pytest.raises(ValueError):
+        G.plan_pages(lens, lens, table, free, one, page_size=0, tokens=4)
+    kv, cache = torch.zeros((2, 576), dtype=torch.bfloat16), torch.zeros((4, 16, 576), dtype=torch.bfloat16)
+    slots = torch.zeros(2, dtype=torch.int64)
+    for a, kw in [((kv.float(), cache, slots), {}), ((kv, cache.half(), slots), {}), ((kv, cache[..., :512], slots), {}),
+                  ((kv, cache, slots.int()), {}), ((kv, cache, slots[:1]), {}), ((kv, cache, slots), dict(rope_dim=576)),
+                  ((kv, cache, slots), dict(positions=lens)), ((kv, cache, slots), dict(queries=kv[:, None, :64])),
+                  ((kv, cache, slots), dict(norm_weight=kv[0, :64]))]:
+        with pytest.raises(ValueError):
+            G.latent_cache_write(*a, **kw)
+    q, qr = torch.zeros((2, 4, 512), dtype=torch.bfloat16), torch.zeros((2, 4, 64), dtype=torch.bfloat16)
+    for a, kw in [((q.float(), qr, cache, table, lens), {}), ((q, qr.half(), cache, table, lens), {}),
+                  ((q[..., :500], qr, cache, table, lens), {}), ((q, None, cache, table, lens), {}),
+                  ((q, qr, cache[:, :12], table, lens), {}), ((q[:1], qr[:1], cache, table, lens), {}),
+                  ((q, qr, cache, table.long(), lens), {}), ((q, qr, cache, table, lens), dict(query_starts=lens)),
+                  ((q, qr, cache, table[:1], lens), {})]:
+        with pytest.raises(ValueError):
+            G.latent_attention_absorbed(*a, scale=1.0, **kw)
+    kn, kr, v = q[..., :192], kv[:, :64], q[..., :256]
+    for a in [(kn.float(), qr, kn, kr, v, one, one), (kn, qr, kn, None, v, one, one), (kn, qr, kn[:1], kr, v, one, one),
+              (q[..., :256], qr, q[..., :256], kr, v, one, one), (kn, qr, kn, kr, q[..., :96], one, one),
+              (kn, qr, kn, kr, v, one, lens), (kn, qr, kn, kr, v, one.long(), one)]:
+        with pytest.raises(ValueError):
+            G.latent_attention_expanded(*a, scale=1.0)
+    if not torch.cuda.is_available():
+        with pytest.raises(RuntimeError, match="CUDA"):
+            G.plan_pages(lens, lens, table, free, one, page_size=16, tokens=4)
+
+
+# --- plan_pages ------------------------------------------------------------
+
+
+def make_plan_case(B, page, most, seed):
+    rng = np.random.default_rng(seed)
+    cached = rng.integers(0, most + 1, B)
+    new = rng.integers(0, most + 1, B)
+    width = int(-(-(2 * most) // page)) + 1
+    ids = rng.permutation(B * width + 7).astype(np.int32)
+    table = np.full((B, width), -1, np.int32)
+    n = 0
+    for i in range(B):
+        held = -(-int(cached[i]) // page)
+        table[i, :held] = ids[n:n + held]
+        n += held
+    return cached.tolist(), new.tolist(), table, ids[n:]
+
+
+def run_plan(cached, new, table, free, count, page, tokens, stride=None):
+    import glm53_flash_mlx_b200 as G
+
+    dev = "cuda"
+    i32 = torch.int32
+    B, width = table.shape
+    full = torch.full((B, stride or width), -7, dtype=i32, device=dev)
+    view = full[:, :width]
+    view.copy_(torch.from_numpy(table))
+    plan = G.plan_pages(torch.tensor(cached, dtype=i32, device=dev), torch.tensor(new, dtype=i32, device=dev), view,
+                        torch.from_numpy(np.asarray(free, np.int32)).to(dev), torch.tensor([count], dtype=i32, device=dev),
+                        page_size=page, tokens=tokens)
+    return plan, view, full
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,page,most,pad,stride", [(1, 16, 40, 0, None), (3, 1, 5, 4, 40), (7, 64, 200, 0, None),
+                                                    (300, 16, 90, 11, None), (8192, 32, 3, 1, None), (33, 48, 700, 0, 90)])
+def test_plan_matches(B, page, most, pad, stride):
+    cached, new, table, free = make_plan_case(B, page, most, B + page)
+    total = sum(new) + pad
+    want = plan64(cached, new, table, free, len(free), page, total)
+    plan, view, full = run_plan(cached, new, table, free, len(free), page, total, stride)
+    assert view.cpu().numpy().tolist() == [list(map(int, row)) for row in want[0]]
+    assert plan.slots.tolist() == list(map(int, want[1]))
+    assert plan.positions.tolist() == want[2]
+    assert plan.query_starts.tolist() == want[3]
+    assert plan.seq_lens.tolist() == want[4]
+    assert plan.free_count.tolist() == [want[5]]
+    if stride:
+        assert (full[:, table.shape[1]:] == -7).all()  # what lies behind the rows is left as it was
+
+
+@pytest.mark.gpu
+def test_plan_of_nothing():
+    plan, _, _ = run_plan([], [], np.zeros((0, 4), np.int32), [1, 2], 2, 16, 3)
+    assert plan.slots.tolist() == [-1] * 3 and plan.query_starts.tolist() == [0] and plan.free_count.tolist() == [2]
+    plan, _, _ = run_plan([5, 0], [0, 0], np.array([[3], [-1]], np.int32), [1], 1, 16, 0)
+    assert plan.seq_lens.tolist() == [5, 0] and plan.free_count.tolist() == [1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", ["pages", "tokens", "width", "negative", "count"])
+def test_plan_that_does_not_fit_plans_nothing(case):
+    import glm53_flash_mlx_b200 as G
+
+    cached, new, table, free = make_plan_case(9, 16, 60, 5)
+    new[4] = 60
+    count, tokens = len(free), sum(new)
+    if case == "pages":
+        count = 2
+    elif case == "tokens":
+        tokens -= 1
+    elif case == "width":
+        new[3] = 16 * table.shape[1] - cached[3] + 1
+        tokens = sum(new)
+    elif case == "negative":
+        new[2] = -1
+    else:
+        count = len(free) + 1
+    plan, view, _ = run_plan(cached, new, table, free, count, 16, tokens)
+    with pytest.raises(RuntimeError, match="page plan"):
+        G.check_latent_status()
+    assert np.array_equal(view.cpu().numpy(), table)
+    assert (plan.slots == -1).all() and (plan.positions == 0).all() and (plan.query_starts == 0).all()
+    assert plan.seq_lens.tolist() == cached and plan.free_count.tolist() == [count]
+    G.check_latent_status()  # raised once
+
+
+# --- latent_cache_write ----------------------------------------------------
+
+
+def write64(kv, slots, w, pos, freq, interleaved, eps, latent):
+    x = kv.double().clone()
+    if w is not None:
+        x[:, :latent] = x[:, :latent] / (x[:, :latent].pow(2).mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    if pos is not None:
+        x[:, latent:] = turn64(x[:, latent:], pos, freq, interleaved)
+    return x
+
+
+def turn64(x, pos, freq, interleaved):
+    x = x.double()
+    ang = pos.double().view(-1, *[1] * (x.dim() - 1)) * freq
+    c, s = ang.cos(), ang.sin()
+    if interleaved:
+        a, b = x[..., 0::2], x[..., 1::2]
+        return torch.stack([a * c - b * s, b * c + a * s], -1).flatten(-2)
+    a, b = x.chunk(2, -1)
+    return torch.cat([a * c - b * s, b * c + a * s], -1)
+
+
+def rounded_close(got, want, scale):
+    """One rounding of the result, and FP32 steps relative to the values that were combined."""
+    fi = torch.finfo(got.dtype)
+    tol = fi.eps / 2 * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -19 * scale + fi.tiny * fi.eps / 2
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,latent,rope,heads,norm,interleaved,page", [
+    (1, 512, 64, 64, True, False, 64), (9, 512, 64, 5, True, True, 16), (130, 512, 64, 0, True, False, 48),
+    (17, 8, 16, 1, True, False, 3), (33, 1024, 256, 3, False, True, 16), (8, 512, 0, 0, True, False, 16),
+    (5, 256, 64, 0, False, False, 16)])
+def test_write_matches(dtype, T, latent, rope, heads, norm, interleaved, page):
+    import glm53_flash_mlx_b200 as G
+
+    dev = "cuda"
+    g = torch.Generator(device=dev).manual_seed(T + latent)
+    pages = -(-T // page) + 2
+    wide = torch.randn((T, latent + rope + 8), generator=g, device=dev).to(dtype)
+    kv = wide[:, :latent + rope]  # strided rows
+    cache = torch.randn((pages, page, latent + rope), generator=g, device=dev).to(dtype)
+    before = cache.clone()
+    slots = torch.randperm(pages * page, generator=g, device=dev)[:T]
+    if T > 4:
+        slots[T // 2] = -1
+    w = (1 + 0.2 * torch.randn(latent, generator=g, device=dev)).to(dtype) if norm else None
+    pos = freq = q = None
+    if rope:
+        pos = torch.randint(0, 1 << 20, (T,), generator=g, device=dev, dtype=torch.int32)
+        freq = 10000.0 ** (-torch.arange(0, rope, 2, device=dev, dtype=torch.float64) / rope)
+        if heads:
+            q = torch.randn((T, heads, rope + 24), generator=g, device=dev).to(dtype)[..., 8:8 + rope]
+    got = G.latent_cache_write(kv, cache, slots, rope_dim=rope, norm_weight=w, eps=1e-5, positions=pos, inv_freq=freq,
+                               interleaved=interleaved, queries=q)
+    G.check_latent_status()
+    want = write64(kv, slots, w, pos, freq, interleaved, 1e-5, latent)
+    flat, old = cache.view(-1, latent + rope), before.view(-1, latent + rope)
+    stored = slots[slots >= 0]
+    rounded_close(flat[stored], want[slots >= 0], 8.0)
+    kept = torch.ones(pages * page, dtype=torch.bool, device=dev)
+    kept[stored] = False
+    assert torch.equal(flat[kept], old[kept])
+    if heads:
+        rounded_close(got, turn64(q, pos, freq, interleaved), 8.0)
+    else:
+        assert got is None
+
+
+@pytest.mark.gpu
+def test_write_reports_a_slot_outside_the_cache():
+    import glm53_flash_mlx_b200 as G
+
+    kv = torch.ones((3, 576), dtype=torch.bfloat16, device="cuda")
+    cache = torch.zeros((2, 16, 576), dtype=torch.bfloat16, device="cuda")
+    G.latent_cache_write(kv, cache, torch.tensor([1, 32, 1 << 40], device="cuda"))
+    with pytest.raises(IndexError, match="slot"):
+        G.check_latent_status()
+    assert (cache.view(32, 576)[1] == 1).all() and cache.float().sum() == 576
+
+
+# --- absorbed form ---------------------------------------------------------
+
+
+def make_absorbed(lens, queries, H, latent, rope, page, dtype, seed=0, strided=False):
+    dev = "cuda"
+    g = torch.Generator(device=dev).manual_seed(seed)
+    B = len(lens)
+    width = max(1, max(-(-n // page) for n in lens))
+    pages = B * width + 3
+    # pages that no request holds, and rows behind a request's end, hold NaN and infinities
+    cache = torch.full((pages, page, latent + rope), float("nan"), dtype=dtype, device=dev)
+    cache[:, 1::2] = float("inf")
+    table = torch.full((B, width + 2), -1, dtype=torch.int32, device=dev)
+    ids = torch.randperm(pages, generator=g, device=dev)
+    rows = []
+    for i, n in enumerate(lens):
+        held = -(-n // page)
+        own = ids[i * width:i * width + held]
+        table[i, :held] = own.int()
+        x = torch.randn((n, latent + rope), generator=g, device=dev).to(dtype)
+        at = torch.arange(n, device=dev)
+        if n:
+            cache.view(-1, latent + rope)[own[at // page] * page + at % page] = x
+        rows.append(x)
+    T = sum(queries)
+    if strided:
+        q = torch.randn((T, H, latent + rope + 8), generator=g, device=dev).to(dtype)
+        ql, qr = q[..., :latent], q[..., latent:latent + rope]
+    else:
+        ql = torch.randn((T, H, latent), generator=g, device=dev).to(dtype)
+        qr = torch.randn((T, H, rope), generator=g, device=dev).to(dtype)
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(queries)]), dtype=torch.int32, device=dev)
+    return ql, (qr if rope else None), cache, table, torch.tensor(lens, dtype=torch.int32, device=dev), starts, rows
+
+
+def absorbed64(ql, qr, rows, lens, queries, scale, dtype):
+    T, H, latent = ql.shape
+    out, lse = torch.zeros((T, H, latent), dtype=torch.float64, device=ql.device), None
+    tol = torch.zeros_like(out)
+    lse = torch.zeros((T, H), dtype=torch.float64, device=ql.device)
+    ltol = torch.zeros_like(lse)
+    t = 0
+    for n, nq, x in zip(lens, queries, rows):
+        for j in range(nq):
+            seen = max(0, n - (nq - 1 - j))
+            q = ql[t] if qr is None else torch.cat([ql[t], qr[t]], -1)
+            vis = torch.full((H,), seen, device=ql.device)
+            out[t], lse[t], tol[t], ltol[t] = attend64(q, x[:seen], x[:seen, :latent], vis, scale, dtype)
+            t += 1
+    return out, lse, tol, ltol
+
+
+ABSORBED = [
+    # lens, queries, heads, latent, rope, page, strided
+    ([777], [1], 64, 512, 64, 64, False),
+    ([1], [1], 64, 512, 64, 16, False),
+    ([0, 5, 0], [1, 1, 1], 64, 512, 64, 16, False),
+    ([63, 64, 65, 127, 128, 129], [1] * 6, 64, 512, 64, 64, True),
+    ([300, 17, 0, 2], [2, 3, 2, 4], 16, 512, 64, 16, False),
+    ([40, 1000], [0, 5], 5, 512, 64, 8, True),
+    ([500, 33], [1, 1], 1, 128, 64, 48, False),
+    ([500, 33], [1, 1], 65, 256, 0, 128, False),
+    ([200], [1], 130, 384, 64, 32, False),
+    ([9000], [1], 64, 512, 64, 64, False),
+    ([2500] * 3 + [1, 0, 70], [1] * 6, 32, 512, 0, 16, False),
+    (list(range(0, 400)), [1] * 400, 8, 128, 64, 16, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", range(len(ABSORBED)))
+def test_absorbed_matches(dtype, case):
+    import glm53_flash_mlx_b200 as G
+
+    lens, queries, H, latent, rope, page, strided = ABSORBED[case]
+    ql, qr, cache, table, n, starts, rows = make_absorbed(lens, queries, H, latent, rope, page, dtype, case, strided)
+    scale = (latent + rope) ** -0.5 * 1.5
+    one_each = all(q == 1 for q in queries)
+    out, lse = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=scale,
+                                           query_starts=None if one_each else starts, return_lse=True)
+    G.check_latent_status()
+    check(out, lse, *absorbed64(ql, qr, rows, lens, queries, scale, dtype))
+    again = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=scale, query_starts=starts)
+    assert torch.equal(again, out)  # same bits from call to call, with and without lse
+
+
+@pytest.mark.gpu
+def test_absorbed_scores_that_grow():
+    """Scores that rise along the keys, so that the running maximum is replaced again and again, and a
+    negative scale."""
+    import glm53_flash_mlx_b200 as G
+
+    lens, queries, H = [1500, 700], [1, 1], 64
+    for sign in (1.0, -1.0):
+        ql, qr, cache, table, n, starts, rows = make_absorbed(lens, queries, H, 512, 64, 64, torch.bfloat16, 3)
+        ql.fill_(0.25)
+        for i, m in enumerate(lens):
+            ramp = (torch.arange(m, device="cuda") / m * 4).to(torch.bfloat16)
+            rows[i][:, :128] = ramp[:, None] * sign
+            at = torch.arange(m, device="cuda")
+            cache.view(-1, 576)[table[i].long()[at // 64] * 64 + at % 64] = rows[i]
+        out, lse = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.5 * sign, return_lse=True)
+        check(out, lse, *absorbed64(ql, qr, rows, lens, queries, 0.5 * sign, torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_absorbed_padded_batch_keeps_or_zeroes_the_rest():
+    import glm53_flash_mlx_b200 as G
+
+    lens, queries = [100, 30], [2, 1]
+    ql, qr, cache, table, n, starts, rows = make_absorbed(lens, queries, 16, 512, 64, 16, torch.bfloat16, 9)
+    pad = lambda x: torch.cat([x, torch.full((4, *x.shape[1:]), float("nan"), dtype=x.dtype, device="cuda")])
+    new, lse = G.latent_attention_absorbed(pad(ql), pad(qr), cache, table, n, scale=0.05, query_starts=starts,
+                                           return_lse=True)
+    want = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05, query_starts=starts)
+    assert torch.equal(new[:3], want) and (new[3:] == 0).all() and (lse[3:] == -math.inf).all()
+    given = torch.full_like(new, 7.0)
+    got = G.latent_attention_absorbed(pad(ql), pad(qr), cache, table, n, scale=0.05, query_starts=starts, out=given)
+    assert got is given and torch.equal(given[:3], want) and (given[3:] == 7).all()
+    G.check_latent_status()
+
+
+@pytest.mark.gpu
+def test_absorbed_reports_bad_pages_and_lengths():
+    import glm53_flash_mlx_b200 as G
+
+    lens = [100, 30]
+    ql, qr, cache, table, n, starts, rows = make_absorbed(lens, [1, 1], 16, 512, 64, 16, torch.bfloat16, 9)
+    want = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05)
+    for bad in (-1, cache.shape[0], 2 ** 31 - 1, -2 ** 31):
+        t2 = table.clone()
+        t2[1, 1] = bad
+        got = G.latent_attention_absorbed(ql, qr, cache, t2, n, scale=0.05)
+        with pytest.raises(IndexError, match="page"):
+            G.check_latent_status()
+        assert torch.equal(got[0], want[0])  # the other request is not touched by it
+    for bad in (-1, 16 * table.shape[1] + 1):
+        n2 = n.clone()
+        n2[1] = bad
+        got = G.latent_attention_absorbed(ql, qr, cache, table, n2, scale=0.05)
+        with pytest.raises(RuntimeError):
+            G.check_latent_status()
+        assert torch.equal(got[0], want[0]) and (got[1] == 0).all()
+
+
+# --- expanded form ---------------------------------------------------------
+
+
+def make_expanded(nq, nk, H, dn, dr, dv, dtype, seed=0):
+    dev = "cuda"
+    g = torch.Generator(device=dev).manual_seed(seed)
+    Tq, Tk = sum(nq), sum(nk)
+    q = torch.randn((Tq, H, dn + dr), generator=g, device=dev).to(dtype)
+    kv = torch.randn((Tk, H, dn + dv), generator=g, device=dev).to(dtype)
+    latent = torch.randn((Tk, 512 + dr), generator=g, device=dev).to(dtype)
+    qs = torch.tensor(np.concatenate([[0], np.cumsum(nq)]), dtype=torch.int32, device=dev)
+    ks = torch.tensor(np.concatenate([[0], np.cumsum(nk)]), dtype=torch.int32, device=dev)
+    qr, kr = (q[..., dn:], latent[:, 512:]) if dr else (None, None)
+    return q[..., :dn], qr, kv[..., :dn], kr, kv[..., dn:], qs, ks
+
+
+def expanded64(qn, qr, kn, kr, v, nq, nk, scale, causal, dtype):
+    Tq, H, dn = qn.shape
+    dv = v.shape[2]
+    out = torch.zeros((Tq, H, dv), dtype=torch.float64, device=qn.device)
+    tol, lse = torch.zeros_like(out), torch.zeros((Tq, H), dtype=torch.float64, device=qn.device)
+    ltol = torch.zeros_like(lse)
+    qa = ka = 0
+    for a, b in zip(nq, nk):
+        vis = torch.arange(a, device=qn.device) + (b - a) + 1 if causal else torch.full((a,), b, device=qn.device)
+        vis = vis.clamp(0, b)
+        for h in range(H if a else 0):
+            q, k = qn[qa:qa + a, h], kn[ka:ka + b, h]
+            if qr is not None:
+                q, k = torch.cat([q, qr[qa:qa + a, h]], -1), torch.cat([k, kr[ka:ka + b]], -1)
+            s = slice(qa, qa + a)
+            out[s, h], lse[s, h], tol[s, h], ltol[s, h] = attend64(q, k, v[ka:ka + b, h], vis, scale, dtype)
+        qa, ka = qa + a, ka + b
+    return out, lse, tol, ltol
+
+
+EXPANDED = [
+    # queries, keys, heads, nope, rope, value, causal
+    ([256], [256], 4, 192, 64, 256, True),
+    ([1], [1], 3, 192, 64, 256, True),
+    ([1], [1000], 2, 192, 64, 256, True),
+    ([129, 1, 0, 127, 128], [129, 640, 5, 300, 128], 2, 128, 64, 128, True),
+    ([300], [300], 2, 64, 0, 64, True),
+    ([200, 40], [500, 0], 1, 192, 64, 192, False),
+    ([130, 20], [50, 7], 2, 64, 64, 256, True),   # fewer keys than queries: the first rows see none
+    ([513], [1100], 1, 256, 0, 256, True),
+    ([3] * 40, list(range(3, 43)), 1, 128, 64, 64, True),
+    ([700], [700], 1, 192, 64, 256, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", range(len(EXPANDED)))
+def test_expanded_matches(dtype, case):
+    import glm53_flash_mlx_b200 as G
+
+    nq, nk, H, dn, dr, dv, causal = EXPANDED[case]
+    t = make_expanded(nq, nk, H, dn, dr, dv, dtype, case)
+    scale = (dn + dr) ** -0.5 * 1.5
+    out, lse = G.latent_attention_expanded(*t, scale=scale, causal=causal, return_lse=True)
+    G.check_latent_status()
+    check(out, lse, *expanded64(*t[:5], nq, nk, scale, causal, dtype))
+    assert torch.equal(G.latent_attention_expanded(*t, scale=scale, causal=causal), out)
+
+
+@pytest.mark.gpu
+def test_expanded_scores_that_grow():
+    import glm53_flash_mlx_b200 as G
+
+    nq, nk = [260], [900]
+    qn, qr, kn, kr, v, qs, ks = make_expanded(nq, nk, 2, 192, 64, 256, torch.bfloat16, 4)
+    qn = torch.full_like(qn, 0.25)
+    kn = kn.clone()
+    kn[..., :64] = (torch.arange(900, device="cuda") / 900 * 8).to(torch.bfloat16)[:, None, None]
+    out, lse = G.latent_attention_expanded(qn, qr, kn, kr, v, qs, ks, scale=0.5, return_lse=True)
+    check(out, lse, *expanded64(qn, qr, kn, kr, v, nq, nk, 0.5, True, torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_expanded_masked_keys_and_values_do_not_enter(what):
+    """A request's rows that are not finite stay out of the requests beside it and of the rows that do not
+    see them; the rows that see them get them."""
+    import glm53_flash_mlx_b200 as G
+
+    nq, nk = [70, 100, 90], [70, 180, 90]
+    qn, qr, kn, kr, v, qs, ks = make_expanded(nq, nk, 2, 192, 64, 256, torch.bfloat16, 6)
+    kn, v, kr = kn.clone(), v.clone(), kr.clone()
+    clean = G.latent_attention_expanded(qn, qr, kn, kr, v, qs, ks, scale=0.06)
+    v[70 + 150, 0, 5] = what    # seen by queries 70.. of the second request
+    v[70 + 151, 1, 200] = what
+    kn[70 + 160, :, 3] = math.nan  # seen by queries 80..
+    got = G.latent_attention_expanded(qn, qr, kn, kr, v, qs, ks, scale=0.06)
+    G.check_latent_status()
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[70 + 70:170, 0, 5] = True
+    hit[70 + 71:170, 1, 200] = True
+    lost = torch.zeros_like(hit)
+    lost[70 + 80:170] = True
+    assert got[lost].isnan().all()
+    if math.isnan(what):
+        assert got[hit & ~lost].isnan().all()
+    else:
+        assert (got[hit & ~lost] == math.inf).all()
+    assert torch.equal(got[~hit & ~lost], clean[~hit & ~lost])
+
+
+@pytest.mark.gpu
+def test_expanded_rows_outside_every_request():
+    import glm53_flash_mlx_b200 as G
+
+    nq, nk = [40, 30], [60, 30]
+    t = make_expanded(nq, nk, 3, 128, 64, 128, torch.bfloat16, 8)
+    want = G.latent_attention_expanded(*t, scale=0.07)
+    more = lambda x: torch.cat([x, torch.full((5, *x.shape[1:]), math.nan, dtype=x.dtype, device="cuda")])
+    q = (more(t[0]), more(t[1]))
+    new, lse = G.latent_attention_expanded(*q, *t[2:], scale=0.07, return_lse=True)
+    assert torch.equal(new[:70], want) and (new[70:] == 0).all() and (lse[70:] == -math.inf).all()
+    given = torch.full_like(new, 3.0)
+    G.latent_attention_expanded(*q, *t[2:], scale=0.07, out=given)
+    assert torch.equal(given[:70], want) and (given[70:] == 3).all()
+    bad = t[6].clone()
+    bad[2] = 91  # past the keys
+    got = G.latent_attention_expanded(*t[:6], bad, scale=0.07)
+    with pytest.raises(RuntimeError):
+        G.check_latent_status()
+    assert torch.equal(got[:40], want[:40]) and (got[40:] == 0).all()
+
+
+# --- streams, graphs, together ---------------------------------------------
+
+
+@pytest.mark.gpu
+def test_two_graphs_and_a_side_stream():
+    """Two captured decodes and an eager one on another stream share nothing: each replay gives its own
+    result, with lengths that changed after the capture."""
+    import glm53_flash_mlx_b200 as G
+
+    cases = [make_absorbed([900, 40], [1, 1], 64, 512, 64, 64, torch.bfloat16, s) for s in (1, 2)]
+    G.latent_attention_absorbed(*cases[0][:5], scale=0.05)
+    graphs, outs = [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(G.latent_attention_absorbed(*c[:5], scale=0.05))
+        graphs.append(g)
+    for c in cases:
+        c[4].copy_(torch.tensor([333, 12], dtype=torch.int32))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+        with torch.cuda.stream(side):
+            third = G.latent_attention_absorbed(*cases[0][:5], scale=0.05)
+    torch.cuda.synchronize()
+    for c, o in zip(cases, outs):
+        check(o, None, *absorbed64(c[0], c[1], [x[:n] for x, n in zip(c[6], (333, 12))], [333, 12], [1, 1], 0.05,
+                                   torch.bfloat16))
+    assert torch.equal(third, outs[0])
+
+
+@pytest.mark.gpu
+def test_a_prompt_and_its_decode_together():
+    """Plan, store, expand and attend a ragged prompt batch, then decode a token each: both forms give the
+    layer's attention, and the output projection reads the result."""
+    import glm53_flash_mlx_b200 as G
+    from glm53_flash_mlx_b200 import synthetic as S
+
+    dev, dt = torch.device("cuda", torch.cuda.current_device()), torch.bfloat16
+    g = torch.Generator(device=dev).manual_seed(11)
+    H, dn, dv, page = 4, 192, 256, 16
+    prompts = [37, 5, 64]
+    i32 = dict(dtype=torch.int32, device=dev)
+    table = torch.full((3, 8), -1, **i32)
+    free = torch.randperm(20, generator=g, device=dev).int()
+    cache = torch.full((20, page, 576), math.nan, dtype=dt, device=dev)
+    w = (1 + 0.1 * torch.randn(R, generator=g, device=dev)).to(dt)
+    freq = 10000.0 ** (-torch.arange(0, r, 2, device=dev, dtype=torch.float64) / r)
+    kvb, kvb_s = S.random_block_fp8(H * (dn + dv), R, seed=5, device=dev)
+    ow, os_ = S.random_block_fp8(256, H * dv, seed=6, device=dev)
+    scale = (dn + r) ** -0.5
+
+    T = sum(prompts)
+    zeros, count = torch.zeros(3, **i32), torch.tensor([20], **i32)
+    plan = G.plan_pages(zeros, torch.tensor(prompts, **i32), table, free, count, page_size=page, tokens=T)
+    kv = torch.randn((T, 576), generator=g, device=dev).to(dt)
+    q = torch.randn((T, H, dn + r), generator=g, device=dev).to(dt)
+    q_rope = G.latent_cache_write(kv, cache, plan.slots, norm_weight=w, positions=plan.positions, inv_freq=freq,
+                                  queries=q[..., dn:])
+    rows = cache.view(-1, 576)[plan.slots]
+    up = G.block_fp8_linear(rows[:, :R].contiguous(), kvb, kvb_s).view(T, H, dn + dv)
+    out = G.latent_attention_expanded(q[..., :dn], q_rope, up[..., :dn], rows[:, R:], up[..., dn:], plan.query_starts,
+                                      plan.query_starts, scale=scale)
+    check(out, None, *expanded64(q[..., :dn], q_rope, up[..., :dn], rows[:, R:], up[..., dn:], prompts, prompts, scale,
+                                 True, dt))
+    projected = G.block_fp8_linear(out.view(T, H * dv), ow, os_)
+    head_major = out.transpose(0, 1).contiguous()
+    assert torch.equal(projected, G.DSAOutputProjection().execute(head_major, ow, os_))
+
+    # one more token each
+    kv1 = torch.randn((3, 576), generator=g, device=dev).to(dt)
+    q1 = torch.randn((3, H, dn + r), generator=g, device=dev).to(dt)
+    step = G.plan_pages(plan.seq_lens, torch.ones(3, **i32), table, free, plan.free_count, page_size=page, tokens=3)
+    qr1 = G.latent_cache_write(kv1, cache, step.slots, norm_weight=w, positions=step.positions, inv_freq=freq,
+                               queries=q1[..., dn:])
+    blocks = kvb.view(torch.float8_e4m3fn).float() * kvb_s.repeat_interleave(128, 0)[: kvb.shape[0]].repeat_interleave(
+        128, 1)[:, :R]
+    up_w = blocks.view(H, dn + dv, R)
+    q_latent = torch.einsum("thd,hdr->thr", q1[..., :dn].float(), up_w[:, :dn]).to(dt)
+    o = G.latent_attention_absorbed(q_latent, qr1, cache, table, step.seq_lens, scale=scale)
+    G.check_latent_status()
+    all_rows = [torch.cat([rows[a:b], cache.view(-1, 576)[step.slots[i:i + 1]]]) for i, (a, b) in
+                enumerate(zip([0, 37, 42], [37, 42, 106]))]
+    check(o, None, *absorbed64(q_latent, qr1, all_rows, [n + 1 for n in prompts], [1, 1, 1], scale, dt))
+    # the expanded form of the same step: the two differ by the roundings of q_latent, the expanded keys
+    # and values, both results and the values that the weights meet: at most eight roundings of 2^-8 each, a
+    # relative error below 2^-5, so a cosine above 1 - 2^-10 / 2 > 0.999
+    lens = [n + 1 for n in prompts]
+    flat = torch.cat(all_rows)
+    up1 = G.block_fp8_linear(flat[:, :R].contiguous(), kvb, kvb_s).view(-1, H, dn + dv)
+    ks = torch.tensor([0, *np.cumsum(lens)], **i32)
+    e = G.latent_attention_expanded(q1[..., :dn], qr1, up1[..., :dn], flat[:, R:], up1[..., dn:],
+                                    torch.arange(4, **i32), ks, scale=scale)
+    a = torch.einsum("thr,hdr->thd", o.float(), up_w[:, dn:])
+    cos = torch.nn.functional.cosine_similarity(a.flatten(1).double(), e.flatten(1).double(), dim=-1)
+    assert (cos > 0.999).all(), cos
