@@ -79,5 +79,33 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
                     Elem<E>::pack(f[6], f[7]));
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// True in every thread of `threads` when `p` holds in any of them (named barrier `id`).
+__device__ __forceinline__ bool any_of(bool p, int id, int threads) {
+  uint32_t r;
+  asm volatile(
+      "{ .reg .pred a, b; setp.ne.u32 a, %1, 0; barrier.cta.red.or.pred b, %2, %3, a; selp.u32 %0, 1, 0, b; }"
+      : "=r"(r)
+      : "r"((uint32_t)p), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Running maxima are replaced (and results rescaled) only when a score passes
+// the one in use by this much, in powers of two: weights stay below 2^8, which
+// every type here holds, and most tiles rescale nothing.
+constexpr float kMaxSlack = 8.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
 }  // namespace latent
 }  // namespace glm53

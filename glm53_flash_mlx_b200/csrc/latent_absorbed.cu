@@ -165,49 +165,6 @@ __global__ void __launch_bounds__(kThreads) absorbed_kernel(AbsorbedArgs a) {
             });
 }
 
-struct ExpandedArgs {
-  const uint16_t *qn, *qr, *kn, *kr, *v;
-  int64_t qn_t, qn_h, qr_t, qr_h, kn_t, kn_h, kr_t, v_t, v_h;
-  int64_t Tq, Tk;
-  int H, dn, dr, dv;
-  const int32_t *q_starts, *k_starts;
-  int B;
-  float scale;
-  int causal;
-  uint16_t* out;
-  float* lse;
-  int fill_tail;
-  uint32_t *status, *status_host;
-};
-
-template <typename E>
-__global__ void __launch_bounds__(kThreads) expanded_kernel(ExpandedArgs a) {
-  __shared__ Joined sm;
-  const int t = blockIdx.x, h = blockIdx.y;
-  const bool tail = a.B == 0 || t < a.q_starts[0] || t >= a.q_starts[a.B];
-  if (tail && !a.fill_tail) return;
-  int64_t visible = 0, k0 = 0;
-  if (!tail) {
-    const int i = request_of(a.q_starts, a.B, t);
-    const int64_t nq = (int64_t)a.q_starts[i + 1] - a.q_starts[i];
-    k0 = a.k_starts[i];
-    const int64_t k1 = a.k_starts[i + 1];
-    if (k0 < 0 || k1 < k0 || k1 > a.Tk || t >= a.q_starts[i + 1]) {
-      if (threadIdx.x == 0) report(a.status, a.status_host, kStatusBadGeometry);
-    } else {
-      visible = a.causal ? (k1 - k0) - nq + (t - a.q_starts[i]) + 1 : k1 - k0;
-    }
-  }
-  attend<E>(sm, a.qn + t * a.qn_t + h * a.qn_h, a.dn, a.qr + t * a.qr_t + h * a.qr_h, a.dr, a.dv,
-            visible > 0 ? visible : 0, a.scale, a.out + ((int64_t)t * a.H + h) * a.dv,
-            a.lse ? a.lse + (int64_t)t * a.H + h : nullptr,
-            [&](int64_t j, const uint16_t*& ka, const uint16_t*& kb, const uint16_t*& kv) {
-              ka = a.kn + (k0 + j) * a.kn_t + h * a.kn_h;
-              kb = a.kr + (k0 + j) * a.kr_t;
-              kv = a.v + (k0 + j) * a.v_t + h * a.v_h;
-            });
-}
-
 bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s < (int64_t)1 << 38; }
 
 }  // namespace
@@ -280,58 +237,5 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
     absorbed_kernel<__nv_bfloat16><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
   else
     absorbed_kernel<__half><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
-  return check_launch(fn);
-}
-
-extern "C" int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, int64_t qn_stride_h, const void* q_rope,
-                                     int64_t qr_stride_t, int64_t qr_stride_h, const void* k_nope, int64_t kn_stride_t,
-                                     int64_t kn_stride_h, const void* k_rope, int64_t kr_stride_t, const void* values,
-                                     int64_t v_stride_t, int64_t v_stride_h, int64_t query_tokens, int64_t key_tokens,
-                                     int64_t heads, int64_t nope_dim, int64_t rope_dim, int64_t value_dim, int dtype,
-                                     const int32_t* query_starts, const int32_t* key_starts, int64_t requests,
-                                     float scale, int causal, void* out, float* lse, int fill_tail, uint32_t* status,
-                                     uint32_t* status_host, void* stream) {
-  const char* fn = "glm53_latent_expanded";
-  if (dtype != GLM53_DTYPE_BF16 && dtype != GLM53_DTYPE_FP16) {
-    set_last_error("%s: unknown element type %d", fn, dtype);
-    return GLM53_ERR_INVALID;
-  }
-  if (nope_dim <= 0 || nope_dim % 64 != 0 || (rope_dim != 0 && rope_dim != 64) || nope_dim + rope_dim > 256 ||
-      value_dim <= 0 || value_dim % 64 != 0 || value_dim > 256) {
-    set_last_error("%s: nope %lld, rotary %lld (0 or 64) and value %lld sizes are multiples of 64; queries and values "
-                   "hold at most 256",
-                   fn, (long long)nope_dim, (long long)rope_dim, (long long)value_dim);
-    return GLM53_ERR_INVALID;
-  }
-  if (query_tokens < 0 || query_tokens > INT32_MAX || key_tokens < 0 || key_tokens > INT32_MAX || heads < 1 ||
-      heads > 1024 || requests < 0 || requests > 65535 || !std::isfinite(scale)) {
-    set_last_error("%s: %lld heads (1 to 1024), %lld requests (up to 65535), a finite scale", fn, (long long)heads,
-                   (long long)requests);
-    return GLM53_ERR_INVALID;
-  }
-  if (!stride_ok(qn_stride_t) || !stride_ok(qn_stride_h) || !stride_ok(kn_stride_t) || !stride_ok(kn_stride_h) ||
-      !stride_ok(v_stride_t) || !stride_ok(v_stride_h) ||
-      (rope_dim && (!stride_ok(qr_stride_t) || !stride_ok(qr_stride_h) || !stride_ok(kr_stride_t)))) {
-    set_last_error("%s: strides must be non-negative multiples of 8", fn);
-    return GLM53_ERR_INVALID;
-  }
-  if (query_tokens == 0) return GLM53_OK;
-  if (!q_nope || !out || (rope_dim && !q_rope) || (key_tokens && (!k_nope || !values || (rope_dim && !k_rope))) ||
-      !query_starts || !key_starts ||
-      (((uintptr_t)q_nope | (uintptr_t)q_rope | (uintptr_t)k_nope | (uintptr_t)k_rope | (uintptr_t)values |
-        (uintptr_t)out) & 15)) {
-    set_last_error("%s: tensors must be non-NULL and 16-byte aligned", fn);
-    return GLM53_ERR_INVALID;
-  }
-  ExpandedArgs a{(const uint16_t*)q_nope, (const uint16_t*)q_rope, (const uint16_t*)k_nope, (const uint16_t*)k_rope,
-                 (const uint16_t*)values, qn_stride_t, qn_stride_h, qr_stride_t, qr_stride_h, kn_stride_t, kn_stride_h,
-                 kr_stride_t, v_stride_t, v_stride_h, query_tokens, key_tokens, (int)heads, (int)nope_dim,
-                 (int)rope_dim, (int)value_dim, query_starts, key_starts, (int)requests, scale, causal,
-                 (uint16_t*)out, lse, fill_tail, status, status_host};
-  const dim3 grid((unsigned)query_tokens, (unsigned)heads);
-  if (dtype == GLM53_DTYPE_BF16)
-    expanded_kernel<__nv_bfloat16><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
-  else
-    expanded_kernel<__half><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
   return check_launch(fn);
 }
