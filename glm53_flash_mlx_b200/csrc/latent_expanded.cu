@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's
   volatile int* abort_flag = &bars->abort_flag;
 
   if (warp == 8) {
@@ -298,60 +298,70 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 9) {
     // ---------------- MMA ----------------
-    if (lane == 0 && tiles > 0) {
+    // The whole warp walks the loop and one elected lane issues, so that
+    // descriptors stay in uniform registers; eight MMAs a slot are unrolled.
+    if (tiles > 0) {
       constexpr bool bf16 = std::is_same<E, __nv_bfloat16>::value;
       constexpr uint32_t id_s = make_idesc_f16(kTile, kTile, bf16, false, false);
-      uint32_t seq = 0;
-      bool ok = mbar_wait(bar(&bars->q_full), 0, abort_flag);
+      const bool leader = elect_one();
+      uint32_t seq = 0, s = 0;
+      bool ok = __all_sync(0xffffffffu, mbar_wait(bar(&bars->q_full), 0, abort_flag));
       const uint64_t qd = make_sw128_desc(smem_addr(q_smem));
-      auto take = [&](uint32_t& s) {
+      const uint64_t kd0 = make_sw128_desc(smem_addr(ring)), vd0 = make_sw128_mn_desc(smem_addr(ring), kChunkBytes);
+      auto take = [&]() {
         s = seq % kSlots;
-        if (ok) ok = mbar_wait(bar(&bars->full[s]), (seq / kSlots) & 1u, abort_flag);
+        __syncwarp();
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(&bars->full[s]), (seq / kSlots) & 1u, abort_flag));
         ++seq;
+        tmem_fence_after();
         return ok;
       };
       for (int t = 0; t <= tiles && ok; ++t) {
         if (t < tiles) {
-          const uint32_t d = tmem + kSCol + (t & 1) * kTile;
-          for (int p = 0; p < kslots && ok; ++p) {
-            uint32_t s;
-            if (!take(s)) break;
-            tmem_fence_after();
-            const int n = min(2, nch - 2 * p);
-            for (int c = 0; c < n; ++c) {
-              const uint64_t ad = qd + (uint64_t)(((2 * p + c) * kChunkBytes) >> 4);
-              const uint64_t kd = make_sw128_desc(smem_addr(ring + s * kSlotBytes + c * kChunkBytes));
+          const uint32_t d = kSCol + (t & 1) * kTile;
+          for (int p = 0; p < kslots && take(); ++p) {
+            const uint64_t ad = qd + (uint64_t)(p * (kSlotBytes >> 4));
+            const uint64_t kd = kd0 + (uint64_t)(s * (kSlotBytes >> 4));
+            if (leader) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_f16_ss(d, ad + 2 * k, kd + 2 * k, id_s, (p | c | k) != 0);
+              for (int k = 0; k < 4; ++k) mma_f16_ss(d, ad + 2 * k, kd + 2 * k, id_s, (p | k) != 0);
+              if (2 * p + 1 < nch) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  mma_f16_ss(d, ad + (kChunkBytes >> 4) + 2 * k, kd + (kChunkBytes >> 4) + 2 * k, id_s, 1);
+              }
+              mma_commit(bar(&bars->empty[s]));
             }
-            mma_commit(bar(&bars->empty[s]));
           }
-          if (ok) mma_commit(bar(&bars->s_full[t & 1]));
+          if (ok && leader) mma_commit(bar(&bars->s_full[t & 1]));
         }
         if (t > 0 && ok) {
           const int u = t - 1;
-          ok = mbar_wait(bar(&bars->p_full[u & 1]), (u >> 1) & 1u, abort_flag);
-          const int valid = min(kTile, nk - u * kTile);
-          const int steps = (valid + 15) >> 4;
-          for (int p = 0; p < vslots && ok; ++p) {
-            uint32_t s;
-            if (!take(s)) break;
-            tmem_fence_after();
-            const int n = min(2, vch - 2 * p);
-            const uint32_t id_o = n == 2 ? make_idesc_f16(kTile, 128, bf16, false, true)
-                                         : make_idesc_f16(kTile, 64, bf16, false, true);
-            const uint64_t vd = make_sw128_mn_desc(smem_addr(ring + s * kSlotBytes), kChunkBytes);
-            for (int k = 0; k < steps; ++k)
-              mma_f16_ts(tmem + kOCol + p * 128, tmem + kSCol + (u & 1) * kTile + 8 * k, vd + (uint64_t)(k * 128), id_o,
-                         (u | k) != 0);
-            mma_commit(bar(&bars->empty[s]));
+          __syncwarp();
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(&bars->p_full[u & 1]), (u >> 1) & 1u, abort_flag));
+          const uint32_t pa = kSCol + (u & 1) * kTile;
+          const int steps = (min(kTile, nk - u * kTile) + 15) >> 4;
+          for (int p = 0; p < vslots && take(); ++p) {
+            const uint32_t id_o = 2 * p + 1 < vch ? make_idesc_f16(kTile, 128, bf16, false, true)
+                                                  : make_idesc_f16(kTile, 64, bf16, false, true);
+            const uint64_t vd = vd0 + (uint64_t)(s * (kSlotBytes >> 4));
+            const uint32_t o = kOCol + p * 128;
+            if (leader) {
+              if (steps == 8) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
+              } else {
+                for (int k = 0; k < steps; ++k) mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
+              }
+              mma_commit(bar(&bars->empty[s]));
+            }
           }
-          if (ok) mma_commit(bar(&bars->o_done));
+          if (ok && leader) mma_commit(bar(&bars->o_done));
         }
       }
       // no MMA is in flight when TMEM is freed
       volatile int never = 0;
-      mma_commit(bar(&bars->drain));
+      if (leader) mma_commit(bar(&bars->drain));
       mbar_wait(bar(&bars->drain), 0, &never);
     }
     __syncwarp();
@@ -498,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0 && bars->abort_flag) report(a.status, a.status_host, kStatusWaitTimeout);
   if (warp == 9) {
     tmem_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars->tmem_base), "r"(512) : "memory");
   }
 }
 
