@@ -1,171 +1,689 @@
-// Latent attention: every token's keys and values come from one shared latent
-// row (512 values at the model's shape) and one rotary row (64).
-//
-// Absorbed form (decode).  The queries are already in the latent space, so
-// for token t and head h over the request's cached rows c_j, r_j
+// Latent attention, absorbed form (decode): the queries are in the latent
+// space already, so for a token's head h over its request's cached rows
+// [c_j | r_j]
 //   s_j = scale (q_latent . c_j + q_rope . r_j),  o = sum_j softmax(s)_j c_j.
-// Expanded form (prefill).  Keys [k_nope_h | k_rope] and values v_h of every
-// head are given; causal rows see the keys up to their own position.
 //
-// One block per (token, head): eight warps walk the keys, each with its own
-// running maximum and sum, and the eight results are joined in shared memory.
+// All heads read the same rows: a row (1,152 bytes at 512 + 64) is used for
+// 64 x 2 x 1,088 FLOPs, 121 FLOP a byte against the 259 where this GPU's
+// tensor cores and memory balance, so the floor is one pass over the cache.
+// The products are formed with the keys on the M side,
+//   S^T [64 keys x 64 heads]    = rows . Q^T        (M64 N64, K = 576)
+//   O^T [latent x 64 heads]    += c^T . P^T         (4 x M128 N64, K = 64)
+// so that 64 heads fill N instead of half of M, O^T needs only 256 of the 512
+// TMEM columns, and a row's latent part is the operand of both products from
+// one copy in shared memory (K-major for the first, MN-major for the second).
+// Shared memory holds Q (72 KB), two tiles of 64 rows (72 KB each, filled and
+// freed in 128-value groups) and P^T (8 KB).
+//
+// A CTA per SM takes an equal run of the flattened list of (token, 64 heads,
+// tile) units, whatever the lengths: the number of tiles is summed on the
+// device, so a captured graph follows its lengths.  A unit that lies within
+// one CTA's run is finished there; others leave FP32 partial results (at most
+// two a CTA) that a second kernel joins.
+//
+// Roles: warps 0-3 softmax (a 16-key strip each) and epilogue, warp 4 TMA,
+// warp 5 issues S^T, warp 6 issues O^T.  Row maxima are replaced only when a
+// score passes them by 2^8 (latent.cuh).  A token never shares a tile's keys
+// with one that sees fewer, so only rows behind a request's end are masked:
+// their scores are replaced, and their values cleared in shared memory (a zero
+// weight does not remove a NaN) up to the 16 rows that an MMA takes.
+// Every mbarrier wait is bounded, as in the expanded form.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
+#include "gemv_tile.cuh"
+#include "kernels.cuh"
 #include "latent.cuh"
+#include "tcgen05.cuh"
 
 namespace glm53 {
 namespace latent {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kMaxDim = 640;    // query values of a head (nope or latent, and rotary)
-constexpr int kMaxValue = 512;  // two 8-value pieces a lane
+using namespace tc;
 
-struct Joined {
-  float q[kMaxDim];
-  float o[kWarps][kMaxValue];
-  float m[kWarps], l[kWarps];
-};
+constexpr int kKeys = 64;                  // cache rows a tile
+constexpr int kHeads = 64;                 // heads a unit
+constexpr int kChunkBytes = kKeys * 128;   // 64 rows of 64 values
+constexpr int kMaxChunks = 9;
+constexpr int kMaxGroups = 5;              // 128-value groups, the rotary part last
+constexpr int kStageBytes = kMaxChunks * kChunkBytes;
+constexpr int kSoftThreads = 128;
+constexpr int kThreads = kSoftThreads + 96;
+constexpr int kSCol = 256;                 // TMEM: O^T at 0..255, two S^T tiles behind
 
-// One (token, head): keys(j, a, b, v) gives key j's two parts and value row.
-template <typename E, typename Keys>
-__device__ __forceinline__ void attend(Joined& sm, const uint16_t* qa, int da, const uint16_t* qb, int db, int dv,
-                                       int64_t visible, float scale, uint16_t* out, float* lse, Keys keys) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < da + db; i += kThreads)
-    sm.q[i] = Elem<E>::to_float(i < da ? qa[i] : qb[i - da]);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, acc[2][8] = {};
-  for (int64_t j = warp; j < visible; j += kWarps) {
-    const uint16_t *ka, *kb, *kv;
-    keys(j, ka, kb, kv);
-    float s = 0.f;
-    for (int v = lane; v < (da + db) >> 3; v += 32) {
-      const int e = v * 8;
-      float f[8];
-      unpack8<E>(*reinterpret_cast<const uint4*>(e < da ? ka + e : kb + e - da), f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s = fmaf(sm.q[e + i], f[i], s);
-    }
-    s = warp_sum(s) * scale;
-    const float top = fmaxf(m, s);
-    const float base = top == -INFINITY ? 0.f : top;
-    const float keep = __expf(m - base), p = __expf(s - base);
-    l = l * keep + p;
-    m = top;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int v = lane + 32 * i;
-      if (v * 8 < dv) {
-        float f[8];
-        unpack8<E>(*reinterpret_cast<const uint4*>(kv + v * 8), f);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) acc[i][k] = fmaf(p, f[k], acc[i][k] * keep);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int v = lane + 32 * i;
-    if (v * 8 < dv)
-      for (int k = 0; k < 8; ++k) sm.o[warp][v * 8 + k] = acc[i][k];
-  }
-  if (lane == 0) {
-    sm.m[warp] = m;
-    sm.l[warp] = l;
-  }
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.m[w]);
-  const float base = top == -INFINITY ? 0.f : top;
-  for (int w = 0; w < kWarps; ++w) sum += sm.l[w] * __expf(sm.m[w] - base);
-  const float inv = visible > 0 ? 1.f / sum : 0.f;
-  for (int i = threadIdx.x; i < dv; i += kThreads) {
-    float o = 0.f;
-    for (int w = 0; w < kWarps; ++w) o = fmaf(sm.o[w][i], __expf(sm.m[w] - base), o);
-    out[i] = visible > 0 ? Elem<E>::from_float(o * inv) : (uint16_t)0;
-  }
-  if (lse && threadIdx.x == 0) *lse = visible > 0 ? top + logf(sum) : -INFINITY;
-}
-
-// Largest i with starts[i] <= t among starts[0..n - 1].
-__device__ __forceinline__ int request_of(const int32_t* starts, int n, int t) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= t)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return lo;
-}
-
-struct AbsorbedArgs {
-  const uint16_t *ql, *qr;
-  int64_t ql_t, ql_h, qr_t, qr_h;
+struct Args {
   int64_t T;
-  int H, R, r;
-  const uint16_t* cache;
+  int H, R, r, G;  // G groups of 64 heads
   int64_t pages;
-  int page;
+  int page, box;   // rows of a page, rows of a TMA box: gcd(page, 64)
   const int32_t* table;
   int64_t table_stride, table_width;
   const int32_t* lens;
   int B;
   const int32_t* starts;
-  float scale;
+  float c;  // scale log2(e)
   uint16_t* out;
   float* lse;
   int fill_tail;
   uint32_t *status, *status_host;
+  // workspace
+  int64_t* plan;     // [0] tiles a CTA; then the first tile of every token (-1: outside every request)
+  int32_t* counts;   // tiles of every token, one group of heads
+  float *po, *pm, *pl;  // partial results [2 grid][64][R], their maxima and sums [2 grid][64]
 };
 
-template <typename E>
-__global__ void __launch_bounds__(kThreads) absorbed_kernel(AbsorbedArgs a) {
-  __shared__ Joined sm;
-  const int t = blockIdx.x, h = blockIdx.y;
-  int i = t;
-  int64_t len = 0, back = 0;
-  bool tail = false;
+struct Request {
+  int q0, nq, len;
+  bool bad;
+};
+__device__ __forceinline__ Request request_at(const Args& a, int i) {
+  Request q{i, 1, a.lens[i], false};
   if (a.starts) {
-    tail = a.B == 0 || t >= a.starts[a.B];
-    if (!tail) {
-      i = request_of(a.starts, a.B, t);
-      back = (int64_t)a.starts[i + 1] - 1 - t;
-      if (back < 0) tail = true;  // starts that do not ascend
+    q.q0 = a.starts[i];
+    const int64_t n = (int64_t)a.starts[i + 1] - q.q0;
+    q.nq = (int)n;
+    if (q.q0 < 0 || n < 0 || q.q0 + n > a.T) {
+      q.bad = true;
+      q.nq = 0;
     }
   }
-  if (tail && !a.fill_tail) return;
-  if (!tail) {
-    len = a.lens[i];
-    if (len < 0 || len > a.table_width * a.page) {
-      if (threadIdx.x == 0) report(a.status, a.status_host, kStatusBadGeometry);
-      len = 0;
-    }
+  if (q.len < 0 || q.len > a.table_width * a.page) {
+    q.bad = true;
+    q.len = 0;
   }
-  const int64_t visible = len - back;
-  const int width = a.R + a.r;
-  const int32_t* row = a.table + (tail ? 0 : i * a.table_stride);
-  attend<E>(sm, a.ql + t * a.ql_t + h * a.ql_h, a.R, a.qr + t * a.qr_t + h * a.qr_h, a.r, a.R,
-            visible > 0 ? visible : 0, a.scale, a.out + ((int64_t)t * a.H + h) * a.R,
-            a.lse ? a.lse + (int64_t)t * a.H + h : nullptr,
-            [&](int64_t j, const uint16_t*& ka, const uint16_t*& kb, const uint16_t*& kv) {
-              const int64_t at = j / a.page;
-              int32_t id = row[at];
-              if (id < 0 || id >= a.pages) {
-                report(a.status, a.status_host, kStatusBadPage);
-                id = 0;
-              }
-              ka = a.cache + ((int64_t)id * a.page + (j - at * a.page)) * width;
-              kb = ka + a.R;
-              kv = ka;
-            });
+  return q;
+}
+__device__ __forceinline__ int visible_of(const Request& q, int j) { return max(0, q.len - (q.nq - 1 - j)); }
+__device__ __forceinline__ int tiles_of(int visible) { return (visible + kKeys - 1) / kKeys; }
+// sum over v = 1..n of ceil(v / 64)
+__device__ __forceinline__ int64_t tiles_up_to(int64_t n) {
+  if (n <= 0) return 0;
+  const int64_t q = n / kKeys, r = n % kKeys;
+  return kKeys * (q * (q + 1) / 2) + r * (q + 1);
 }
 
-bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s < (int64_t)1 << 38; }
+// A CTA's place in the flattened list: request i, its token j, head group g,
+// tile of that unit, and tiles left in the run.
+struct Cursor {
+  int i, j, g, tile;
+  int64_t left;
+};
+struct Segment {
+  int token, g, tile, n, tiles, visible, request;
+};
+__device__ __forceinline__ bool next_segment(const Args& a, Cursor& c, Segment& s) {
+  while (c.left > 0 && c.i < a.B) {
+    const Request q = request_at(a, c.i);
+    while (c.j < q.nq) {
+      const int vis = visible_of(q, c.j), n = tiles_of(vis);
+      if (n == 0) {
+        ++c.j;
+        continue;
+      }
+      s.token = q.q0 + c.j;
+      s.g = c.g;
+      s.tile = c.tile;
+      s.tiles = n;
+      s.visible = vis;
+      s.request = c.i;
+      s.n = (int)min(c.left, (int64_t)(n - c.tile));
+      c.left -= s.n;
+      c.tile = 0;
+      if (++c.g == a.G) {
+        c.g = 0;
+        ++c.j;
+      }
+      return true;
+    }
+    ++c.i;
+    c.j = 0;
+  }
+  return false;
+}
+
+struct __align__(8) Bars {
+  uint64_t q_full, q_empty, full[2][kMaxGroups], empty[2][kMaxGroups], s_full[2], p_full[2], o_done, drain[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  Cursor cursor;
+  int64_t warp_sum[kThreads / 32];
+  float factor[kHeads];
+  float xchg[4][kHeads];
+};
+// alignment slack, Q, two stages, P^T, barriers
+constexpr size_t kSmemBytes = 1024 + 3 * (size_t)kStageBytes + kChunkBytes + 2048;
+static_assert(sizeof(Bars) <= 2048, "barriers share two KB");
+static_assert(kSmemBytes <= 232448, "227 KB a CTA");
+
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  __syncwarp();
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+template <typename E>
+__global__ void __launch_bounds__(kThreads, 1)
+    absorbed_kernel(const __grid_constant__ CUtensorMap ql_map, const __grid_constant__ CUtensorMap qr_map,
+                    const __grid_constant__ CUtensorMap kv_map, Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* q_smem = smem;
+  uint8_t* kv_smem = smem + kStageBytes;
+  uint8_t* p_smem = kv_smem + 2 * kStageBytes;
+  Bars* bars = reinterpret_cast<Bars*>(p_smem + kChunkBytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto bar = [&](uint64_t* p) { return smem_addr(p); };
+
+  // the join kernel may be set up beside this one; it waits for its end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // tiles of all requests, this CTA's run of them, and where it begins
+  {
+    const int per = (a.B + kThreads - 1) / kThreads;
+    const int i0 = min(a.B, tid * per), i1 = min(a.B, i0 + per);
+    int64_t n = 0;
+    for (int i = i0; i < i1; ++i) {
+      const Request q = request_at(a, i);
+      n += (tiles_up_to(q.len) - tiles_up_to((int64_t)q.len - q.nq)) * a.G;
+      if (q.bad && blockIdx.x == 0) report(a.status, a.status_host, kStatusBadGeometry);
+    }
+    int64_t s = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += x;
+    }
+    if (lane == 31) bars->warp_sum[warp] = s;
+    if (tid == 0) {
+      bars->cursor.left = 0;
+      bars->abort_flag = 0;
+      mbar_init(bar(&bars->q_full), 1);
+      mbar_init(bar(&bars->q_empty), 1);
+      for (int b = 0; b < 2; ++b) {
+        for (int g = 0; g < kMaxGroups; ++g) {
+          mbar_init(bar(&bars->full[b][g]), 1);
+          mbar_init(bar(&bars->empty[b][g]), 1);
+        }
+        mbar_init(bar(&bars->s_full[b]), 1);
+        mbar_init(bar(&bars->p_full[b]), 4);
+        mbar_init(bar(&bars->drain[b]), 1);
+      }
+      mbar_init(bar(&bars->o_done), 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (blockIdx.x == 0)
+      for (int64_t t = tid; t < a.T; t += kThreads) a.plan[1 + t] = -1;
+    __syncthreads();
+    int64_t total = 0, before = s - n;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += bars->warp_sum[w];
+      total += bars->warp_sum[w];
+    }
+    const int64_t run = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
+    const int64_t begin = min(total, (int64_t)blockIdx.x * run), end = min(total, begin + run);
+    if (blockIdx.x == 0) {
+      if (tid == 0) a.plan[0] = run;
+      int64_t f = before;
+      for (int i = i0; i < i1; ++i) {
+        const Request q = request_at(a, i);
+        for (int j = 0; j < q.nq; ++j) {
+          const int k = tiles_of(visible_of(q, j));
+          a.plan[1 + q.q0 + j] = f;
+          a.counts[q.q0 + j] = k;
+          f += (int64_t)k * a.G;
+        }
+      }
+    }
+    if (begin < end && before <= begin && begin < before + n) {
+      int64_t f = before;
+      for (int i = i0; i < i1; ++i) {
+        const Request q = request_at(a, i);
+        const int64_t all = (tiles_up_to(q.len) - tiles_up_to((int64_t)q.len - q.nq)) * a.G;
+        if (begin >= f + all) {
+          f += all;
+          continue;
+        }
+        int j = 0;
+        for (;; ++j) {
+          const int64_t k = (int64_t)tiles_of(visible_of(q, j)) * a.G;
+          if (begin < f + k) break;
+          f += k;
+        }
+        const int k = tiles_of(visible_of(q, j));
+        const int rest = (int)(begin - f);
+        bars->cursor = Cursor{i, j, rest / k, rest % k, end - begin};
+        break;
+      }
+    }
+  }
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(&bars->tmem_base)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  volatile int* abort_flag = &bars->abort_flag;
+  constexpr bool bf16 = std::is_same<E, __nv_bfloat16>::value;
+  const int groups = a.R / 128, all_groups = groups + (a.r ? 1 : 0);
+  Cursor cur = bars->cursor;
+  Segment sg;
+  uint32_t n = 0;  // tiles so far, over all segments
+
+  if (warp == 4) {
+    // ---------------- TMA ----------------
+    const int boxes = kKeys / a.box;
+    const int64_t cache_rows = a.pages * a.page;
+    bool ok = true;
+    uint32_t queries = 0;  // Q tiles asked for
+    int at_group = 0;
+    while (ok && next_segment(a, cur, sg)) {
+      if (queries) ok = mbar_wait_warp(bar(&bars->q_empty), (queries - 1) & 1u, abort_flag);
+      if (!ok) break;
+      ++queries;
+      if (lane == 0) {
+        mbar_expect_tx(bar(&bars->q_full), (a.R + a.r) / 64 * kChunkBytes);
+        for (int c = 0; c < a.R / 64; ++c)
+          tma_load_3d(smem_addr(q_smem + c * kChunkBytes), &ql_map, c * 64, sg.g * kHeads, sg.token,
+                      bar(&bars->q_full));
+        if (a.r)
+          tma_load_3d(smem_addr(q_smem + a.R / 64 * kChunkBytes), &qr_map, 0, sg.g * kHeads, sg.token,
+                      bar(&bars->q_full));
+      }
+      const int32_t* row = a.table + sg.request * a.table_stride;
+      for (int t = sg.tile; t < sg.tile + sg.n && ok; ++t, ++n) {
+        // lane k fetches box k: rows pos .. pos + box of the request
+        const int pos = t * kKeys + lane * a.box;
+        const bool mine = lane < boxes && pos < sg.visible;
+        int y = 0;
+        if (mine) {
+          const int at = pos / a.page;
+          const int32_t id = row[at];
+          if (id < 0 || id >= a.pages) {
+            report(a.status, a.status_host, kStatusBadPage);
+            y = (int)cache_rows;  // outside the map: zeros
+          } else {
+            y = id * a.page + (pos - at * a.page);
+          }
+        }
+        const int count = __popc(__ballot_sync(0xffffffffu, mine));
+        const uint32_t b = n & 1, use = n >> 1;
+        for (at_group = 0; at_group < all_groups; ++at_group) {
+          const int g = at_group;
+          if (use) ok = mbar_wait_warp(bar(&bars->empty[b][g]), (use - 1) & 1u, abort_flag);
+          if (!ok) break;
+          const int chunks = g < groups ? 2 : 1;
+          if (lane == 0) mbar_expect_tx(bar(&bars->full[b][g]), count * chunks * a.box * 128);
+          __syncwarp();
+          if (mine)
+            for (int c = 0; c < chunks; ++c)
+              tma_load_2d(smem_addr(kv_smem + b * kStageBytes + (2 * g + c) * kChunkBytes + lane * a.box * 128),
+                          &kv_map, (2 * g + c) * 64, y, bar(&bars->full[b][g]));
+        }
+        if (!ok) break;
+        at_group = 0;
+      }
+    }
+    if (!ok && lane == 0) {
+      // copies still in flight write this CTA's shared memory: wait for them
+      volatile int never = 0;
+      if (queries) mbar_wait(bar(&bars->q_full), (queries - 1) & 1u, &never);
+      for (int b = 0; b < 2; ++b)
+        for (int g = 0; g < all_groups; ++g) {
+          // the last tile of this stage whose group g was issued
+          int64_t last = (int64_t)n - ((n & 1) == (uint32_t)b ? (g < at_group ? 0 : 2) : 1);
+          never = 0;
+          if (last >= 0) mbar_wait(bar(&bars->full[b][g]), (uint32_t)(last >> 1) & 1u, &never);
+        }
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    // ---------------- S^T = rows . Q^T ----------------
+    const bool leader = elect_one();
+    constexpr uint32_t id_s = make_idesc_f16(kKeys, kHeads, bf16, false, false);
+    const uint64_t qd0 = make_sw128_desc(smem_addr(q_smem)), kd0 = make_sw128_desc(smem_addr(kv_smem));
+    bool ok = true;
+    for (uint32_t segments = 0; ok && next_segment(a, cur, sg); ++segments) {
+      ok = mbar_wait_warp(bar(&bars->q_full), segments & 1u, abort_flag);
+      for (int t = 0; t < sg.n && ok; ++t, ++n) {
+        const uint32_t b = n & 1, use = n >> 1;
+        if (use) ok = mbar_wait_warp(bar(&bars->p_full[b]), (use - 1) & 1u, abort_flag);  // S^T buffer read
+        for (int g = 0; g < all_groups && ok; ++g) {
+          ok = mbar_wait_warp(bar(&bars->full[b][g]), use & 1u, abort_flag);
+          if (!ok) break;
+          tmem_fence_after();
+          const uint64_t kd = kd0 + (uint64_t)((b * kStageBytes + 2 * g * kChunkBytes) >> 4);
+          const uint64_t qd = qd0 + (uint64_t)((2 * g * kChunkBytes) >> 4);
+          const uint32_t d = kSCol + b * kHeads;
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_f16_ss(d, kd + 2 * k, qd + 2 * k, id_s, (g | k) != 0);
+            if (g < groups) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_f16_ss(d, kd + (kChunkBytes >> 4) + 2 * k, qd + (kChunkBytes >> 4) + 2 * k, id_s, 1);
+            } else {
+              mma_commit(bar(&bars->empty[b][g]));  // the rotary part is not a value
+            }
+          }
+          __syncwarp();
+        }
+        if (ok && leader) mma_commit(bar(&bars->s_full[b]));
+      }
+      if (ok && leader) mma_commit(bar(&bars->q_empty));
+    }
+    volatile int never = 0;
+    if (leader) mma_commit(bar(&bars->drain[0]));
+    __syncwarp();
+    mbar_wait(bar(&bars->drain[0]), 0, &never);
+    __syncwarp();
+  } else if (warp == 6) {
+    // ---------------- O^T += c^T . P^T ----------------
+    const bool leader = elect_one();
+    constexpr uint32_t id_o = make_idesc_f16(128, kHeads, bf16, true, true);
+    const uint64_t vd0 = make_sw128_mn_desc(smem_addr(kv_smem), kChunkBytes);
+    const uint64_t pd0 = make_sw128_mn_desc(smem_addr(p_smem), kChunkBytes);
+    bool ok = true;
+    while (ok && next_segment(a, cur, sg)) {
+      for (int t = 0; t < sg.n && ok; ++t, ++n) {
+        const uint32_t b = n & 1, use = n >> 1;
+        ok = mbar_wait_warp(bar(&bars->p_full[b]), use & 1u, abort_flag);
+        if (!ok) break;
+        tmem_fence_after();
+        const int valid = min(kKeys, sg.visible - (sg.tile + t) * kKeys);
+        const int steps = (valid + 15) >> 4;
+        for (int g = 0; g < groups; ++g) {
+          const uint64_t vd = vd0 + (uint64_t)((b * kStageBytes + 2 * g * kChunkBytes) >> 4);
+          if (leader) {
+            if (steps == 4) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_f16_ss(g * kHeads, vd + 128 * k, pd0 + 128 * k, id_o, (t | k) != 0);
+            } else {
+              for (int k = 0; k < steps; ++k)
+                mma_f16_ss(g * kHeads, vd + 128 * k, pd0 + 128 * k, id_o, (t | k) != 0);
+            }
+            mma_commit(bar(&bars->empty[b][g]));
+          }
+          __syncwarp();
+        }
+        if (leader) mma_commit(bar(&bars->o_done));
+      }
+    }
+    volatile int never = 0;
+    if (leader) mma_commit(bar(&bars->drain[1]));
+    __syncwarp();
+    mbar_wait(bar(&bars->drain[1]), 0, &never);
+    __syncwarp();
+  } else {
+    // ---------------- softmax, epilogue ----------------
+    // this thread's keys of a tile: k0 and k0 + 8; its heads: 8 j + h0 + {0, 1}
+    const int k0 = 16 * warp + (lane >> 2), h0 = 2 * (lane & 3);
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    bool stop = false;
+    for (int segment = 0; !stop && next_segment(a, cur, sg); ++segment) {
+      float m[16], l[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+      }
+      for (int t = 0; t < sg.n; ++t, ++n) {
+        const uint32_t b = n & 1, use = n >> 1;
+        if (!mbar_wait_warp(bar(&bars->s_full[b]), use & 1u, abort_flag)) stop = true;
+        const int valid = min(kKeys, sg.visible - (sg.tile + t) * kKeys);
+        float v[32];
+        bool grow = stop;
+        if (!stop) {
+          tmem_fence_after();
+          uint32_t w[32];
+          tmem_ld16x64(lanes + kSCol + b * kHeads, w);
+          tmem_wait_ld();
+          const bool in0 = k0 < valid, in1 = k0 + 8 < valid;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] = ((i & 2) ? in1 : in0) ? __uint_as_float(w[i]) * a.c : -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int e = (i >> 1) * 4 + (i & 1);
+            grow |= fmaxf(v[e], v[e + 2]) > m[i] + kMaxSlack;
+          }
+          if (valid < kKeys) {
+            // clear the value rows that the last MMA step takes beyond the end
+            const int r16 = (valid + 15) & ~15, pieces = a.R / 8;
+            for (int i = tid; i < (r16 - valid) * pieces; i += kSoftThreads) {
+              const int row = valid + i / pieces, p = i % pieces;
+              *reinterpret_cast<uint4*>(kv_smem + b * kStageBytes + (p >> 3) * kChunkBytes + row * 128 + (p & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            }
+          }
+        }
+        if (any_of(grow, 1, kSoftThreads)) {
+          stop = any_of(stop, 1, kSoftThreads);
+          if (stop) break;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int e = (i >> 1) * 4 + (i & 1);
+            float x = fmaxf(v[e], v[e + 2]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            if (lane < 4) bars->xchg[warp][8 * (i >> 1) + h0 + (i & 1)] = x;
+          }
+          bar_sync(1, kSoftThreads);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int h = 8 * (i >> 1) + h0 + (i & 1);
+            const float top = fmaxf(m[i], fmaxf(fmaxf(bars->xchg[0][h], bars->xchg[1][h]),
+                                                fmaxf(bars->xchg[2][h], bars->xchg[3][h])));
+            const float f = top == m[i] ? 1.f : ex2(m[i] - top);
+            m[i] = top;
+            l[i] *= f;
+            if (tid < 4) bars->factor[h] = f;
+          }
+          bar_sync(1, kSoftThreads);
+          if (t > 0 && mbar_wait_warp(bar(&bars->o_done), (n - 1) & 1u, abort_flag)) {
+            tmem_fence_after();
+            for (int o = 0; o < groups * kHeads; o += 32) {
+              uint32_t w[32];
+              tmem_ld32(lanes + o, w);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                w[i] = __float_as_uint(__uint_as_float(w[i]) * bars->factor[(o & 32) + i]);
+              tmem_st32(lanes + o, w);
+            }
+            tmem_wait_st();
+          }
+        }
+        // P^T: rows of keys, 64 heads of 2 bytes, 128-byte swizzle
+        uint32_t p0[8], p1[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float s0 = m[2 * j] == -INFINITY ? 0.f : m[2 * j], s1 = m[2 * j + 1] == -INFINITY ? 0.f : m[2 * j + 1];
+          const float a0 = ex2(v[4 * j] - s0), a1 = ex2(v[4 * j + 1] - s1);
+          const float b0 = ex2(v[4 * j + 2] - s0), b1 = ex2(v[4 * j + 3] - s1);
+          l[2 * j] += a0 + b0;
+          l[2 * j + 1] += a1 + b1;
+          p0[j] = Elem<E>::pack(a0, a1);
+          p1[j] = Elem<E>::pack(b0, b1);
+        }
+        if (n > 0) mbar_wait_warp(bar(&bars->o_done), (n - 1) & 1u, abort_flag);  // P^T of the last tile is read
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint8_t* at = p_smem + k0 * 128 + ((j ^ (k0 & 7)) << 4) + 2 * h0;
+          *reinterpret_cast<uint32_t*>(at) = p0[j];
+          *reinterpret_cast<uint32_t*>(at + 8 * 128) = p1[j];
+        }
+        fence_async_shared();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(&bars->p_full[b]));
+      }
+      if (!stop) stop = !mbar_wait_warp(bar(&bars->o_done), (n - 1) & 1u, abort_flag);
+      stop = any_of(stop, 1, kSoftThreads);
+      if (stop) break;
+      // row sums over the 64 keys of every strip
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float x = l[i];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (lane < 4) bars->xchg[warp][8 * (i >> 1) + h0 + (i & 1)] = x;
+      }
+      bar_sync(1, kSoftThreads);
+      const int heads = min(kHeads, a.H - sg.g * kHeads);
+      const bool whole = sg.n == sg.tiles;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (segment ? 1 : 0);
+      const int64_t first = (int64_t)sg.token * a.H + sg.g * kHeads;  // row of out
+      if (tid < 4) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int h = 8 * (i >> 1) + h0 + (i & 1);
+          const float sum = (bars->xchg[0][h] + bars->xchg[1][h]) + (bars->xchg[2][h] + bars->xchg[3][h]);
+          bars->factor[h] = whole ? 1.f / sum : 1.f;
+          if (!whole) {
+            a.pm[slot * kHeads + h] = m[i];
+            a.pl[slot * kHeads + h] = sum;
+          } else if (a.lse && h < heads) {
+            a.lse[first + h] = ((m[i] == -INFINITY ? 0.f : m[i]) + log2f(sum)) * kLn2;
+          }
+        }
+      }
+      bar_sync(1, kSoftThreads);
+      tmem_fence_after();
+      for (int o = 0; o < groups * kHeads; o += 32) {
+        uint32_t w[32];
+        tmem_ld32(lanes + o, w);
+        tmem_wait_ld();
+        const int d = (o >> 6) * 128 + tid;  // latent index
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int h = (o & 32) + i;
+          if (h < heads) {
+            const float x = __uint_as_float(w[i]) * bars->factor[h];
+            if (whole)
+              a.out[(first + h) * a.R + d] = Elem<E>::from_float(x);
+            else
+              a.po[(slot * kHeads + h) * a.R + d] = x;
+          }
+        }
+      }
+      tmem_fence_before();
+      bar_sync(1, kSoftThreads);  // factor and xchg are free again
+    }
+  }
+  __syncthreads();
+  if (tid == 0 && bars->abort_flag) report(a.status, a.status_host, kStatusWaitTimeout);
+  if (warp == 5) {
+    tmem_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars->tmem_base), "r"(512) : "memory");
+  }
+}
+
+// Joins the partial results of units that several CTAs shared:
+//   o = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p,  M the largest m_p,
+// and fills what no CTA wrote (tokens that see nothing; with fill_tail those
+// outside every request).  A block takes one (token, head); four thread groups
+// take every fourth part, 16 bytes a thread.
+constexpr int kJoinThreads = 512;
+
+template <typename E>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, int grid) {
+  __shared__ float4 part[4][128];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int t = blockIdx.x, h = blockIdx.y;
+  const int64_t first = a.plan[1 + t], run = a.plan[0], at = (int64_t)t * a.H + h;
+  const int col = threadIdx.x & 127, quarter = threadIdx.x >> 7;
+  const int n = first < 0 ? 0 : a.counts[t];
+  if (n == 0) {
+    if (first < 0 && !a.fill_tail) return;
+    if (quarter == 0 && 4 * col < a.R) *reinterpret_cast<uint2*>(a.out + at * a.R + 4 * col) = make_uint2(0, 0);
+    if (a.lse && threadIdx.x == 0) a.lse[at] = -INFINITY;
+    return;
+  }
+  const int64_t f = first + (int64_t)(h / kHeads) * n;
+  const int c0 = (int)(f / run), c1 = (int)((f + n - 1) / run), hl = h % kHeads;
+  if (c0 == c1) return;
+  auto slot = [&](int c) { return 2 * (int64_t)c + (c == c0 && f != c0 * run ? 1 : 0); };
+  float top = -INFINITY;
+  for (int c = c0; c <= c1; ++c) top = fmaxf(top, a.pm[slot(c) * kHeads + hl]);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = c0; c <= c1; ++c) sum += a.pl[slot(c) * kHeads + hl] * ex2(a.pm[slot(c) * kHeads + hl] - base);
+  if (4 * col < a.R) {
+#pragma unroll 4
+    for (int c = c0 + quarter; c <= c1; c += 4) {
+      const int64_t s = slot(c) * kHeads + hl;
+      const float w = ex2(a.pm[s] - base);
+      const float4 x = *reinterpret_cast<const float4*>(a.po + s * a.R + 4 * col);
+      o.x = fmaf(w, x.x, o.x);
+      o.y = fmaf(w, x.y, o.y);
+      o.z = fmaf(w, x.z, o.z);
+      o.w = fmaf(w, x.w, o.w);
+    }
+  }
+  part[quarter][col] = o;
+  __syncthreads();
+  if (quarter == 0 && 4 * col < a.R) {
+    const float inv = 1.f / sum;
+    float4 y = part[0][col];
+    for (int k = 1; k < 4; ++k) {
+      y.x += part[k][col].x;
+      y.y += part[k][col].y;
+      y.z += part[k][col].z;
+      y.w += part[k][col].w;
+    }
+    *reinterpret_cast<uint2*>(a.out + at * a.R + 4 * col) =
+        make_uint2(Elem<E>::pack(y.x * inv, y.y * inv), Elem<E>::pack(y.z * inv, y.w * inv));
+  }
+  if (a.lse && threadIdx.x == 0) a.lse[at] = (base + log2f(sum)) * kLn2;
+}
+
+size_t plan_bytes(int64_t tokens) { return align_up((size_t)(tokens + 1) * 8, 256) + align_up((size_t)tokens * 4, 256); }
+size_t part_bytes(int64_t latent_dim) {
+  return 2 * (size_t)sm_count() * kHeads * ((size_t)latent_dim + 2) * sizeof(float);
+}
+
+bool stride_ok(int64_t s, int64_t count) {
+  return s % 8 == 0 && s < (int64_t)1 << 38 && (count > 1 ? s > 0 : s >= 0);
+}
+
+int make_map(CUtensorMap* map, const void* base, bool bf16, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+             const cuuint32_t* box) {
+  auto fn = encode_fn();
+  if (!fn) {
+    set_last_error("glm53_latent_absorbed: cuTensorMapEncodeTiled is unavailable");
+    return GLM53_ERR_CUDA;
+  }
+  const cuuint32_t step[3] = {1, 1, 1};
+  const CUresult r =
+      fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base),
+         dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_last_error("glm53_latent_absorbed: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return GLM53_ERR_CUDA;
+  }
+  return GLM53_OK;
+}
+
+template <typename E>
+int launch(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMap& kv, const Args& a, cudaStream_t st) {
+  const int rc = ensure_max_smem((const void*)absorbed_kernel<E>, kSmemBytes);
+  if (rc) return rc;
+  const int grid = sm_count();
+  absorbed_kernel<E><<<grid, kThreads, kSmemBytes, st>>>(ql, qr, kv, a);
+  int err = check_launch("absorbed_kernel");
+  if (err) return err;
+  launch_programmatic(join_kernel<E>, dim3((unsigned)a.T, (unsigned)a.H), dim3(kJoinThreads), 0, st, a, grid);
+  return check_launch("join_kernel");
+}
 
 }  // namespace
 }  // namespace latent
@@ -175,10 +693,8 @@ using namespace glm53;
 using namespace glm53::latent;
 
 extern "C" size_t glm53_latent_absorbed_workspace_bytes(int64_t tokens, int64_t heads, int64_t latent_dim) {
-  (void)tokens;
-  (void)heads;
-  (void)latent_dim;
-  return 256;
+  if (tokens < 0 || heads < 1 || latent_dim < 1 || latent_dim > 512) return 0;
+  return plan_bytes(tokens) + part_bytes(latent_dim);
 }
 
 extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, int64_t ql_stride_h,
@@ -207,9 +723,9 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
                    fn, (long long)heads, (long long)page_size, (long long)pages, (long long)table_width);
     return GLM53_ERR_INVALID;
   }
-  if (!std::isfinite(scale) || !stride_ok(ql_stride_t) || !stride_ok(ql_stride_h) || ql_stride_h < latent_dim ||
-      (rope_dim && (!stride_ok(qr_stride_t) || !stride_ok(qr_stride_h) || qr_stride_h < rope_dim))) {
-    set_last_error("%s: the scale must be finite and strides non-negative multiples of 8", fn);
+  if (!std::isfinite(scale) || !stride_ok(ql_stride_t, tokens) || !stride_ok(ql_stride_h, heads) ||
+      (rope_dim && (!stride_ok(qr_stride_t, tokens) || !stride_ok(qr_stride_h, heads)))) {
+    set_last_error("%s: the scale must be finite and strides positive multiples of 8", fn);
     return GLM53_ERR_INVALID;
   }
   if (!query_starts && tokens != requests) {
@@ -228,14 +744,62 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
     set_last_error("%s: the workspace is too small", fn);
     return GLM53_ERR_INVALID;
   }
-  AbsorbedArgs a{(const uint16_t*)q_latent, (const uint16_t*)q_rope, ql_stride_t, ql_stride_h, qr_stride_t, qr_stride_h,
-                 tokens, (int)heads, (int)latent_dim, (int)rope_dim, (const uint16_t*)cache, pages, (int)page_size,
-                 block_table, table_stride, table_width, seq_lens, (int)requests, query_starts, scale, (uint16_t*)out,
-                 lse, fill_tail, status, status_host};
-  const dim3 grid((unsigned)tokens, (unsigned)heads);
-  if (dtype == GLM53_DTYPE_BF16)
-    absorbed_kernel<__nv_bfloat16><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
-  else
-    absorbed_kernel<__half><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
-  return check_launch(fn);
+  if ((uintptr_t)workspace & 255) {
+    set_last_error("%s: the workspace must be 256-byte aligned", fn);
+    return GLM53_ERR_INVALID;
+  }
+  const bool bf16 = dtype == GLM53_DTYPE_BF16;
+  CUtensorMap ql, qr, kv;
+  const cuuint64_t ql_dims[3] = {(cuuint64_t)latent_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  const cuuint64_t ql_strides[2] = {(cuuint64_t)(ql_stride_h ? ql_stride_h : 8) * 2,
+                                    (cuuint64_t)(ql_stride_t ? ql_stride_t : 8) * 2};
+  const cuuint32_t q_box[3] = {64, kHeads, 1};
+  int rc = make_map(&ql, q_latent, bf16, 3, ql_dims, ql_strides, q_box);
+  if (rc) return rc;
+  qr = kv = ql;  // maps that no load reads (no rotary part, no pages)
+  if (rope_dim) {
+    const cuuint64_t dims[3] = {(cuuint64_t)rope_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)(qr_stride_h ? qr_stride_h : 8) * 2,
+                                   (cuuint64_t)(qr_stride_t ? qr_stride_t : 8) * 2};
+    if ((rc = make_map(&qr, q_rope, bf16, 3, dims, strides, q_box))) return rc;
+  }
+  // rows of a TMA box: the largest divisor of 64 that divides a page
+  int box = 64;
+  while (page_size % box) box >>= 1;
+  if (pages) {
+    const cuuint64_t dims[2] = {(cuuint64_t)(latent_dim + rope_dim), (cuuint64_t)(pages * page_size)};
+    const cuuint64_t strides[1] = {(cuuint64_t)(latent_dim + rope_dim) * 2};
+    const cuuint32_t kv_box[2] = {64, (cuuint32_t)box};
+    if ((rc = make_map(&kv, cache, bf16, 2, dims, strides, kv_box))) return rc;
+  }
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int64_t slots = 2 * (int64_t)sm_count() * kHeads;
+  Args a{};
+  a.T = tokens;
+  a.H = (int)heads;
+  a.R = (int)latent_dim;
+  a.r = (int)rope_dim;
+  a.G = (int)((heads + kHeads - 1) / kHeads);
+  a.pages = pages;
+  a.page = (int)page_size;
+  a.box = box;
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.table_width = pages ? table_width : 0;  // no page can be named
+  a.lens = seq_lens;
+  a.B = (int)requests;
+  a.starts = query_starts;
+  a.c = scale * kLog2e;
+  a.out = (uint16_t*)out;
+  a.lse = lse;
+  a.fill_tail = fill_tail;
+  a.status = status;
+  a.status_host = status_host;
+  a.plan = reinterpret_cast<int64_t*>(ws);
+  a.counts = reinterpret_cast<int32_t*>(ws + align_up((size_t)(tokens + 1) * 8, 256));
+  a.po = reinterpret_cast<float*>(ws + plan_bytes(tokens));
+  a.pm = a.po + slots * latent_dim;
+  a.pl = a.pm + slots;
+  return bf16 ? launch<__nv_bfloat16>(ql, qr, kv, a, (cudaStream_t)stream)
+              : launch<__half>(ql, qr, kv, a, (cudaStream_t)stream);
 }
