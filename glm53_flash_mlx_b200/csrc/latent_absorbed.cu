@@ -12,8 +12,16 @@
 // so that 64 heads fill N instead of half of M, O^T needs only 256 of the 512
 // TMEM columns, and a row's latent part is the operand of both products from
 // one copy in shared memory (K-major for the first, MN-major for the second).
+// Measured alone, one thread issuing: 32 cycles an M64 N64 MMA, 48 an M128
+// N64, so a tile of 64 rows is 1,920 cycles against ~3,070 of its share of the
+// memory bandwidth.
+//
 // Shared memory holds Q (72 KB), two tiles of 64 rows (72 KB each, filled and
-// freed in 128-value groups) and P^T (8 KB).
+// freed in two halves of the row) and P^T (8 KB).  Inside a half, eight rows
+// of each 64-value chunk are one swizzle atom and the chunks of eight rows lie
+// side by side, so that one TMA (a 4-D view: 64 values, 8 rows, chunks, row
+// groups) brings a half of all rows that are contiguous in the cache, whatever
+// the page size.
 //
 // A CTA per SM takes an equal run of the flattened list of (token, 64 heads,
 // tile) units, whatever the lengths: the number of tiles is summed on the
@@ -47,10 +55,11 @@ constexpr int kKeys = 64;                  // cache rows a tile
 constexpr int kHeads = 64;                 // heads a unit
 constexpr int kChunkBytes = kKeys * 128;   // 64 rows of 64 values
 constexpr int kMaxChunks = 9;
-constexpr int kMaxGroups = 5;              // 128-value groups, the rotary part last
+constexpr int kAtomBytes = 1024;           // 8 rows of a chunk
 constexpr int kStageBytes = kMaxChunks * kChunkBytes;
 constexpr int kSoftThreads = 128;
 constexpr int kThreads = kSoftThreads + 96;
+constexpr int kMaxGrid = 256;              // parts a join block holds weights of, halved
 constexpr int kSCol = 256;                 // TMEM: O^T at 0..255, two S^T tiles behind
 
 struct Args {
@@ -58,6 +67,7 @@ struct Args {
   int H, R, r, G;  // G groups of 64 heads
   int64_t pages;
   int page, box;   // rows of a page, rows of a TMA box: gcd(page, 64)
+  int half[2];     // chunks of the two halves of a row: whole 128-value groups, the rotary part last
   const int32_t* table;
   int64_t table_stride, table_width;
   const int32_t* lens;
@@ -69,7 +79,7 @@ struct Args {
   int fill_tail;
   uint32_t *status, *status_host;
   // workspace
-  int64_t* plan;     // [0] tiles a CTA; then the first tile of every token (-1: outside every request)
+  int32_t* plan;     // [0] tiles a CTA; then the first tile of every token (-1: outside every request)
   int32_t* counts;   // tiles of every token, one group of heads
   float *po, *pm, *pl;  // partial results [2 grid][64][R], their maxima and sums [2 grid][64]
 };
@@ -103,12 +113,17 @@ __device__ __forceinline__ int64_t tiles_up_to(int64_t n) {
   const int64_t q = n / kKeys, r = n % kKeys;
   return kKeys * (q * (q + 1) / 2) + r * (q + 1);
 }
+// Tiles of all of a request's units (the host checks that the sum over all
+// requests stays below 2^31).
+__device__ __forceinline__ int tiles_of(const Request& q, int G) {
+  const int n = q.nq == 1 ? tiles_of(q.len) : (int)(tiles_up_to(q.len) - tiles_up_to((int64_t)q.len - q.nq));
+  return n * G;
+}
 
 // A CTA's place in the flattened list: request i, its token j, head group g,
 // tile of that unit, and tiles left in the run.
 struct Cursor {
-  int i, j, g, tile;
-  int64_t left;
+  int i, j, g, tile, left;
 };
 struct Segment {
   int token, g, tile, n, tiles, visible, request;
@@ -128,7 +143,7 @@ __device__ __forceinline__ bool next_segment(const Args& a, Cursor& c, Segment& 
       s.tiles = n;
       s.visible = vis;
       s.request = c.i;
-      s.n = (int)min(c.left, (int64_t)(n - c.tile));
+      s.n = min(c.left, n - c.tile);
       c.left -= s.n;
       c.tile = 0;
       if (++c.g == a.G) {
@@ -144,12 +159,12 @@ __device__ __forceinline__ bool next_segment(const Args& a, Cursor& c, Segment& 
 }
 
 struct __align__(8) Bars {
-  uint64_t q_full, q_empty, full[2][kMaxGroups], empty[2][kMaxGroups], s_full[2], p_full[2], o_done, drain[2];
+  uint64_t q_full, q_empty, full[2][2], empty[2][2], s_full[2], p_full[2], o_done, drain[2];
   uint32_t tmem_base;
   int abort_flag;
   Cursor cursor;
-  int64_t warp_sum[kThreads / 32];
-  float factor[kHeads];
+  int warp_sum[kThreads / 32];
+  float factor[kHeads], top[kHeads];
   float xchg[4][kHeads];
 };
 // alignment slack, Q, two stages, P^T, barriers
@@ -159,13 +174,14 @@ static_assert(kSmemBytes <= 232448, "227 KB a CTA");
 
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   __syncwarp();
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+  return __all_sync(0xffffffffu, mbar_wait_fast(bar, parity, abort_flag));
 }
 
 template <typename E>
 __global__ void __launch_bounds__(kThreads, 1)
     absorbed_kernel(const __grid_constant__ CUtensorMap ql_map, const __grid_constant__ CUtensorMap qr_map,
-                    const __grid_constant__ CUtensorMap kv_map, Args a) {
+                    const __grid_constant__ CUtensorMap kv0_map, const __grid_constant__ CUtensorMap kv1_map,
+                    Args a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* q_smem = smem;
@@ -182,28 +198,32 @@ __global__ void __launch_bounds__(kThreads, 1)
   {
     const int per = (a.B + kThreads - 1) / kThreads;
     const int i0 = min(a.B, tid * per), i1 = min(a.B, i0 + per);
-    int64_t n = 0;
+    int n = 0;
     for (int i = i0; i < i1; ++i) {
       const Request q = request_at(a, i);
-      n += (tiles_up_to(q.len) - tiles_up_to((int64_t)q.len - q.nq)) * a.G;
+      n += tiles_of(q, a.G);
       if (q.bad && blockIdx.x == 0) report(a.status, a.status_host, kStatusBadGeometry);
     }
-    int64_t s = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += x;
-    }
-    if (lane == 31) bars->warp_sum[warp] = s;
-    if (tid == 0) {
+    if (warp == 5) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_addr(&bars->tmem_base)),
+                   "r"(512)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (warp == 4 && lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&ql_map)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qr_map)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kv0_map)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kv1_map)) : "memory");
+    } else if (tid == 0) {
       bars->cursor.left = 0;
       bars->abort_flag = 0;
       mbar_init(bar(&bars->q_full), 1);
       mbar_init(bar(&bars->q_empty), 1);
       for (int b = 0; b < 2; ++b) {
-        for (int g = 0; g < kMaxGroups; ++g) {
-          mbar_init(bar(&bars->full[b][g]), 1);
-          mbar_init(bar(&bars->empty[b][g]), 1);
+        for (int h = 0; h < 2; ++h) {
+          mbar_init(bar(&bars->full[b][h]), 1);
+          mbar_init(bar(&bars->empty[b][h]), 1);
         }
         mbar_init(bar(&bars->s_full[b]), 1);
         mbar_init(bar(&bars->p_full[b]), 4);
@@ -212,75 +232,73 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(&bars->o_done), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
+    int s = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += x;
+    }
+    if (lane == 31) bars->warp_sum[warp] = s;
     if (blockIdx.x == 0)
       for (int64_t t = tid; t < a.T; t += kThreads) a.plan[1 + t] = -1;
     __syncthreads();
-    int64_t total = 0, before = s - n;
+    int total = 0, before = s - n;
+#pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) before += bars->warp_sum[w];
       total += bars->warp_sum[w];
     }
-    const int64_t run = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
-    const int64_t begin = min(total, (int64_t)blockIdx.x * run), end = min(total, begin + run);
+    const int run = max(1, (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x));
+    const int64_t begin = (int64_t)blockIdx.x * run;
     if (blockIdx.x == 0) {
       if (tid == 0) a.plan[0] = run;
-      int64_t f = before;
+      int f = before;
       for (int i = i0; i < i1; ++i) {
         const Request q = request_at(a, i);
         for (int j = 0; j < q.nq; ++j) {
           const int k = tiles_of(visible_of(q, j));
           a.plan[1 + q.q0 + j] = f;
           a.counts[q.q0 + j] = k;
-          f += (int64_t)k * a.G;
+          f += k * a.G;
         }
       }
     }
-    if (begin < end && before <= begin && begin < before + n) {
-      int64_t f = before;
+    if (begin < total && before <= begin && begin < (int64_t)before + n) {
+      int f = before;
       for (int i = i0; i < i1; ++i) {
         const Request q = request_at(a, i);
-        const int64_t all = (tiles_up_to(q.len) - tiles_up_to((int64_t)q.len - q.nq)) * a.G;
+        const int all = tiles_of(q, a.G);
         if (begin >= f + all) {
           f += all;
           continue;
         }
         int j = 0;
-        for (;; ++j) {
-          const int64_t k = (int64_t)tiles_of(visible_of(q, j)) * a.G;
-          if (begin < f + k) break;
-          f += k;
-        }
-        const int k = tiles_of(visible_of(q, j));
-        const int rest = (int)(begin - f);
-        bars->cursor = Cursor{i, j, rest / k, rest % k, end - begin};
+        while (begin >= f + tiles_of(visible_of(q, j)) * a.G) f += tiles_of(visible_of(q, j++)) * a.G;
+        const int k = tiles_of(visible_of(q, j)), rest = (int)(begin - f);
+        const int g = a.G == 1 ? 0 : rest / k;
+        bars->cursor = Cursor{i, j, g, rest - g * k, min(run, total - (int)begin)};
         break;
       }
     }
-  }
-  if (warp == 5) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_addr(&bars->tmem_base)),
-                 "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
   volatile int* abort_flag = &bars->abort_flag;
   constexpr bool bf16 = std::is_same<E, __nv_bfloat16>::value;
-  const int groups = a.R / 128, all_groups = groups + (a.r ? 1 : 0);
+  const int groups = a.R / 128, halves = a.half[1] ? 2 : 1;
+  const int half_bytes = a.half[0] * kChunkBytes;  // of the first half of a tile
   Cursor cur = bars->cursor;
   Segment sg;
   uint32_t n = 0;  // tiles so far, over all segments
 
   if (warp == 4) {
     // ---------------- TMA ----------------
-    const int boxes = kKeys / a.box;
-    const int64_t cache_rows = a.pages * a.page;
+    const int boxes = kKeys / a.box, box_groups = a.box / 8;
     bool ok = true;
     uint32_t queries = 0;  // Q tiles asked for
-    int at_group = 0;
+    int at_half = 0;
     while (ok && next_segment(a, cur, sg)) {
       if (queries) ok = mbar_wait_warp(bar(&bars->q_empty), (queries - 1) & 1u, abort_flag);
       if (!ok) break;
@@ -299,33 +317,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         // lane k fetches box k: rows pos .. pos + box of the request
         const int pos = t * kKeys + lane * a.box;
         const bool mine = lane < boxes && pos < sg.visible;
-        int y = 0;
+        int y = 0;  // group of eight rows in the cache
         if (mine) {
           const int at = pos / a.page;
           const int32_t id = row[at];
           if (id < 0 || id >= a.pages) {
             report(a.status, a.status_host, kStatusBadPage);
-            y = (int)cache_rows;  // outside the map: zeros
+            y = (int)(a.pages * a.page / 8);  // outside the map: zeros
           } else {
-            y = id * a.page + (pos - at * a.page);
+            y = (id * a.page + (pos - at * a.page)) / 8;
           }
         }
         const int count = __popc(__ballot_sync(0xffffffffu, mine));
         const uint32_t b = n & 1, use = n >> 1;
-        for (at_group = 0; at_group < all_groups; ++at_group) {
-          const int g = at_group;
-          if (use) ok = mbar_wait_warp(bar(&bars->empty[b][g]), (use - 1) & 1u, abort_flag);
+        for (at_half = 0; at_half < halves; ++at_half) {
+          const int h = at_half;
+          if (use) ok = mbar_wait_warp(bar(&bars->empty[b][h]), (use - 1) & 1u, abort_flag);
           if (!ok) break;
-          const int chunks = g < groups ? 2 : 1;
-          if (lane == 0) mbar_expect_tx(bar(&bars->full[b][g]), count * chunks * a.box * 128);
+          const int row_bytes = a.half[h] * kAtomBytes;  // eight rows
+          if (lane == 0) mbar_expect_tx(bar(&bars->full[b][h]), count * box_groups * row_bytes);
           __syncwarp();
           if (mine)
-            for (int c = 0; c < chunks; ++c)
-              tma_load_2d(smem_addr(kv_smem + b * kStageBytes + (2 * g + c) * kChunkBytes + lane * a.box * 128),
-                          &kv_map, (2 * g + c) * 64, y, bar(&bars->full[b][g]));
+            tma_load_4d(smem_addr(kv_smem + b * kStageBytes + h * half_bytes + lane * box_groups * row_bytes),
+                        h ? &kv1_map : &kv0_map, 0, 0, h ? a.half[0] : 0, y, bar(&bars->full[b][h]));
         }
         if (!ok) break;
-        at_group = 0;
+        at_half = 0;
       }
     }
     if (!ok && lane == 0) {
@@ -333,49 +350,50 @@ __global__ void __launch_bounds__(kThreads, 1)
       volatile int never = 0;
       if (queries) mbar_wait(bar(&bars->q_full), (queries - 1) & 1u, &never);
       for (int b = 0; b < 2; ++b)
-        for (int g = 0; g < all_groups; ++g) {
-          // the last tile of this stage whose group g was issued
-          int64_t last = (int64_t)n - ((n & 1) == (uint32_t)b ? (g < at_group ? 0 : 2) : 1);
+        for (int h = 0; h < halves; ++h) {
+          // the last tile of this stage whose half h was asked for
+          const int64_t last = (int64_t)n - ((n & 1) == (uint32_t)b ? (h < at_half ? 0 : 2) : 1);
           never = 0;
-          if (last >= 0) mbar_wait(bar(&bars->full[b][g]), (uint32_t)(last >> 1) & 1u, &never);
+          if (last >= 0) mbar_wait(bar(&bars->full[b][h]), (uint32_t)(last >> 1) & 1u, &never);
         }
     }
     __syncwarp();
   } else if (warp == 5) {
     // ---------------- S^T = rows . Q^T ----------------
+    // All lanes walk the loops, so that descriptors stay uniform; one waits and issues.
     const bool leader = elect_one();
     constexpr uint32_t id_s = make_idesc_f16(kKeys, kHeads, bf16, false, false);
-    const uint64_t qd0 = make_sw128_desc(smem_addr(q_smem)), kd0 = make_sw128_desc(smem_addr(kv_smem));
+    const uint64_t qd0 = make_sw128_desc(smem_addr(q_smem));
     bool ok = true;
-    for (uint32_t segments = 0; ok && next_segment(a, cur, sg); ++segments) {
-      ok = mbar_wait_warp(bar(&bars->q_full), segments & 1u, abort_flag);
-      for (int t = 0; t < sg.n && ok; ++t, ++n) {
-        const uint32_t b = n & 1, use = n >> 1;
-        if (use) ok = mbar_wait_warp(bar(&bars->p_full[b]), (use - 1) & 1u, abort_flag);  // S^T buffer read
-        for (int g = 0; g < all_groups && ok; ++g) {
-          ok = mbar_wait_warp(bar(&bars->full[b][g]), use & 1u, abort_flag);
-          if (!ok) break;
-          tmem_fence_after();
-          const uint64_t kd = kd0 + (uint64_t)((b * kStageBytes + 2 * g * kChunkBytes) >> 4);
-          const uint64_t qd = qd0 + (uint64_t)((2 * g * kChunkBytes) >> 4);
-          const uint32_t d = kSCol + b * kHeads;
+    for (uint32_t segments = 0; next_segment(a, cur, sg); ++segments) {
+      if (leader) ok = ok && mbar_wait_fast(bar(&bars->q_full), segments & 1u, abort_flag);
+      for (int t = 0; t < sg.n; ++t, ++n) {
+        const uint32_t b = n & 1, use = n >> 1, d = kSCol + b * kHeads;
+        // softmax has read the buffer's last tile
+        if (leader && use) ok = ok && mbar_wait_fast(bar(&bars->p_full[b]), (use - 1) & 1u, abort_flag);
+        for (int h = 0; h < halves; ++h) {
+          const uint64_t kd = make_sw128_desc(smem_addr(kv_smem) + b * kStageBytes + h * half_bytes,
+                                              a.half[h] * kAtomBytes);
+          const uint64_t qd = qd0 + (uint64_t)((h * half_bytes) >> 4);
+          const int chunks = a.half[h];
           if (leader) {
+            ok = ok && mbar_wait_fast(bar(&bars->full[b][h]), use & 1u, abort_flag);
+            tmem_fence_after();
+            if (ok) {
+              for (int c = 0; c < chunks; ++c) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_f16_ss(d, kd + 2 * k, qd + 2 * k, id_s, (g | k) != 0);
-            if (g < groups) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_f16_ss(d, kd + (kChunkBytes >> 4) + 2 * k, qd + (kChunkBytes >> 4) + 2 * k, id_s, 1);
-            } else {
-              mma_commit(bar(&bars->empty[b][g]));  // the rotary part is not a value
+                for (int k = 0; k < 4; ++k)
+                  mma_f16_ss(d, kd + c * (kAtomBytes >> 4) + 2 * k, qd + c * (kChunkBytes >> 4) + 2 * k, id_s,
+                             (h | c | k) != 0);
+              }
             }
           }
-          __syncwarp();
         }
-        if (ok && leader) mma_commit(bar(&bars->s_full[b]));
+        if (leader && ok) mma_commit(bar(&bars->s_full[b]));
       }
-      if (ok && leader) mma_commit(bar(&bars->q_empty));
+      if (leader && ok) mma_commit(bar(&bars->q_empty));
     }
+    __syncwarp();
     volatile int never = 0;
     if (leader) mma_commit(bar(&bars->drain[0]));
     __syncwarp();
@@ -385,34 +403,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- O^T += c^T . P^T ----------------
     const bool leader = elect_one();
     constexpr uint32_t id_o = make_idesc_f16(128, kHeads, bf16, true, true);
-    const uint64_t vd0 = make_sw128_mn_desc(smem_addr(kv_smem), kChunkBytes);
-    const uint64_t pd0 = make_sw128_mn_desc(smem_addr(p_smem), kChunkBytes);
+    const uint64_t pd = make_sw128_mn_desc(smem_addr(p_smem), kChunkBytes);
+    const int groups0 = min(groups, a.half[0] / 2);
     bool ok = true;
-    while (ok && next_segment(a, cur, sg)) {
-      for (int t = 0; t < sg.n && ok; ++t, ++n) {
+    while (next_segment(a, cur, sg)) {
+      for (int t = 0; t < sg.n; ++t, ++n) {
         const uint32_t b = n & 1, use = n >> 1;
-        ok = mbar_wait_warp(bar(&bars->p_full[b]), use & 1u, abort_flag);
-        if (!ok) break;
-        tmem_fence_after();
         const int valid = min(kKeys, sg.visible - (sg.tile + t) * kKeys);
         const int steps = (valid + 15) >> 4;
-        for (int g = 0; g < groups; ++g) {
-          const uint64_t vd = vd0 + (uint64_t)((b * kStageBytes + 2 * g * kChunkBytes) >> 4);
-          if (leader) {
-            if (steps == 4) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) mma_f16_ss(g * kHeads, vd + 128 * k, pd0 + 128 * k, id_o, (t | k) != 0);
-            } else {
-              for (int k = 0; k < steps; ++k)
-                mma_f16_ss(g * kHeads, vd + 128 * k, pd0 + 128 * k, id_o, (t | k) != 0);
-            }
-            mma_commit(bar(&bars->empty[b][g]));
-          }
-          __syncwarp();
+        if (leader) {
+          ok = ok && mbar_wait_fast(bar(&bars->p_full[b]), use & 1u, abort_flag);
+          tmem_fence_after();
         }
-        if (leader) mma_commit(bar(&bars->o_done));
+        for (int h = 0; h < halves; ++h) {
+          const int g0 = h ? groups0 : 0, g1 = h ? groups : groups0;
+          const uint64_t vd = make_sw128_mn_desc(smem_addr(kv_smem) + b * kStageBytes + h * half_bytes, kAtomBytes,
+                                                 a.half[h] * kAtomBytes);
+          const uint32_t step = a.half[h] * (2 * kAtomBytes >> 4);  // 16 keys
+          if (leader && ok) {
+            for (int g = g0; g < g1; ++g) {
+              const uint64_t v = vd + (uint64_t)((g - g0) * (2 * kAtomBytes >> 4));
+              if (steps == 4) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma_f16_ss(g * kHeads, v + k * step, pd + 128 * k, id_o, (t | k) != 0);
+              } else {
+                for (int k = 0; k < steps; ++k)
+                  mma_f16_ss(g * kHeads, v + k * step, pd + 128 * k, id_o, (t | k) != 0);
+              }
+            }
+            mma_commit(bar(&bars->empty[b][h]));
+          }
+        }
+        if (leader && ok) mma_commit(bar(&bars->o_done));
       }
     }
+    __syncwarp();
     volatile int never = 0;
     if (leader) mma_commit(bar(&bars->drain[1]));
     __syncwarp();
@@ -455,9 +480,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             // clear the value rows that the last MMA step takes beyond the end
             const int r16 = (valid + 15) & ~15, pieces = a.R / 8;
             for (int i = tid; i < (r16 - valid) * pieces; i += kSoftThreads) {
-              const int row = valid + i / pieces, p = i % pieces;
-              *reinterpret_cast<uint4*>(kv_smem + b * kStageBytes + (p >> 3) * kChunkBytes + row * 128 + (p & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
+              const int row = valid + i / pieces, p = i % pieces, c = p >> 3;
+              const int h = c >= a.half[0] ? 1 : 0;
+              uint8_t* at = kv_smem + b * kStageBytes + h * half_bytes +
+                            ((row >> 3) * a.half[h] + c - h * a.half[0]) * kAtomBytes;
+              *reinterpret_cast<uint4*>(at + (row & 7) * 128 + (p & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
           }
         }
@@ -536,22 +563,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane < 4) bars->xchg[warp][8 * (i >> 1) + h0 + (i & 1)] = x;
       }
       bar_sync(1, kSoftThreads);
+      if (tid < 4) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bars->top[8 * (i >> 1) + h0 + (i & 1)] = m[i];
+      }
+      bar_sync(1, kSoftThreads);
       const int heads = min(kHeads, a.H - sg.g * kHeads);
       const bool whole = sg.n == sg.tiles;
       const int64_t slot = 2 * (int64_t)blockIdx.x + (segment ? 1 : 0);
       const int64_t first = (int64_t)sg.token * a.H + sg.g * kHeads;  // row of out
-      if (tid < 4) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int h = 8 * (i >> 1) + h0 + (i & 1);
-          const float sum = (bars->xchg[0][h] + bars->xchg[1][h]) + (bars->xchg[2][h] + bars->xchg[3][h]);
-          bars->factor[h] = whole ? 1.f / sum : 1.f;
-          if (!whole) {
-            a.pm[slot * kHeads + h] = m[i];
-            a.pl[slot * kHeads + h] = sum;
-          } else if (a.lse && h < heads) {
-            a.lse[first + h] = ((m[i] == -INFINITY ? 0.f : m[i]) + log2f(sum)) * kLn2;
-          }
+      if (tid < kHeads) {
+        const float sum = (bars->xchg[0][tid] + bars->xchg[1][tid]) + (bars->xchg[2][tid] + bars->xchg[3][tid]);
+        const float top = bars->top[tid];
+        bars->factor[tid] = 1.f / sum;
+        if (!whole) {
+          a.pm[slot * kHeads + tid] = top;
+          a.pl[slot * kHeads + tid] = sum;
+        } else if (a.lse && tid < heads) {
+          a.lse[first + tid] = ((top == -INFINITY ? 0.f : top) + log2f(sum)) * kLn2;
         }
       }
       bar_sync(1, kSoftThreads);
@@ -560,21 +589,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t w[32];
         tmem_ld32(lanes + o, w);
         tmem_wait_ld();
-        const int d = (o >> 6) * 128 + tid;  // latent index
+        const int d = (o >> 6) * 128 + tid, hb = o & 32;  // latent index, first head
+        const int lim = heads - hb;
+        if (!whole) {
+          float* dst = a.po + (slot * kHeads + hb) * a.R + d;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int h = (o & 32) + i;
-          if (h < heads) {
-            const float x = __uint_as_float(w[i]) * bars->factor[h];
-            if (whole)
-              a.out[(first + h) * a.R + d] = Elem<E>::from_float(x);
-            else
-              a.po[(slot * kHeads + h) * a.R + d] = x;
+          for (int i = 0; i < 32; ++i)
+            if (i < lim) dst[i * a.R] = __uint_as_float(w[i]);
+        } else {
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 x = reinterpret_cast<const float4*>(bars->factor + hb)[i];
+            f[4 * i] = x.x;
+            f[4 * i + 1] = x.y;
+            f[4 * i + 2] = x.z;
+            f[4 * i + 3] = x.w;
+          }
+          // lane pairs exchange values, so that a store holds two latent values
+          const int odd = lane & 1;
+          uint16_t* dst = a.out + (first + hb + odd) * a.R + (d - odd);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float x0 = __uint_as_float(w[i]) * f[i], x1 = __uint_as_float(w[i + 1]) * f[i + 1];
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? x0 : x1, 1);
+            if (i + odd < lim)
+              *reinterpret_cast<uint32_t*>(dst + i * a.R) = odd ? Elem<E>::pack(got, x1) : Elem<E>::pack(x0, got);
           }
         }
       }
       tmem_fence_before();
-      bar_sync(1, kSoftThreads);  // factor and xchg are free again
+      bar_sync(1, kSoftThreads);  // factor, top and xchg are free again
     }
   }
   __syncthreads();
@@ -588,66 +633,82 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the partial results of units that several CTAs shared:
 //   o = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p,  M the largest m_p,
 // and fills what no CTA wrote (tokens that see nothing; with fill_tail those
-// outside every request).  A block takes one (token, head); four thread groups
-// take every fourth part, 16 bytes a thread.
-constexpr int kJoinThreads = 512;
-
-template <typename E>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, int grid) {
-  __shared__ float4 part[4][128];
+// outside every request).  Few results (WAYS = 8): a block takes a fourth of a
+// (token, head), and eight warps every eighth part of it.  Many (WAYS = 1): a
+// block takes a whole one.
+template <typename E, int WAYS>
+__global__ void __launch_bounds__(WAYS == 1 ? 128 : 32 * WAYS) join_kernel(Args a) {
+  constexpr int kCols = WAYS == 1 ? 128 : 32;  // float4 columns a block
+  __shared__ float weight[2 * kMaxGrid];
+  __shared__ float4 part[WAYS][kCols];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int t = blockIdx.x, h = blockIdx.y;
-  const int64_t first = a.plan[1 + t], run = a.plan[0], at = (int64_t)t * a.H + h;
-  const int col = threadIdx.x & 127, quarter = threadIdx.x >> 7;
-  const int n = first < 0 ? 0 : a.counts[t];
+  const int first = a.plan[1 + t], run = a.plan[0], n = first < 0 ? 0 : a.counts[t];
+  const int64_t at = (int64_t)t * a.H + h;
+  const int way = threadIdx.x / kCols, col = 4 * (blockIdx.z * kCols + threadIdx.x % kCols);
+  const bool mine = col < a.R;
   if (n == 0) {
     if (first < 0 && !a.fill_tail) return;
-    if (quarter == 0 && 4 * col < a.R) *reinterpret_cast<uint2*>(a.out + at * a.R + 4 * col) = make_uint2(0, 0);
-    if (a.lse && threadIdx.x == 0) a.lse[at] = -INFINITY;
+    if (way == 0 && mine) *reinterpret_cast<uint2*>(a.out + at * a.R + col) = make_uint2(0, 0);
+    if (a.lse && threadIdx.x == 0 && blockIdx.z == 0) a.lse[at] = -INFINITY;
     return;
   }
-  const int64_t f = first + (int64_t)(h / kHeads) * n;
-  const int c0 = (int)(f / run), c1 = (int)((f + n - 1) / run), hl = h % kHeads;
+  const int f = first + (h / kHeads) * n, c0 = f / run, c1 = (f + n - 1) / run, hl = h % kHeads;
   if (c0 == c1) return;
-  auto slot = [&](int c) { return 2 * (int64_t)c + (c == c0 && f != c0 * run ? 1 : 0); };
-  float top = -INFINITY;
-  for (int c = c0; c <= c1; ++c) top = fmaxf(top, a.pm[slot(c) * kHeads + hl]);
+  // a CTA's first segment is its slot 2 c, a last one that begins a unit 2 c + 1
+  const bool late = f != c0 * run;
+  const int parts = c1 - c0 + 1;
+  auto slot = [&](int p) { return (int64_t)(2 * (c0 + p) + (p == 0 && late ? 1 : 0)) * kHeads + hl; };
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY, sum = 0.f;
+  for (int p = lane; p < parts; p += 32) top = fmaxf(top, a.pm[slot(p)]);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
+  for (int p = lane; p < parts; p += 32) {
+    const float w = ex2(a.pm[slot(p)] - base);
+    if (threadIdx.x < 32) weight[p] = w;
+    sum = fmaf(a.pl[slot(p)], w, sum);
+  }
+  sum = warp_sum(sum);
+  __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = c0; c <= c1; ++c) sum += a.pl[slot(c) * kHeads + hl] * ex2(a.pm[slot(c) * kHeads + hl] - base);
-  if (4 * col < a.R) {
-#pragma unroll 4
-    for (int c = c0 + quarter; c <= c1; c += 4) {
-      const int64_t s = slot(c) * kHeads + hl;
-      const float w = ex2(a.pm[s] - base);
-      const float4 x = *reinterpret_cast<const float4*>(a.po + s * a.R + 4 * col);
+  if (mine) {
+#pragma unroll 6
+    for (int p = way; p < parts; p += WAYS) {
+      const float w = weight[p];
+      const float4 x = *reinterpret_cast<const float4*>(a.po + slot(p) * a.R + col);
       o.x = fmaf(w, x.x, o.x);
       o.y = fmaf(w, x.y, o.y);
       o.z = fmaf(w, x.z, o.z);
       o.w = fmaf(w, x.w, o.w);
     }
   }
-  part[quarter][col] = o;
-  __syncthreads();
-  if (quarter == 0 && 4 * col < a.R) {
-    const float inv = 1.f / sum;
-    float4 y = part[0][col];
-    for (int k = 1; k < 4; ++k) {
-      y.x += part[k][col].x;
-      y.y += part[k][col].y;
-      y.z += part[k][col].z;
-      y.w += part[k][col].w;
+  if constexpr (WAYS > 1) {
+    part[way][threadIdx.x % kCols] = o;
+    __syncthreads();
+    if (way) return;
+#pragma unroll
+    for (int k = 1; k < WAYS; ++k) {
+      const float4 x = part[k][threadIdx.x % kCols];
+      o.x += x.x;
+      o.y += x.y;
+      o.z += x.z;
+      o.w += x.w;
     }
-    *reinterpret_cast<uint2*>(a.out + at * a.R + 4 * col) =
-        make_uint2(Elem<E>::pack(y.x * inv, y.y * inv), Elem<E>::pack(y.z * inv, y.w * inv));
   }
-  if (a.lse && threadIdx.x == 0) a.lse[at] = (base + log2f(sum)) * kLn2;
+  if (mine) {
+    const float inv = 1.f / sum;
+    *reinterpret_cast<uint2*>(a.out + at * a.R + col) =
+        make_uint2(Elem<E>::pack(o.x * inv, o.y * inv), Elem<E>::pack(o.z * inv, o.w * inv));
+  }
+  if (a.lse && threadIdx.x == 0 && blockIdx.z == 0) a.lse[at] = (base + log2f(sum)) * kLn2;
 }
 
-size_t plan_bytes(int64_t tokens) { return align_up((size_t)(tokens + 1) * 8, 256) + align_up((size_t)tokens * 4, 256); }
+int grid_size() { return std::min(sm_count(), kMaxGrid); }
+size_t plan_bytes(int64_t tokens) { return align_up((size_t)(2 * tokens + 1) * 4, 256); }
 size_t part_bytes(int64_t latent_dim) {
-  return 2 * (size_t)sm_count() * kHeads * ((size_t)latent_dim + 2) * sizeof(float);
+  return 2 * (size_t)grid_size() * kHeads * ((size_t)latent_dim + 2) * sizeof(float);
 }
 
 bool stride_ok(int64_t s, int64_t count) {
@@ -661,7 +722,7 @@ int make_map(CUtensorMap* map, const void* base, bool bf16, int rank, const cuui
     set_last_error("glm53_latent_absorbed: cuTensorMapEncodeTiled is unavailable");
     return GLM53_ERR_CUDA;
   }
-  const cuuint32_t step[3] = {1, 1, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
   const CUresult r =
       fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base),
          dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -674,14 +735,16 @@ int make_map(CUtensorMap* map, const void* base, bool bf16, int rank, const cuui
 }
 
 template <typename E>
-int launch(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMap& kv, const Args& a, cudaStream_t st) {
-  const int rc = ensure_max_smem((const void*)absorbed_kernel<E>, kSmemBytes);
+int launch(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMap& kv0, const CUtensorMap& kv1, const Args& a,
+           cudaStream_t st) {
+  int rc = ensure_max_smem((const void*)absorbed_kernel<E>, kSmemBytes);
   if (rc) return rc;
-  const int grid = sm_count();
-  absorbed_kernel<E><<<grid, kThreads, kSmemBytes, st>>>(ql, qr, kv, a);
-  int err = check_launch("absorbed_kernel");
-  if (err) return err;
-  launch_programmatic(join_kernel<E>, dim3((unsigned)a.T, (unsigned)a.H), dim3(kJoinThreads), 0, st, a, grid);
+  absorbed_kernel<E><<<grid_size(), kThreads, kSmemBytes, st>>>(ql, qr, kv0, kv1, a);
+  if ((rc = check_launch("absorbed_kernel"))) return rc;
+  if (a.T * a.H <= 512)
+    launch_programmatic(join_kernel<E, 8>, dim3((unsigned)a.T, (unsigned)a.H, 4), dim3(256), 0, st, a);
+  else
+    launch_programmatic(join_kernel<E, 1>, dim3((unsigned)a.T, (unsigned)a.H), dim3(128), 0, st, a);
   return check_launch("join_kernel");
 }
 
@@ -733,6 +796,11 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
                    (long long)tokens, (long long)requests);
     return GLM53_ERR_INVALID;
   }
+  if ((double)tokens * (double)((heads + 63) / 64) * (double)((table_width * page_size + 63) / 64) >= 2147483648.0) {
+    set_last_error("%s: %lld tokens over a table of %lld rows: 2^31 tiles of 64 rows at most", fn, (long long)tokens,
+                   (long long)(table_width * page_size));
+    return GLM53_ERR_INVALID;
+  }
   if (tokens == 0) return GLM53_OK;
   if (!q_latent || (rope_dim && !q_rope) || !out || (requests && !seq_lens) ||
       (requests && table_width && !block_table) || (pages && !cache) ||
@@ -749,14 +817,14 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
     return GLM53_ERR_INVALID;
   }
   const bool bf16 = dtype == GLM53_DTYPE_BF16;
-  CUtensorMap ql, qr, kv;
+  CUtensorMap ql, qr, kv0, kv1;
   const cuuint64_t ql_dims[3] = {(cuuint64_t)latent_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
   const cuuint64_t ql_strides[2] = {(cuuint64_t)(ql_stride_h ? ql_stride_h : 8) * 2,
                                     (cuuint64_t)(ql_stride_t ? ql_stride_t : 8) * 2};
   const cuuint32_t q_box[3] = {64, kHeads, 1};
   int rc = make_map(&ql, q_latent, bf16, 3, ql_dims, ql_strides, q_box);
   if (rc) return rc;
-  qr = kv = ql;  // maps that no load reads (no rotary part, no pages)
+  qr = kv0 = kv1 = ql;  // maps that no load reads (no rotary part, no pages, no second half)
   if (rope_dim) {
     const cuuint64_t dims[3] = {(cuuint64_t)rope_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
     const cuuint64_t strides[2] = {(cuuint64_t)(qr_stride_h ? qr_stride_h : 8) * 2,
@@ -766,14 +834,20 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
   // rows of a TMA box: the largest divisor of 64 that divides a page
   int box = 64;
   while (page_size % box) box >>= 1;
+  // the two halves of a row, in 64-value chunks: whole 128-value groups first
+  const int groups = (int)latent_dim / 128;
+  const int half[2] = {2 * ((groups + 1) / 2), 2 * (groups / 2) + (rope_dim ? 1 : 0)};
   if (pages) {
-    const cuuint64_t dims[2] = {(cuuint64_t)(latent_dim + rope_dim), (cuuint64_t)(pages * page_size)};
-    const cuuint64_t strides[1] = {(cuuint64_t)(latent_dim + rope_dim) * 2};
-    const cuuint32_t kv_box[2] = {64, (cuuint32_t)box};
-    if ((rc = make_map(&kv, cache, bf16, 2, dims, strides, kv_box))) return rc;
+    const cuuint64_t width = 2 * (cuuint64_t)(latent_dim + rope_dim);  // bytes
+    const cuuint64_t dims[4] = {64, 8, (cuuint64_t)(latent_dim + rope_dim) / 64, (cuuint64_t)(pages * page_size / 8)};
+    const cuuint64_t strides[3] = {width, 128, 8 * width};
+    cuuint32_t kv_box[4] = {64, 8, (cuuint32_t)half[0], (cuuint32_t)box / 8};
+    if ((rc = make_map(&kv0, cache, bf16, 4, dims, strides, kv_box))) return rc;
+    kv_box[2] = (cuuint32_t)half[1];
+    if (half[1] && (rc = make_map(&kv1, cache, bf16, 4, dims, strides, kv_box))) return rc;
   }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const int64_t slots = 2 * (int64_t)sm_count() * kHeads;
+  const int64_t slots = 2 * (int64_t)grid_size() * kHeads;
   Args a{};
   a.T = tokens;
   a.H = (int)heads;
@@ -795,11 +869,13 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
   a.fill_tail = fill_tail;
   a.status = status;
   a.status_host = status_host;
-  a.plan = reinterpret_cast<int64_t*>(ws);
-  a.counts = reinterpret_cast<int32_t*>(ws + align_up((size_t)(tokens + 1) * 8, 256));
+  a.half[0] = half[0];
+  a.half[1] = half[1];
+  a.plan = reinterpret_cast<int32_t*>(ws);
+  a.counts = a.plan + tokens + 1;
   a.po = reinterpret_cast<float*>(ws + plan_bytes(tokens));
   a.pm = a.po + slots * latent_dim;
   a.pl = a.pm + slots;
-  return bf16 ? launch<__nv_bfloat16>(ql, qr, kv, a, (cudaStream_t)stream)
-              : launch<__half>(ql, qr, kv, a, (cudaStream_t)stream);
+  return bf16 ? launch<__nv_bfloat16>(ql, qr, kv0, kv1, a, (cudaStream_t)stream)
+              : launch<__half>(ql, qr, kv0, kv1, a, (cudaStream_t)stream);
 }
