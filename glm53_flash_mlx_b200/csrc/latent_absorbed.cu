@@ -52,7 +52,7 @@ namespace {
 using namespace tc;
 
 constexpr int kKeys = 64;                  // cache rows a tile
-constexpr int kHeads = 64;                 // heads a unit
+constexpr int kMaxHeads = 64;              // heads a unit, at most
 constexpr int kChunkBytes = kKeys * 128;   // 64 rows of 64 values
 constexpr int kMaxChunks = 9;
 constexpr int kAtomBytes = 1024;           // 8 rows of a chunk
@@ -164,8 +164,8 @@ struct __align__(8) Bars {
   int abort_flag;
   Cursor cursor;
   int warp_sum[kThreads / 32];
-  float factor[kHeads], top[kHeads];
-  float xchg[4][kHeads];
+  float factor[kMaxHeads], top[kMaxHeads];
+  float xchg[4][kMaxHeads];
 };
 // alignment slack, Q, two stages, P^T, barriers
 constexpr size_t kSmemBytes = 1024 + 3 * (size_t)kStageBytes + kChunkBytes + 2048;
@@ -177,7 +177,8 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, mbar_wait_fast(bar, parity, abort_flag));
 }
 
-template <typename E>
+// N: heads a unit, 16, 32 or 64
+template <typename E, int N>
 __global__ void __launch_bounds__(kThreads, 1)
     absorbed_kernel(const __grid_constant__ CUtensorMap ql_map, const __grid_constant__ CUtensorMap qr_map,
                     const __grid_constant__ CUtensorMap kv0_map, const __grid_constant__ CUtensorMap kv1_map,
@@ -304,30 +305,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       ++queries;
       if (lane == 0) {
-        mbar_expect_tx(bar(&bars->q_full), (a.R + a.r) / 64 * kChunkBytes);
+        mbar_expect_tx(bar(&bars->q_full), (a.R + a.r) / 64 * (N * 128));
         for (int c = 0; c < a.R / 64; ++c)
-          tma_load_3d(smem_addr(q_smem + c * kChunkBytes), &ql_map, c * 64, sg.g * kHeads, sg.token,
+          tma_load_3d(smem_addr(q_smem + c * (N * 128)), &ql_map, c * 64, sg.g * N, sg.token,
                       bar(&bars->q_full));
         if (a.r)
-          tma_load_3d(smem_addr(q_smem + a.R / 64 * kChunkBytes), &qr_map, 0, sg.g * kHeads, sg.token,
+          tma_load_3d(smem_addr(q_smem + a.R / 64 * (N * 128)), &qr_map, 0, sg.g * N, sg.token,
                       bar(&bars->q_full));
       }
+      // lane k fetches box k of a tile: rows pos .. pos + box of the request
       const int32_t* row = a.table + sg.request * a.table_stride;
-      for (int t = sg.tile; t < sg.tile + sg.n && ok; ++t, ++n) {
-        // lane k fetches box k: rows pos .. pos + box of the request
+      auto place = [&](int t) {  // group of eight rows in the cache, -1 for none
         const int pos = t * kKeys + lane * a.box;
-        const bool mine = lane < boxes && pos < sg.visible;
-        int y = 0;  // group of eight rows in the cache
-        if (mine) {
-          const int at = pos / a.page;
-          const int32_t id = row[at];
-          if (id < 0 || id >= a.pages) {
-            report(a.status, a.status_host, kStatusBadPage);
-            y = (int)(a.pages * a.page / 8);  // outside the map: zeros
-          } else {
-            y = (id * a.page + (pos - at * a.page)) / 8;
-          }
+        if (lane >= boxes || pos >= sg.visible || t >= sg.tile + sg.n) return -1;
+        const int at = pos / a.page;
+        const int32_t id = row[at];
+        if (id < 0 || id >= a.pages) {
+          report(a.status, a.status_host, kStatusBadPage);
+          return (int)(a.pages * a.page / 8);  // outside the map: zeros
         }
+        return (id * a.page + (pos - at * a.page)) / 8;
+      };
+      int next = place(sg.tile);
+      for (int t = sg.tile; t < sg.tile + sg.n && ok; ++t, ++n) {
+        const int y = next;
+        const bool mine = y >= 0;
+        next = place(t + 1);  // read ahead of the waits below
         const int count = __popc(__ballot_sync(0xffffffffu, mine));
         const uint32_t b = n & 1, use = n >> 1;
         for (at_half = 0; at_half < halves; ++at_half) {
@@ -362,19 +365,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- S^T = rows . Q^T ----------------
     // All lanes walk the loops, so that descriptors stay uniform; one waits and issues.
     const bool leader = elect_one();
-    constexpr uint32_t id_s = make_idesc_f16(kKeys, kHeads, bf16, false, false);
+    constexpr uint32_t id_s = make_idesc_f16(kKeys, N, bf16, false, false);
     const uint64_t qd0 = make_sw128_desc(smem_addr(q_smem));
     bool ok = true;
     for (uint32_t segments = 0; next_segment(a, cur, sg); ++segments) {
       if (leader) ok = ok && mbar_wait_fast(bar(&bars->q_full), segments & 1u, abort_flag);
       for (int t = 0; t < sg.n; ++t, ++n) {
-        const uint32_t b = n & 1, use = n >> 1, d = kSCol + b * kHeads;
+        const uint32_t b = n & 1, use = n >> 1, d = kSCol + b * N;
         // softmax has read the buffer's last tile
         if (leader && use) ok = ok && mbar_wait_fast(bar(&bars->p_full[b]), (use - 1) & 1u, abort_flag);
         for (int h = 0; h < halves; ++h) {
           const uint64_t kd = make_sw128_desc(smem_addr(kv_smem) + b * kStageBytes + h * half_bytes,
                                               a.half[h] * kAtomBytes);
-          const uint64_t qd = qd0 + (uint64_t)((h * half_bytes) >> 4);
+          const uint64_t qd = qd0 + (uint64_t)((h * a.half[0] * N * 128) >> 4);
           const int chunks = a.half[h];
           if (leader) {
             ok = ok && mbar_wait_fast(bar(&bars->full[b][h]), use & 1u, abort_flag);
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int c = 0; c < chunks; ++c) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  mma_f16_ss(d, kd + c * (kAtomBytes >> 4) + 2 * k, qd + c * (kChunkBytes >> 4) + 2 * k, id_s,
+                  mma_f16_ss(d, kd + c * (kAtomBytes >> 4) + 2 * k, qd + c * (N * 128 >> 4) + 2 * k, id_s,
                              (h | c | k) != 0);
               }
             }
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 6) {
     // ---------------- O^T += c^T . P^T ----------------
     const bool leader = elect_one();
-    constexpr uint32_t id_o = make_idesc_f16(128, kHeads, bf16, true, true);
+    constexpr uint32_t id_o = make_idesc_f16(128, N, bf16, true, true);
     const uint64_t pd = make_sw128_mn_desc(smem_addr(p_smem), kChunkBytes);
     const int groups0 = min(groups, a.half[0] / 2);
     bool ok = true;
@@ -425,10 +428,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint64_t v = vd + (uint64_t)((g - g0) * (2 * kAtomBytes >> 4));
               if (steps == 4) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_f16_ss(g * kHeads, v + k * step, pd + 128 * k, id_o, (t | k) != 0);
+                for (int k = 0; k < 4; ++k) mma_f16_ss(g * N, v + k * step, pd + 128 * k, id_o, (t | k) != 0);
               } else {
                 for (int k = 0; k < steps; ++k)
-                  mma_f16_ss(g * kHeads, v + k * step, pd + 128 * k, id_o, (t | k) != 0);
+                  mma_f16_ss(g * N, v + k * step, pd + 128 * k, id_o, (t | k) != 0);
               }
             }
             mma_commit(bar(&bars->empty[b][h]));
@@ -450,9 +453,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     bool stop = false;
     for (int segment = 0; !stop && next_segment(a, cur, sg); ++segment) {
-      float m[16], l[16];
+      float m[N / 4], l[N / 4];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < N / 4; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.f;
       }
@@ -460,19 +463,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t b = n & 1, use = n >> 1;
         if (!mbar_wait_warp(bar(&bars->s_full[b]), use & 1u, abort_flag)) stop = true;
         const int valid = min(kKeys, sg.visible - (sg.tile + t) * kKeys);
-        float v[32];
+        float v[N / 2];
         bool grow = stop;
         if (!stop) {
           tmem_fence_after();
-          uint32_t w[32];
-          tmem_ld16x64(lanes + kSCol + b * kHeads, w);
+          uint32_t w[N / 2];
+          tmem_ld16_frag(lanes + kSCol + b * N, w);
           tmem_wait_ld();
           const bool in0 = k0 < valid, in1 = k0 + 8 < valid;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int i = 0; i < N / 2; ++i)
             v[i] = ((i & 2) ? in1 : in0) ? __uint_as_float(w[i]) * a.c : -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < N / 4; ++i) {
             const int e = (i >> 1) * 4 + (i & 1);
             grow |= fmaxf(v[e], v[e + 2]) > m[i] + kMaxSlack;
           }
@@ -492,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           stop = any_of(stop, 1, kSoftThreads);
           if (stop) break;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < N / 4; ++i) {
             const int e = (i >> 1) * 4 + (i & 1);
             float x = fmaxf(v[e], v[e + 2]);
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           bar_sync(1, kSoftThreads);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < N / 4; ++i) {
             const int h = 8 * (i >> 1) + h0 + (i & 1);
             const float top = fmaxf(m[i], fmaxf(fmaxf(bars->xchg[0][h], bars->xchg[1][h]),
                                                 fmaxf(bars->xchg[2][h], bars->xchg[3][h])));
@@ -514,22 +517,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           bar_sync(1, kSoftThreads);
           if (t > 0 && mbar_wait_warp(bar(&bars->o_done), (n - 1) & 1u, abort_flag)) {
             tmem_fence_after();
-            for (int o = 0; o < groups * kHeads; o += 32) {
-              uint32_t w[32];
-              tmem_ld32(lanes + o, w);
+            for (int o = 0; o < groups * N; o += 16) {
+              uint32_t w[16];
+              tmem_ld16(lanes + o, w);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                w[i] = __float_as_uint(__uint_as_float(w[i]) * bars->factor[(o & 32) + i]);
-              tmem_st32(lanes + o, w);
+              for (int i = 0; i < 16; ++i)
+                w[i] = __float_as_uint(__uint_as_float(w[i]) * bars->factor[(o & (N - 1)) + i]);
+              tmem_st16(lanes + o, w);
             }
             tmem_wait_st();
           }
         }
         // P^T: rows of keys, 64 heads of 2 bytes, 128-byte swizzle
-        uint32_t p0[8], p1[8];
+        uint32_t p0[N / 8], p1[N / 8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < N / 8; ++j) {
           const float s0 = m[2 * j] == -INFINITY ? 0.f : m[2 * j], s1 = m[2 * j + 1] == -INFINITY ? 0.f : m[2 * j + 1];
           const float a0 = ex2(v[4 * j] - s0), a1 = ex2(v[4 * j + 1] - s1);
           const float b0 = ex2(v[4 * j + 2] - s0), b1 = ex2(v[4 * j + 3] - s1);
@@ -540,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (n > 0) mbar_wait_warp(bar(&bars->o_done), (n - 1) & 1u, abort_flag);  // P^T of the last tile is read
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < N / 8; ++j) {
           uint8_t* at = p_smem + k0 * 128 + ((j ^ (k0 & 7)) << 4) + 2 * h0;
           *reinterpret_cast<uint32_t*>(at) = p0[j];
           *reinterpret_cast<uint32_t*>(at + 8 * 128) = p1[j];
@@ -555,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (stop) break;
       // row sums over the 64 keys of every strip
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < N / 4; ++i) {
         float x = l[i];
         x += __shfl_xor_sync(0xffffffffu, x, 4);
         x += __shfl_xor_sync(0xffffffffu, x, 8);
@@ -565,52 +568,54 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_sync(1, kSoftThreads);
       if (tid < 4) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) bars->top[8 * (i >> 1) + h0 + (i & 1)] = m[i];
+        for (int i = 0; i < N / 4; ++i) bars->top[8 * (i >> 1) + h0 + (i & 1)] = m[i];
       }
       bar_sync(1, kSoftThreads);
-      const int heads = min(kHeads, a.H - sg.g * kHeads);
+      const int heads = min(N, a.H - sg.g * N);
       const bool whole = sg.n == sg.tiles;
       const int64_t slot = 2 * (int64_t)blockIdx.x + (segment ? 1 : 0);
-      const int64_t first = (int64_t)sg.token * a.H + sg.g * kHeads;  // row of out
-      if (tid < kHeads) {
+      const int64_t first = (int64_t)sg.token * a.H + sg.g * N;  // row of out
+      if (tid < N) {
         const float sum = (bars->xchg[0][tid] + bars->xchg[1][tid]) + (bars->xchg[2][tid] + bars->xchg[3][tid]);
         const float top = bars->top[tid];
         bars->factor[tid] = 1.f / sum;
         if (!whole) {
-          a.pm[slot * kHeads + tid] = top;
-          a.pl[slot * kHeads + tid] = sum;
+          a.pm[slot * N + tid] = top;
+          a.pl[slot * N + tid] = sum;
         } else if (a.lse && tid < heads) {
           a.lse[first + tid] = ((top == -INFINITY ? 0.f : top) + log2f(sum)) * kLn2;
         }
       }
       bar_sync(1, kSoftThreads);
       tmem_fence_after();
-      for (int o = 0; o < groups * kHeads; o += 32) {
-        uint32_t w[32];
-        tmem_ld32(lanes + o, w);
+      // a thread holds 16 heads of one latent index: a store of one head is 128
+      // bytes a warp in FP32; for the 16-bit result lane pairs exchange values
+      const int odd = lane & 1;
+#pragma unroll 2
+      for (int o = 0; o < groups * N; o += 16) {
+        uint32_t w[16];
+        tmem_ld16(lanes + o, w);
+        const int hb = o & (N - 1), lim = heads - hb;
+        const int64_t col = (int64_t)(o / N) * 128 + tid;
         tmem_wait_ld();
-        const int d = (o >> 6) * 128 + tid, hb = o & 32;  // latent index, first head
-        const int lim = heads - hb;
         if (!whole) {
-          float* dst = a.po + (slot * kHeads + hb) * a.R + d;
+          float* part = a.po + (slot * N + hb) * a.R + col;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i < lim) dst[i * a.R] = __uint_as_float(w[i]);
+          for (int i = 0; i < 16; ++i)
+            if (i < lim) part[i * a.R] = __uint_as_float(w[i]);
         } else {
-          float f[32];
+          uint16_t* dst = a.out + (first + hb + odd) * a.R + (col - odd);
+          float f[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 4; ++i) {
             const float4 x = reinterpret_cast<const float4*>(bars->factor + hb)[i];
             f[4 * i] = x.x;
             f[4 * i + 1] = x.y;
             f[4 * i + 2] = x.z;
             f[4 * i + 3] = x.w;
           }
-          // lane pairs exchange values, so that a store holds two latent values
-          const int odd = lane & 1;
-          uint16_t* dst = a.out + (first + hb + odd) * a.R + (d - odd);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
+          for (int i = 0; i < 16; i += 2) {
             const float x0 = __uint_as_float(w[i]) * f[i], x1 = __uint_as_float(w[i + 1]) * f[i + 1];
             const float got = __shfl_xor_sync(0xffffffffu, odd ? x0 : x1, 1);
             if (i + odd < lim)
@@ -633,11 +638,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the partial results of units that several CTAs shared:
 //   o = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p,  M the largest m_p,
 // and fills what no CTA wrote (tokens that see nothing; with fill_tail those
-// outside every request).  Few results (WAYS = 8): a block takes a fourth of a
-// (token, head), and eight warps every eighth part of it.  Many (WAYS = 1): a
+// outside every request).  Few results (WAYS = 16): a block takes a fourth of a
+// (token, head), and each of 16 warps every 16th part of it.  Many (WAYS = 1): a
 // block takes a whole one.
 template <typename E, int WAYS>
-__global__ void __launch_bounds__(WAYS == 1 ? 128 : 32 * WAYS) join_kernel(Args a) {
+__global__ void __launch_bounds__(WAYS == 1 ? 128 : 32 * WAYS) join_kernel(Args a, int heads) {
   constexpr int kCols = WAYS == 1 ? 128 : 32;  // float4 columns a block
   __shared__ float weight[2 * kMaxGrid];
   __shared__ float4 part[WAYS][kCols];
@@ -653,12 +658,21 @@ __global__ void __launch_bounds__(WAYS == 1 ? 128 : 32 * WAYS) join_kernel(Args 
     if (a.lse && threadIdx.x == 0 && blockIdx.z == 0) a.lse[at] = -INFINITY;
     return;
   }
-  const int f = first + (h / kHeads) * n, c0 = f / run, c1 = (f + n - 1) / run, hl = h % kHeads;
+  const int f = first + (h / heads) * n, c0 = f / run, c1 = (f + n - 1) / run, hl = h % heads;
   if (c0 == c1) return;
   // a CTA's first segment is its slot 2 c, a last one that begins a unit 2 c + 1
   const bool late = f != c0 * run;
   const int parts = c1 - c0 + 1;
-  auto slot = [&](int p) { return (int64_t)(2 * (c0 + p) + (p == 0 && late ? 1 : 0)) * kHeads + hl; };
+  auto slot = [&](int p) { return (int64_t)(2 * (c0 + p) + (p == 0 && late ? 1 : 0)) * heads + hl; };
+  // the first rows are on their way while the weights are formed
+  constexpr int kBatch = 6;
+  float4 x[kBatch];
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k) {
+    const int p = way + k * WAYS;
+    x[k] = mine && p < parts ? *reinterpret_cast<const float4*>(a.po + slot(p) * a.R + col)
+                             : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   const int lane = threadIdx.x & 31;
   float top = -INFINITY, sum = 0.f;
   for (int p = lane; p < parts; p += 32) top = fmaxf(top, a.pm[slot(p)]);
@@ -673,15 +687,17 @@ __global__ void __launch_bounds__(WAYS == 1 ? 128 : 32 * WAYS) join_kernel(Args 
   sum = warp_sum(sum);
   __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (mine) {
-#pragma unroll 6
-    for (int p = way; p < parts; p += WAYS) {
-      const float w = weight[p];
-      const float4 x = *reinterpret_cast<const float4*>(a.po + slot(p) * a.R + col);
-      o.x = fmaf(w, x.x, o.x);
-      o.y = fmaf(w, x.y, o.y);
-      o.z = fmaf(w, x.z, o.z);
-      o.w = fmaf(w, x.w, o.w);
+  for (int p0 = way; p0 < parts; p0 += kBatch * WAYS) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int p = p0 + k * WAYS, next = p + kBatch * WAYS;
+      const float w = p < parts ? weight[p] : 0.f;
+      o.x = fmaf(w, x[k].x, o.x);
+      o.y = fmaf(w, x[k].y, o.y);
+      o.z = fmaf(w, x[k].z, o.z);
+      o.w = fmaf(w, x[k].w, o.w);
+      x[k] = mine && next < parts ? *reinterpret_cast<const float4*>(a.po + slot(next) * a.R + col)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
   if constexpr (WAYS > 1) {
@@ -708,7 +724,7 @@ __global__ void __launch_bounds__(WAYS == 1 ? 128 : 32 * WAYS) join_kernel(Args 
 int grid_size() { return std::min(sm_count(), kMaxGrid); }
 size_t plan_bytes(int64_t tokens) { return align_up((size_t)(2 * tokens + 1) * 4, 256); }
 size_t part_bytes(int64_t latent_dim) {
-  return 2 * (size_t)grid_size() * kHeads * ((size_t)latent_dim + 2) * sizeof(float);
+  return 2 * (size_t)grid_size() * kMaxHeads * ((size_t)latent_dim + 2) * sizeof(float);
 }
 
 bool stride_ok(int64_t s, int64_t count) {
@@ -734,19 +750,23 @@ int make_map(CUtensorMap* map, const void* base, bool bf16, int rank, const cuui
   return GLM53_OK;
 }
 
-template <typename E>
+template <typename E, int N>
 int launch(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMap& kv0, const CUtensorMap& kv1, const Args& a,
            cudaStream_t st) {
-  int rc = ensure_max_smem((const void*)absorbed_kernel<E>, kSmemBytes);
+  int rc = ensure_max_smem((const void*)absorbed_kernel<E, N>, kSmemBytes);
   if (rc) return rc;
-  absorbed_kernel<E><<<grid_size(), kThreads, kSmemBytes, st>>>(ql, qr, kv0, kv1, a);
+  absorbed_kernel<E, N><<<grid_size(), kThreads, kSmemBytes, st>>>(ql, qr, kv0, kv1, a);
   if ((rc = check_launch("absorbed_kernel"))) return rc;
   if (a.T * a.H <= 512)
-    launch_programmatic(join_kernel<E, 8>, dim3((unsigned)a.T, (unsigned)a.H, 4), dim3(256), 0, st, a);
+    launch_programmatic(join_kernel<E, 16>, dim3((unsigned)a.T, (unsigned)a.H, 4), dim3(512), 0, st, a, N);
   else
-    launch_programmatic(join_kernel<E, 1>, dim3((unsigned)a.T, (unsigned)a.H), dim3(128), 0, st, a);
+    launch_programmatic(join_kernel<E, 1>, dim3((unsigned)a.T, (unsigned)a.H), dim3(128), 0, st, a, N);
   return check_launch("join_kernel");
 }
+
+// Heads a unit: the fewest of 16, 32 and 64 that hold all heads, else 64.  A
+// unit of 16 heads pays a third of the MMA cycles of one of 64.
+int unit_heads(int64_t heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }
 
 }  // namespace
 }  // namespace latent
@@ -821,7 +841,8 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
   const cuuint64_t ql_dims[3] = {(cuuint64_t)latent_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
   const cuuint64_t ql_strides[2] = {(cuuint64_t)(ql_stride_h ? ql_stride_h : 8) * 2,
                                     (cuuint64_t)(ql_stride_t ? ql_stride_t : 8) * 2};
-  const cuuint32_t q_box[3] = {64, kHeads, 1};
+  const int unit = unit_heads(heads);
+  const cuuint32_t q_box[3] = {64, (cuuint32_t)unit, 1};
   int rc = make_map(&ql, q_latent, bf16, 3, ql_dims, ql_strides, q_box);
   if (rc) return rc;
   qr = kv0 = kv1 = ql;  // maps that no load reads (no rotary part, no pages, no second half)
@@ -847,13 +868,13 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
     if (half[1] && (rc = make_map(&kv1, cache, bf16, 4, dims, strides, kv_box))) return rc;
   }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const int64_t slots = 2 * (int64_t)grid_size() * kHeads;
+  const int64_t slots = 2 * (int64_t)grid_size() * kMaxHeads;
   Args a{};
   a.T = tokens;
   a.H = (int)heads;
   a.R = (int)latent_dim;
   a.r = (int)rope_dim;
-  a.G = (int)((heads + kHeads - 1) / kHeads);
+  a.G = (int)((heads + unit - 1) / unit);
   a.pages = pages;
   a.page = (int)page_size;
   a.box = box;
@@ -876,6 +897,12 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
   a.po = reinterpret_cast<float*>(ws + plan_bytes(tokens));
   a.pm = a.po + slots * latent_dim;
   a.pl = a.pm + slots;
-  return bf16 ? launch<__nv_bfloat16>(ql, qr, kv0, kv1, a, (cudaStream_t)stream)
-              : launch<__half>(ql, qr, kv0, kv1, a, (cudaStream_t)stream);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (bf16)
+    return unit == 16   ? launch<__nv_bfloat16, 16>(ql, qr, kv0, kv1, a, st)
+           : unit == 32 ? launch<__nv_bfloat16, 32>(ql, qr, kv0, kv1, a, st)
+                        : launch<__nv_bfloat16, 64>(ql, qr, kv0, kv1, a, st);
+  return unit == 16   ? launch<__half, 16>(ql, qr, kv0, kv1, a, st)
+         : unit == 32 ? launch<__half, 32>(ql, qr, kv0, kv1, a, st)
+                      : launch<__half, 64>(ql, qr, kv0, kv1, a, st);
 }
