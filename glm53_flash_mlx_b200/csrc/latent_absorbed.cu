@@ -30,7 +30,8 @@
 // two a CTA) that a second kernel joins.
 //
 // Roles: warps 0-3 softmax (a 16-key strip each) and epilogue, warp 4 TMA,
-// warp 5 issues S^T, warp 6 issues O^T.  Row maxima are replaced only when a
+// warp 5 issues S^T, warp 6 issues O^T; in the last three one lane waits and
+// issues, since a lane that spins must not hold up one with work.  Row maxima are replaced only when a
 // score passes them by 2^8 (latent.cuh).  A token never shares a tile's keys
 // with one that sees fewer, so only rows behind a request's end are masked:
 // their scores are replaced, and their values cleared in shared memory (a zero
@@ -296,24 +297,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 4) {
     // ---------------- TMA ----------------
+    // Lane 0 waits and issues; the lanes look up a tile's boxes side by side.
     const int boxes = kKeys / a.box, box_groups = a.box / 8;
     bool ok = true;
     uint32_t queries = 0;  // Q tiles asked for
     int at_half = 0;
-    while (ok && next_segment(a, cur, sg)) {
-      if (queries) ok = mbar_wait_warp(bar(&bars->q_empty), (queries - 1) & 1u, abort_flag);
-      if (!ok) break;
-      ++queries;
+    while (next_segment(a, cur, sg)) {
       if (lane == 0) {
-        mbar_expect_tx(bar(&bars->q_full), (a.R + a.r) / 64 * (N * 128));
-        for (int c = 0; c < a.R / 64; ++c)
-          tma_load_3d(smem_addr(q_smem + c * (N * 128)), &ql_map, c * 64, sg.g * N, sg.token,
-                      bar(&bars->q_full));
-        if (a.r)
-          tma_load_3d(smem_addr(q_smem + a.R / 64 * (N * 128)), &qr_map, 0, sg.g * N, sg.token,
-                      bar(&bars->q_full));
+        if (queries) ok = ok && mbar_wait_fast(bar(&bars->q_empty), (queries - 1) & 1u, abort_flag);
+        if (ok) {
+          ++queries;
+          mbar_expect_tx(bar(&bars->q_full), (a.R + a.r) / 64 * (N * 128));
+          for (int c = 0; c < a.R / 64; ++c)
+            tma_load_3d(smem_addr(q_smem + c * (N * 128)), &ql_map, c * 64, sg.g * N, sg.token, bar(&bars->q_full));
+          if (a.r)
+            tma_load_3d(smem_addr(q_smem + a.R / 64 * (N * 128)), &qr_map, 0, sg.g * N, sg.token,
+                        bar(&bars->q_full));
+        }
       }
-      // lane k fetches box k of a tile: rows pos .. pos + box of the request
+      __syncwarp();
+      // lane k looks up box k of a tile: rows pos .. pos + box of the request
       const int32_t* row = a.table + sg.request * a.table_stride;
       auto place = [&](int t) {  // group of eight rows in the cache, -1 for none
         const int pos = t * kKeys + lane * a.box;
@@ -327,28 +330,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         return (id * a.page + (pos - at * a.page)) / 8;
       };
       int next = place(sg.tile);
-      for (int t = sg.tile; t < sg.tile + sg.n && ok; ++t, ++n) {
-        const int y = next;
-        const bool mine = y >= 0;
+      for (int t = sg.tile; t < sg.tile + sg.n; ++t) {
+        const int count = __popc(__ballot_sync(0xffffffffu, next >= 0));
+        int y[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = __shfl_sync(0xffffffffu, next, k);
         next = place(t + 1);  // read ahead of the waits below
-        const int count = __popc(__ballot_sync(0xffffffffu, mine));
-        const uint32_t b = n & 1, use = n >> 1;
-        for (at_half = 0; at_half < halves; ++at_half) {
-          const int h = at_half;
-          if (use) ok = mbar_wait_warp(bar(&bars->empty[b][h]), (use - 1) & 1u, abort_flag);
-          if (!ok) break;
-          const int row_bytes = a.half[h] * kAtomBytes;  // eight rows
-          if (lane == 0) mbar_expect_tx(bar(&bars->full[b][h]), count * box_groups * row_bytes);
-          __syncwarp();
-          if (mine)
-            tma_load_4d(smem_addr(kv_smem + b * kStageBytes + h * half_bytes + lane * box_groups * row_bytes),
-                        h ? &kv1_map : &kv0_map, 0, 0, h ? a.half[0] : 0, y, bar(&bars->full[b][h]));
+        if (lane == 0 && ok) {
+          const uint32_t b = n & 1, use = n >> 1;
+          for (at_half = 0; at_half < halves; ++at_half) {
+            const int h = at_half;
+            if (use) ok = mbar_wait_fast(bar(&bars->empty[b][h]), (use - 1) & 1u, abort_flag);
+            if (!ok) break;
+            const int box_bytes = a.half[h] * kAtomBytes * box_groups;
+            mbar_expect_tx(bar(&bars->full[b][h]), count * box_bytes);
+            const uint32_t dst = smem_addr(kv_smem + b * kStageBytes + h * half_bytes);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (k < count)
+                tma_load_4d(dst + k * box_bytes, h ? &kv1_map : &kv0_map, 0, 0, h ? a.half[0] : 0, y[k],
+                            bar(&bars->full[b][h]));
+          }
+          if (ok) {
+            at_half = 0;
+            ++n;
+          }
         }
-        if (!ok) break;
-        at_half = 0;
+        __syncwarp();
       }
     }
-    if (!ok && lane == 0) {
+    if (!ok) {
       // copies still in flight write this CTA's shared memory: wait for them
       volatile int never = 0;
       if (queries) mbar_wait(bar(&bars->q_full), (queries - 1) & 1u, &never);
@@ -396,11 +407,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (leader && ok) mma_commit(bar(&bars->q_empty));
     }
-    __syncwarp();
-    volatile int never = 0;
-    if (leader) mma_commit(bar(&bars->drain[0]));
-    __syncwarp();
-    mbar_wait(bar(&bars->drain[0]), 0, &never);
+    // no MMA is in flight when TMEM is freed; a lane that spins must not keep its
+    // warp from one with work, so the lane that issued waits alone
+    if (leader) {
+      volatile int never = 0;
+      mma_commit(bar(&bars->drain[0]));
+      if (!mbar_wait(bar(&bars->drain[0]), 0, &never)) *abort_flag = 1;
+    }
     __syncwarp();
   } else if (warp == 6) {
     // ---------------- O^T += c^T . P^T ----------------
@@ -440,11 +453,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (leader && ok) mma_commit(bar(&bars->o_done));
       }
     }
-    __syncwarp();
-    volatile int never = 0;
-    if (leader) mma_commit(bar(&bars->drain[1]));
-    __syncwarp();
-    mbar_wait(bar(&bars->drain[1]), 0, &never);
+    // no MMA is in flight when TMEM is freed; a lane that spins must not keep its
+    // warp from one with work, so the lane that issued waits alone
+    if (leader) {
+      volatile int never = 0;
+      mma_commit(bar(&bars->drain[1]));
+      if (!mbar_wait(bar(&bars->drain[1]), 0, &never)) *abort_flag = 1;
+    }
     __syncwarp();
   } else {
     // ---------------- softmax, epilogue ----------------

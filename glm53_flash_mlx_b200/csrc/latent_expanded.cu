@@ -69,7 +69,7 @@ struct Args {
 };
 
 struct __align__(8) Bars {
-  uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], o_done, drain;
+  uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], o_done[2], drain;
   uint32_t tmem_base;
   int abort_flag;
   int poison;                       // a masked tile holds values that are not finite
@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar(&bars->s_full[s]), 1);
       mbar_init(bar(&bars->p_full[s]), kSoftWarps);
+      mbar_init(bar(&bars->o_done[s]), 1);
     }
-    mbar_init(bar(&bars->o_done), 1);
     mbar_init(bar(&bars->drain), 1);
     bars->abort_flag = 0;
     bars->poison = 0;
@@ -298,75 +298,82 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 9) {
     // ---------------- MMA ----------------
-    // The whole warp walks the loop and one elected lane issues, so that
-    // descriptors stay in uniform registers; eight MMAs a slot are unrolled.
+    // All lanes walk the loops, so that descriptors stay in uniform registers;
+    // one elected lane waits and issues, eight unrolled MMAs a slot.
     if (tiles > 0) {
       constexpr bool bf16 = std::is_same<E, __nv_bfloat16>::value;
       constexpr uint32_t id_s = make_idesc_f16(kTile, kTile, bf16, false, false);
       const bool leader = elect_one();
-      uint32_t seq = 0, s = 0;
-      bool ok = __all_sync(0xffffffffu, mbar_wait(bar(&bars->q_full), 0, abort_flag));
+      uint32_t seq = 0;
+      bool ok = true;
       const uint64_t qd = make_sw128_desc(smem_addr(q_smem));
       const uint64_t kd0 = make_sw128_desc(smem_addr(ring)), vd0 = make_sw128_mn_desc(smem_addr(ring), kChunkBytes);
-      auto take = [&]() {
-        s = seq % kSlots;
-        __syncwarp();
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(&bars->full[s]), (seq / kSlots) & 1u, abort_flag));
-        ++seq;
-        tmem_fence_after();
-        return ok;
-      };
-      for (int t = 0; t <= tiles && ok; ++t) {
+      if (leader) ok = mbar_wait_fast(bar(&bars->q_full), 0, abort_flag);
+      for (int t = 0; t <= tiles; ++t) {
         if (t < tiles) {
           const uint32_t d = kSCol + (t & 1) * kTile;
-          for (int p = 0; p < kslots && take(); ++p) {
+          for (int p = 0; p < kslots; ++p, ++seq) {
+            const uint32_t s = seq % kSlots, phase = (seq / kSlots) & 1u;
             const uint64_t ad = qd + (uint64_t)(p * (kSlotBytes >> 4));
             const uint64_t kd = kd0 + (uint64_t)(s * (kSlotBytes >> 4));
             if (leader) {
+              ok = ok && mbar_wait_fast(bar(&bars->full[s]), phase, abort_flag);
+              tmem_fence_after();
+              if (ok) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_f16_ss(d, ad + 2 * k, kd + 2 * k, id_s, (p | k) != 0);
-              if (2 * p + 1 < nch) {
+                for (int k = 0; k < 4; ++k) mma_f16_ss(d, ad + 2 * k, kd + 2 * k, id_s, (p | k) != 0);
+                if (2 * p + 1 < nch) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  mma_f16_ss(d, ad + (kChunkBytes >> 4) + 2 * k, kd + (kChunkBytes >> 4) + 2 * k, id_s, 1);
+                  for (int k = 0; k < 4; ++k)
+                    mma_f16_ss(d, ad + (kChunkBytes >> 4) + 2 * k, kd + (kChunkBytes >> 4) + 2 * k, id_s, 1);
+                }
+                mma_commit(bar(&bars->empty[s]));
               }
-              mma_commit(bar(&bars->empty[s]));
             }
           }
-          if (ok && leader) mma_commit(bar(&bars->s_full[t & 1]));
+          if (leader && ok) mma_commit(bar(&bars->s_full[t & 1]));
         }
-        if (t > 0 && ok) {
+        if (t > 0) {
           const int u = t - 1;
-          __syncwarp();
-          ok = __all_sync(0xffffffffu, mbar_wait(bar(&bars->p_full[u & 1]), (u >> 1) & 1u, abort_flag));
           const uint32_t pa = kSCol + (u & 1) * kTile;
           const int steps = (min(kTile, nk - u * kTile) + 15) >> 4;
-          for (int p = 0; p < vslots && take(); ++p) {
+          if (leader) ok = ok && mbar_wait_fast(bar(&bars->p_full[u & 1]), (u >> 1) & 1u, abort_flag);
+          for (int p = 0; p < vslots; ++p, ++seq) {
+            const uint32_t s = seq % kSlots, phase = (seq / kSlots) & 1u;
             const uint32_t id_o = 2 * p + 1 < vch ? make_idesc_f16(kTile, 128, bf16, false, true)
                                                   : make_idesc_f16(kTile, 64, bf16, false, true);
             const uint64_t vd = vd0 + (uint64_t)(s * (kSlotBytes >> 4));
             const uint32_t o = kOCol + p * 128;
             if (leader) {
-              if (steps == 8) {
+              ok = ok && mbar_wait_fast(bar(&bars->full[s]), phase, abort_flag);
+              tmem_fence_after();
+              if (ok) {
+                if (steps == 8) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
-              } else {
-                for (int k = 0; k < steps; ++k) mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
+                  for (int k = 0; k < 8; ++k) mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
+                } else {
+                  for (int k = 0; k < steps; ++k) mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
+                }
+                mma_commit(bar(&bars->empty[s]));
               }
-              mma_commit(bar(&bars->empty[s]));
             }
           }
-          if (ok && leader) mma_commit(bar(&bars->o_done));
+          if (leader && ok) mma_commit(bar(&bars->o_done[u & 1]));
         }
       }
-      // no MMA is in flight when TMEM is freed
-      volatile int never = 0;
-      if (leader) mma_commit(bar(&bars->drain));
-      mbar_wait(bar(&bars->drain), 0, &never);
+      // no MMA is in flight when TMEM is freed.  The lane that issued waits
+      // alone: a lane that spins must not keep its warp from one with work.
+      if (leader) {
+        volatile int never = 0;
+        mma_commit(bar(&bars->drain));
+        if (!mbar_wait(bar(&bars->drain), 0, &never)) *abort_flag = 1;
+      }
     }
     __syncwarp();
   } else {
     // ---------------- softmax, epilogue ----------------
+    // When S of tile t is there, P V of tile t - 2 is done and that of t - 1
+    // may not be: two barriers by tile parity keep the waits unambiguous.
     const int quarter = warp & 3, half = warp >> 2;
     const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -378,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* xchg = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 1024);  // [2][128]
     for (int t = 0; t < tiles; ++t) {
       const int b = t & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(bar(&bars->s_full[b]), (t >> 1) & 1u, abort_flag))) {
+      if (!__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->s_full[b]), (t >> 1) & 1u, abort_flag))) {
         stop = true;
       }
       float v[64];
@@ -418,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l *= f;
         if (t > 0) {
           // (a warp whose wait gives up goes on: all stop at the next tile)
-          if (__all_sync(0xffffffffu, mbar_wait(bar(&bars->o_done), (t - 1) & 1u, abort_flag))) {
+          if (__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(t - 1) & 1]), ((t - 1) >> 1) & 1u, abort_flag))) {
             tmem_fence_after();
             for (int o = 0; o < ocols; o += 32) {
               uint32_t w[32];
@@ -446,12 +453,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         // tile t - 1 is multiplied, each slot's previous use is over and its
         // barrier's parity means this one
         const uint32_t s0 = kslots + t * (kslots + vslots) + (t + 1 < tiles ? kslots : 0);
-        bool ready = t == 0 || __all_sync(0xffffffffu, mbar_wait(bar(&bars->o_done), (t - 1) & 1u, abort_flag));
+        bool ready = t == 0 || __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(t - 1) & 1]), ((t - 1) >> 1) & 1u, abort_flag));
         bool found = false;
         for (int c = 0; c < vch && ready; ++c) {
           const uint32_t q = s0 + (c >> 1), s = q % kSlots;
           if (!(c & 1))
-            ready = __all_sync(0xffffffffu, mbar_wait(bar(&bars->full[s]), (q / kSlots) & 1u, abort_flag));
+            ready = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->full[s]), (q / kSlots) & 1u, abort_flag));
           if (ready)
             found |= clean_chunk<E>(ring + s * kSlotBytes + (c & 1) * kChunkBytes, tid, nk - t * kTile);
         }
@@ -464,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(bar(&bars->p_full[b]));
     }
     if (!stop && tiles > 0)
-      stop = !__all_sync(0xffffffffu, mbar_wait(bar(&bars->o_done), (tiles - 1) & 1u, abort_flag));
+      stop = !__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(tiles - 1) & 1]), ((tiles - 1) >> 1) & 1u, abort_flag));
     stop = any_of(stop, 1, kSoftThreads);
     if (!stop) {
       tmem_fence_after();
