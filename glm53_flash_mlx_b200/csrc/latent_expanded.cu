@@ -20,15 +20,16 @@
 // values) share in the order the MMAs take them.
 //
 // Roles: warps 0-7 softmax (two threads a row, 64 keys each) and epilogue,
-// warp 8 TMA, warp 9 MMA.  Every mbarrier wait is bounded; a CTA that gives up
+// warp 8 TMA, warp 9 MMA, warps 10 and 11 clean values (below).  Every mbarrier wait is bounded; a CTA that gives up
 // sets GLM53_STATUS_WAIT_TIMEOUT, waits for its copies and MMAs, frees its
 // TMEM and exits.
 //
 // Masked places must not enter, whatever they hold.  Masked scores are
 // replaced before the maximum.  A masked weight is 0, but 0 x NaN is not, so on
-// the tiles that the mask cuts the softmax warps clear value rows behind the
-// request's last key and values that are not finite before the product reads
-// them; the epilogue then adds the latter to the rows that do see them.
+// the tiles that the mask cuts two warps clear value rows behind the request's
+// last key and values that are not finite, under the softmax and before the
+// product reads them; the epilogue then adds the latter to the rows that do
+// see them.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -49,7 +50,8 @@ constexpr int kSlotBytes = 2 * kChunkBytes;
 constexpr int kSlots = 5;
 constexpr int kSoftWarps = 8;
 constexpr int kSoftThreads = kSoftWarps * 32;
-constexpr int kThreads = kSoftThreads + 64;
+constexpr int kCleanWarps = 2;
+constexpr int kThreads = kSoftThreads + 128;
 constexpr int kOCol = 0;     // TMEM: O at 0..255, S tiles at 256 and 384
 constexpr int kSCol = 256;
 
@@ -73,8 +75,10 @@ struct __align__(8) Bars {
   uint32_t tmem_base;
   int abort_flag;
   int poison;                       // a masked tile holds values that are not finite
-  int request, first, total;        // this CTA's request, its first query row in it, tiles in all
-  int warp_sum[kThreads / 32 + 1];
+  int found;                        // this CTA has a query tile
+  int first;                        // its first query row in the request
+  int64_t q0, k0, nq, nk;           // the request's rows
+  int warp_sum[kThreads / 32];
 };
 
 // alignment slack, Q, ring, barriers, two floats a row
@@ -106,46 +110,48 @@ __device__ __forceinline__ Bounds bounds_of(const Args& a, int i) {
   return b;
 }
 
+// Infinities and NaN: the exponent bits are all ones.
+template <typename E>
+constexpr uint32_t kExponent = std::is_same<E, __half>::value ? 0x7C00u : 0x7F80u;
 template <typename E>
 __device__ __forceinline__ bool not_finite(uint32_t half) {
-  constexpr uint32_t mask = std::is_same<E, __half>::value ? 0x7C00u : 0x7F80u;
-  return (half & mask) == mask;
+  return (half & kExponent<E>) == kExponent<E>;
+}
+// Bit 15 (31) is set when the lower (upper) half is not finite: adding the
+// exponent's lowest bit to an exponent of ones carries into it.
+template <typename E>
+__device__ __forceinline__ uint32_t not_finite_bits(uint32_t w) {
+  constexpr uint32_t both = kExponent<E> * 0x10001u, low = (kExponent<E> & (0u - kExponent<E>)) * 0x10001u;
+  return ((w & both) + low) & 0x80008000u;
 }
 
-// Clears, in the value rows of one key tile, rows >= valid and values that are
-// not finite; true when there were any of the latter.  Thread i of 256 takes
-// row i % 128 and every second 16-byte piece.
+// Clears row `row` of a 64-value chunk of one key tile's values where it lies
+// behind the last valid key, and its values that are not finite elsewhere;
+// true when there were any of the latter.
 template <typename E>
-__device__ __forceinline__ bool clean_chunk(uint8_t* chunk, int tid, int valid) {
-  const int row = tid & 127, half = tid >> 7;
-  if (row >= ((valid + 15) & ~15)) return false;  // the product stops there
-  bool found = false;
-  uint8_t* line = chunk + row * 128;
+__device__ __forceinline__ bool clean_row(uint8_t* chunk, int row, int valid) {
+  uint4* line = reinterpret_cast<uint4*>(chunk + row * 128);
+  if (row >= valid) {
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    uint4* at = reinterpret_cast<uint4*>(line + 16 * ((2 * p + half) ^ (row & 7)));
-    uint4 w = *at;
-    uint32_t x[4] = {w.x, w.y, w.z, w.w};
-    bool dirty = false;
-    if (row >= valid) {
-      dirty = true;
-      x[0] = x[1] = x[2] = x[3] = 0;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (not_finite<E>(x[k])) {
-          x[k] &= 0xFFFF0000u;
-          dirty = found = true;
-        }
-        if (not_finite<E>(x[k] >> 16)) {
-          x[k] &= 0x0000FFFFu;
-          dirty = found = true;
-        }
-      }
-    }
-    if (dirty) *at = make_uint4(x[0], x[1], x[2], x[3]);
+    for (int p = 0; p < 8; ++p) line[p ^ (row & 7)] = make_uint4(0, 0, 0, 0);
+    return false;
   }
-  return found;
+  uint4 w[8];
+  uint32_t any = 0;
+#pragma unroll
+  for (int p = 0; p < 8; ++p) w[p] = line[p ^ (row & 7)];
+#pragma unroll
+  for (int p = 0; p < 8; ++p)
+    any |= not_finite_bits<E>(w[p].x) | not_finite_bits<E>(w[p].y) | not_finite_bits<E>(w[p].z) |
+           not_finite_bits<E>(w[p].w);
+  if (!any) return false;
+  auto clean = [](uint32_t x) {
+    return (not_finite<E>(x) ? 0u : x & 0xFFFFu) | (not_finite<E>(x >> 16) ? 0u : x & 0xFFFF0000u);
+  };
+#pragma unroll
+  for (int p = 0; p < 8; ++p)
+    line[p ^ (row & 7)] = make_uint4(clean(w[p].x), clean(w[p].y), clean(w[p].z), clean(w[p].w));
+  return true;
 }
 
 template <typename E>
@@ -162,14 +168,46 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int head = blockIdx.y;
   auto bar = [&](uint64_t* p) { return smem_addr(p); };
 
+  if (tid == 0) {
+    bars->found = 0;
+    bars->abort_flag = 0;
+    bars->poison = 0;
+    mbar_init(bar(&bars->q_full), 1);
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(bar(&bars->full[s]), 1);
+      mbar_init(bar(&bars->empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(&bars->s_full[s]), 1);
+      mbar_init(bar(&bars->p_full[s]), kSoftWarps + kCleanWarps);
+      mbar_init(bar(&bars->o_done[s]), 1);
+    }
+    mbar_init(bar(&bars->drain), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(&bars->tmem_base)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (warp == 8 && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qn_map)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qr_map)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kn_map)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kr_map)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
+  }
+  __syncwarp();
+
   // which request and query tile: count tiles over the requests, a block's
   // worth at a time
-  if (tid == 0) bars->request = -1;
   int base = 0;
   for (int r0 = 0; r0 < a.B; r0 += kThreads) {
     int n = 0;
+    Bounds b{};
     if (r0 + tid < a.B) {
-      const Bounds b = bounds_of(a, r0 + tid);
+      b = bounds_of(a, r0 + tid);
       n = (int)((b.nq + kTile - 1) / kTile);
       if (b.bad && blockIdx.x == 0 && head == 0) report(a.status, a.status_host, kStatusBadGeometry);
     }
@@ -182,22 +220,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 31) bars->warp_sum[warp] = s;
     __syncthreads();
     int before = base;
+#pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) before += bars->warp_sum[w];
       base += bars->warp_sum[w];
     }
     const int lo = before + s - n;
     if ((int)blockIdx.x >= lo && (int)blockIdx.x < lo + n) {
-      bars->request = r0 + tid;
+      bars->found = 1;
       // the later query tiles see more keys: they go first
       bars->first = (n - 1 - ((int)blockIdx.x - lo)) * kTile;
+      bars->q0 = b.q0;
+      bars->nq = b.nq;
+      bars->k0 = b.k0;
+      bars->nk = b.nk;
     }
-    __syncthreads();
     if (base > (int)blockIdx.x) break;
+    __syncthreads();
   }
+  tmem_fence_before();
   __syncthreads();
-  const int request = bars->request;
-  if (request < 0) {
+  tmem_fence_after();
+  if (!bars->found) {
+    if (warp == 9)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars->tmem_base), "r"(512) : "memory");
     // surplus CTAs zero the rows outside every request
     if (a.fill_tail) {
       int64_t lo = a.B ? a.q_starts[a.B] : 0, hi = a.B ? a.q_starts[0] : 0;
@@ -215,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     return;
   }
-  const Bounds bd = bounds_of(a, request);
+  const Bounds bd{bars->q0, bars->nq, bars->k0, bars->nk, false};
   const int j0 = bars->first;
   const int rows = (int)(bd.nq - j0 < kTile ? bd.nq - j0 : kTile);
   const int nk = (int)bd.nk;
@@ -225,32 +271,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int nch = (a.dn + a.dr) / 64, kslots = (nch + 1) / 2, vch = a.dv / 64, vslots = (vch + 1) / 2;
   const int64_t q0 = bd.q0 + j0, k0 = bd.k0;
 
-  if (tid == 0) {
-    mbar_init(bar(&bars->q_full), 1);
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(bar(&bars->full[s]), 1);
-      mbar_init(bar(&bars->empty[s]), 1);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(bar(&bars->s_full[s]), 1);
-      mbar_init(bar(&bars->p_full[s]), kSoftWarps);
-      mbar_init(bar(&bars->o_done[s]), 1);
-    }
-    mbar_init(bar(&bars->drain), 1);
-    bars->abort_flag = 0;
-    bars->poison = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_addr(&bars->tmem_base)),
-                 "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  tmem_fence_before();
-  __syncthreads();
-  tmem_fence_after();
   constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's
   volatile int* abort_flag = &bars->abort_flag;
 
@@ -370,6 +390,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
+  } else if (warp >= 10) {
+    // ---------------- values of the tiles that the mask cuts ----------------
+    bool ok = true;
+    for (int t = 0; t < tiles; ++t) {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->s_full[t & 1]), (t >> 1) & 1u, abort_flag));
+      if ((t + 1) * kTile > vis0 && ok) {
+        // value slots of tile t in the order the producer fills the ring; once
+        // tile t - 1 is multiplied, each slot's previous use is over and its
+        // barrier's parity means this one
+        if (t > 0)
+          ok = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(t - 1) & 1]), ((t - 1) >> 1) & 1u, abort_flag));
+        const uint32_t s0 = kslots + t * (kslots + vslots) + (t + 1 < tiles ? kslots : 0);
+        const int valid = min(kTile, nk - t * kTile), end = (valid + 15) & ~15;  // the product stops at `end`
+        bool found = false;
+        for (int c = 0; c < vch && ok; ++c) {
+          const uint32_t q = s0 + (c >> 1), s = q % kSlots;
+          if (!(c & 1))
+            ok = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->full[s]), (q / kSlots) & 1u, abort_flag));
+          for (int row = tid - 320; row < end && ok; row += 64)
+            found |= clean_row<E>(ring + s * kSlotBytes + (c & 1) * kChunkBytes, row, valid);
+        }
+        if (found) bars->poison = 1;
+        fence_async_shared();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(&bars->p_full[t & 1]));
+      __syncwarp();
+    }
   } else {
     // ---------------- softmax, epilogue ----------------
     // When S of tile t is there, P V of tile t - 2 is done and that of t - 1
@@ -381,7 +429,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int ocols = a.dv >> 1, o0 = half * ocols;  // this thread's result columns
     float m = -INFINITY, l = 0.f;
     bool stop = false;
-    int first_masked = tiles;  // first tile that the mask cuts
     float* xchg = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 1024);  // [2][128]
     for (int t = 0; t < tiles; ++t) {
       const int b = t & 1;
@@ -404,7 +451,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int key0 = t * kTile + half * 64;
       const bool masked = (t + 1) * kTile > vis0;
       if (masked) {
-        first_masked = min(first_masked, t);
 #pragma unroll
         for (int i = 0; i < 64; ++i) v[i] = key0 + i < vis ? v[i] : -INFINITY;
       }
@@ -448,27 +494,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         w[i] = Elem<E>::pack(p0, p1);
       }
       tmem_st32(tmem + lanes + kSCol + b * kTile + half * 32, w);
-      if (masked) {
-        // value slots of tile t in the order the producer fills the ring; once
-        // tile t - 1 is multiplied, each slot's previous use is over and its
-        // barrier's parity means this one
-        const uint32_t s0 = kslots + t * (kslots + vslots) + (t + 1 < tiles ? kslots : 0);
-        bool ready = t == 0 || __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(t - 1) & 1]), ((t - 1) >> 1) & 1u, abort_flag));
-        bool found = false;
-        for (int c = 0; c < vch && ready; ++c) {
-          const uint32_t q = s0 + (c >> 1), s = q % kSlots;
-          if (!(c & 1))
-            ready = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->full[s]), (q / kSlots) & 1u, abort_flag));
-          if (ready)
-            found |= clean_chunk<E>(ring + s * kSlotBytes + (c & 1) * kChunkBytes, tid, nk - t * kTile);
-        }
-        if (found) bars->poison = 1;
-        fence_async_shared();
-      }
       tmem_wait_st();
       tmem_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(&bars->p_full[b]));
+      __syncwarp();
     }
     if (!stop && tiles > 0)
       stop = !__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(tiles - 1) & 1]), ((tiles - 1) >> 1) & 1u, abort_flag));
@@ -483,30 +513,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t at = (q0 + r) * a.H + head;
       if (r < rows && a.lse && half == 0)
         a.lse[at] = vis > 0 ? ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2 : -INFINITY;
+      // 16-bit rows into the Q buffer (every S is done), pieces of 16 bytes
+      // swizzled by row, then whole rows to memory
+      const int row_bytes = a.dv * 2;
       for (int o = 0; o < ocols; o += 32) {
         uint32_t w[32];
         if (tiles > 0) {
           tmem_ld32(tmem + lanes + kOCol + o0 + o, w);
           tmem_wait_ld();
         }
-        if (r < rows) {
-          float f[32];
+        float f[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = vis > 0 ? __uint_as_float(w[i]) * inv : 0.f;
-          if (poison) {
-            for (int k = first_masked * kTile; k < vis; ++k) {
-              const uint16_t* src = a.v + (k0 + k) * a.v_t + head * a.v_h + o0 + o;
+        for (int i = 0; i < 32; ++i) f[i] = vis > 0 ? __uint_as_float(w[i]) * inv : 0.f;
+        if (poison) {
+          for (int k = vis0 / kTile * kTile; k < vis; ++k) {
+            const uint16_t* src = a.v + (k0 + k) * a.v_t + head * a.v_h + o0 + o;
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (not_finite<E>(src[i])) f[i] += Elem<E>::to_float(src[i]);
-            }
+            for (int i = 0; i < 32; ++i)
+              if (not_finite<E>(src[i])) f[i] += Elem<E>::to_float(src[i]);
           }
-          uint4* dst = reinterpret_cast<uint4*>(a.out + at * a.dv + o0 + o);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            dst[i] = make_uint4(Elem<E>::pack(f[8 * i], f[8 * i + 1]), Elem<E>::pack(f[8 * i + 2], f[8 * i + 3]),
-                                Elem<E>::pack(f[8 * i + 4], f[8 * i + 5]), Elem<E>::pack(f[8 * i + 6], f[8 * i + 7]));
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(q_smem + r * row_bytes + 16 * (((o0 + o) / 8 + i) ^ (r & 7))) =
+              make_uint4(Elem<E>::pack(f[8 * i], f[8 * i + 1]), Elem<E>::pack(f[8 * i + 2], f[8 * i + 3]),
+                         Elem<E>::pack(f[8 * i + 4], f[8 * i + 5]), Elem<E>::pack(f[8 * i + 6], f[8 * i + 7]));
+      }
+      bar_sync(1, kSoftThreads);
+      const int pieces = a.dv >> 3;
+      uint4* out = reinterpret_cast<uint4*>(a.out + (q0 * a.H + head) * a.dv);
+      if (lane < pieces) {
+#pragma unroll 4
+        for (int row = warp; row < rows; row += kSoftWarps)
+          out[(int64_t)row * a.H * pieces + lane] =
+              *reinterpret_cast<const uint4*>(q_smem + row * row_bytes + 16 * (lane ^ (row & 7)));
       }
     }
     tmem_fence_before();
