@@ -60,7 +60,8 @@ struct Args {
   int H, dn, dr, dv;
   const int32_t *q_starts, *k_starts;
   int B;
-  float c;  // scale log2(e)
+  float c;       // |scale| log2(e), not 0: a masked score is -inf and stays that
+  int negative;  // the scale's sign
   int causal;
   const uint16_t* v;
   int64_t v_t, v_h;
@@ -71,7 +72,7 @@ struct Args {
 };
 
 struct __align__(8) Bars {
-  uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], o_done[2], drain;
+  uint64_t q_full, full[kSlots], empty[kSlots], cut_full[2], s_full[2], p_full[2], o_done[2], drain;
   uint32_t tmem_base;
   int abort_flag;
   int poison;                       // a masked tile holds values that are not finite
@@ -154,7 +155,7 @@ __device__ __forceinline__ bool clean_row(uint8_t* chunk, int row, int valid) {
   return true;
 }
 
-template <typename E>
+template <typename E, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     expanded_kernel(const __grid_constant__ CUtensorMap qn_map, const __grid_constant__ CUtensorMap qr_map,
                     const __grid_constant__ CUtensorMap kn_map, const __grid_constant__ CUtensorMap kr_map,
@@ -166,6 +167,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   Bars* bars = reinterpret_cast<Bars*>(ring + kSlots * kSlotBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int head = blockIdx.y;
+  constexpr int kCtas = PAIR ? 2 : 1, kUnit = kCtas * kTile;  // queries a CTA or pair takes
+  const int rank = PAIR ? (int)cluster_rank() : 0;
+  const int unit = (int)blockIdx.x / kCtas;
   auto bar = [&](uint64_t* p) { return smem_addr(p); };
 
   if (tid == 0) {
@@ -178,19 +182,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(&bars->empty[s]), 1);
     }
     for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(&bars->cut_full[s]), 1);
       mbar_init(bar(&bars->s_full[s]), 1);
-      mbar_init(bar(&bars->p_full[s]), kSoftWarps + kCleanWarps);
+      mbar_init(bar(&bars->p_full[s]), kCtas * (kSoftWarps + kCleanWarps));
       mbar_init(bar(&bars->o_done[s]), 1);
     }
     mbar_init(bar(&bars->drain), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_addr(&bars->tmem_base)),
-                 "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_alloc_all<PAIR>(smem_addr(&bars->tmem_base));
   } else if (warp == 8 && lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qn_map)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qr_map)) : "memory");
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Bounds b{};
     if (r0 + tid < a.B) {
       b = bounds_of(a, r0 + tid);
-      n = (int)((b.nq + kTile - 1) / kTile);
+      n = (int)((b.nq + kUnit - 1) / kUnit);
       if (b.bad && blockIdx.x == 0 && head == 0) report(a.status, a.status_host, kStatusBadGeometry);
     }
     int s = n;
@@ -226,24 +227,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       base += bars->warp_sum[w];
     }
     const int lo = before + s - n;
-    if ((int)blockIdx.x >= lo && (int)blockIdx.x < lo + n) {
+    if (unit >= lo && unit < lo + n) {
       bars->found = 1;
       // the later query tiles see more keys: they go first
-      bars->first = (n - 1 - ((int)blockIdx.x - lo)) * kTile;
+      bars->first = (n - 1 - (unit - lo)) * kUnit;
       bars->q0 = b.q0;
       bars->nq = b.nq;
       bars->k0 = b.k0;
       bars->nk = b.nk;
     }
-    if (base > (int)blockIdx.x) break;
+    if (base > unit) break;
     __syncthreads();
   }
   tmem_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the other CTA's barriers are set up
   tmem_fence_after();
   if (!bars->found) {
-    if (warp == 9)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars->tmem_base), "r"(512) : "memory");
+    if (warp == 9) tmem_free_all<PAIR>(bars->tmem_base);
     // surplus CTAs zero the rows outside every request
     if (a.fill_tail) {
       int64_t lo = a.B ? a.q_starts[a.B] : 0, hi = a.B ? a.q_starts[0] : 0;
@@ -251,141 +252,208 @@ __global__ void __launch_bounds__(kThreads, 1)
       hi = hi < 0 ? 0 : (hi > a.Tq ? a.Tq : hi);
       const int64_t rows = hi + (a.Tq > lo ? a.Tq - lo : 0);
       const int pieces = a.dv >> 3;
-      const int64_t step = (int64_t)(gridDim.x - base) * kThreads;
-      for (int64_t i = (int64_t)(blockIdx.x - base) * kThreads + tid; i < rows * pieces; i += step) {
+      const int64_t step = (int64_t)(gridDim.x - base * kCtas) * kThreads;
+      for (int64_t i = (int64_t)(blockIdx.x - base * kCtas) * kThreads + tid; i < rows * pieces; i += step) {
         const int64_t k = i / pieces, row = k < hi ? k : lo + (k - hi);
         const int64_t at = row * a.H + head;
         reinterpret_cast<uint4*>(a.out + at * a.dv)[i - k * pieces] = make_uint4(0, 0, 0, 0);
         if (a.lse && i == k * pieces) a.lse[at] = -INFINITY;
       }
     }
+    if constexpr (PAIR) cluster_sync();
     return;
   }
   const Bounds bd{bars->q0, bars->nq, bars->k0, bars->nk, false};
-  const int j0 = bars->first;
-  const int rows = (int)(bd.nq - j0 < kTile ? bd.nq - j0 : kTile);
+  const int first = bars->first, j0 = first + rank * kTile;
+  const int rows = (int)max((int64_t)0, min(bd.nq - j0, (int64_t)kTile));  // of this CTA
   const int nk = (int)bd.nk;
-  const int vis0 = a.causal ? (int)max((int64_t)0, min(bd.nk, bd.nk - bd.nq + j0 + 1)) : nk;  // row 0's keys
-  const int vis_last = a.causal ? (int)max((int64_t)0, min(bd.nk, bd.nk - bd.nq + j0 + rows)) : nk;
-  const int tiles = (vis_last + kTile - 1) / kTile;
-  const int nch = (a.dn + a.dr) / 64, kslots = (nch + 1) / 2, vch = a.dv / 64, vslots = (vch + 1) / 2;
+  // keys that query j of the request sees
+  auto seen = [&](int64_t j) {
+    return a.causal ? (int)max((int64_t)0, min(bd.nk, bd.nk - bd.nq + j + 1)) : nk;
+  };
+  const int vis0 = seen(j0);       // of this CTA's first row
+  const int unit_vis0 = seen(first);  // of the unit's first row
+  const int cut0 = unit_vis0 / kTile;  // first tile that the mask cuts for some row of the unit
+  const int tiles = (seen(min(bd.nq, (int64_t)first + kUnit) - 1) + kTile - 1) / kTile;
+  // A pair holds half the keys of a K tile (64 rows, four chunks a slot) and
+  // half the values of a V tile in each CTA.
+  constexpr int kKeyRows = kTile / kCtas, kKeyChunk = kKeyRows * 128, kKeyChunks = kSlotBytes / kKeyChunk;
+  const int nch = (a.dn + a.dr) / 64, kslots = (nch + kKeyChunks - 1) / kKeyChunks;
+  const int vch = a.dv / 64 / kCtas, vslots = (vch + 1) / 2;
   const int64_t q0 = bd.q0 + j0, k0 = bd.k0;
 
   constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's
   volatile int* abort_flag = &bars->abort_flag;
 
+  auto p_arrive = [&](int t) {
+    if constexpr (PAIR)
+      mbar_arrive_at_relaxed(bar(&bars->p_full[t & 1]), 0);
+    else
+      mbar_arrive(bar(&bars->p_full[t & 1]));
+  };
+
   if (warp == 8) {
     // ---------------- TMA ----------------
+    // full[s] counts the bytes of both CTAs of a pair, at rank 0.  The values of
+    // a tile that the mask cuts are counted at cut_full of the CTA that holds
+    // (and cleans) them; the product learns of them through p_full.
     if (lane == 0 && tiles > 0) {
-      mbar_expect_tx(bar(&bars->q_full), nch * kChunkBytes);
+      auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int z, uint64_t* p) {
+        if constexpr (PAIR)
+          tma_load_3d_at(dst, map, x, head, z, bar(p), 0);
+        else
+          tma_load_3d(dst, map, x, head, z, bar(p));
+      };
+      if (rank == 0) mbar_expect_tx(bar(&bars->q_full), kCtas * nch * kChunkBytes);
       for (int c = 0; c < nch; ++c) {
         const bool rope = c * 64 >= a.dn;
-        tma_load_3d(smem_addr(q_smem + c * kChunkBytes), rope ? &qr_map : &qn_map, rope ? 0 : c * 64, head, (int)q0,
-                    bar(&bars->q_full));
+        load(smem_addr(q_smem + c * kChunkBytes), rope ? &qr_map : &qn_map, rope ? 0 : c * 64, (int)q0, &bars->q_full);
       }
       uint32_t seq = 0;
+      int cut = 0;  // value tiles that the mask cuts, so far
       bool ok = true;
-      auto slot = [&](bool value, int tile, int part, int chunks) {
+      auto slot = [&](bool value, int tile, int part) {
         const uint32_t s = seq % kSlots;
-        if (seq >= kSlots) ok = mbar_wait(bar(&bars->empty[s]), (seq / kSlots - 1) & 1u, abort_flag);
+        if (seq >= kSlots) ok = mbar_wait_fast(bar(&bars->empty[s]), (seq / kSlots - 1) & 1u, abort_flag);
         if (!ok) return;
-        const int n = min(2, chunks - 2 * part);
-        mbar_expect_tx(bar(&bars->full[s]), n * kChunkBytes);
+        const int per = value ? 2 : kKeyChunks, bytes = value ? kChunkBytes : kKeyChunk;
+        const int n = min(per, (value ? vch : nch) - per * part);
+        const bool masked = value && tile >= cut0;
+        uint64_t* local = &bars->cut_full[(tile - cut0) & 1];
+        if (masked) {
+          if (part == 0) {
+            mbar_expect_tx(bar(local), vch * kChunkBytes);
+            ++cut;
+          }
+          if (rank == 0) mbar_arrive(bar(&bars->full[s]));
+        } else if (rank == 0) {
+          mbar_expect_tx(bar(&bars->full[s]), kCtas * n * bytes);
+        }
         for (int c = 0; c < n; ++c) {
-          const uint32_t dst = smem_addr(ring + s * kSlotBytes + c * kChunkBytes);
-          const int x = (2 * part + c) * 64, z = (int)(k0 + (int64_t)tile * kTile);
-          if (value)
-            tma_load_3d(dst, &v_map, x, head, z, bar(&bars->full[s]));
-          else if (x >= a.dn)
-            tma_load_2d(dst, &kr_map, 0, z, bar(&bars->full[s]));
+          const uint32_t dst = smem_addr(ring + s * kSlotBytes + c * bytes);
+          const int x = (per * part + c) * 64, z = (int)(k0 + (int64_t)tile * kTile);
+          if (masked)
+            tma_load_3d(dst, &v_map, rank * vch * 64 + x, head, z, bar(local));
+          else if (value)
+            load(dst, &v_map, rank * vch * 64 + x, z, &bars->full[s]);
+          else if (x < a.dn)
+            load(dst, &kn_map, x, z + rank * kKeyRows, &bars->full[s]);
+          else if constexpr (PAIR)
+            tma_load_2d_at(dst, &kr_map, 0, z + rank * kKeyRows, bar(&bars->full[s]), 0);
           else
-            tma_load_3d(dst, &kn_map, x, head, z, bar(&bars->full[s]));
+            tma_load_2d(dst, &kr_map, 0, z, bar(&bars->full[s]));
         }
         ++seq;
       };
       for (int t = 0; t <= tiles && ok; ++t) {
-        for (int p = 0; p < kslots && ok && t < tiles; ++p) slot(false, t, p, nch);
-        for (int p = 0; p < vslots && ok && t > 0; ++p) slot(true, t - 1, p, vch);
+        for (int p = 0; p < kslots && ok && t < tiles; ++p) slot(false, t, p);
+        for (int p = 0; p < vslots && ok && t > 0; ++p) slot(true, t - 1, p);
       }
       if (!ok) {
-        // copies still in flight write this CTA's shared memory: wait for them
+        // copies still in flight write this CTA's (this pair's) shared memory:
+        // wait for them; a pair leaves together
         volatile int never = 0;
-        for (uint32_t k = seq > kSlots ? seq - kSlots : 0; k < seq; ++k)
+        for (uint32_t k = seq > kSlots ? seq - kSlots : 0; k < seq && rank == 0; ++k)
           mbar_wait(bar(&bars->full[k % kSlots]), (k / kSlots) & 1u, &never);
         never = 0;
-        mbar_wait(bar(&bars->q_full), 0, &never);
+        if (rank == 0) mbar_wait(bar(&bars->q_full), 0, &never);
+        never = 0;
+        for (int k = max(0, cut - 2); k < cut; ++k) mbar_wait(bar(&bars->cut_full[k & 1]), (k >> 1) & 1u, &never);
       }
     }
   } else if (warp == 9) {
     // ---------------- MMA ----------------
     // All lanes walk the loops, so that descriptors stay in uniform registers;
-    // one elected lane waits and issues, eight unrolled MMAs a slot.
-    if (tiles > 0) {
+    // one elected lane waits and issues the unrolled MMAs of a slot.
+    if (tiles > 0 && rank == 0) {
       constexpr bool bf16 = std::is_same<E, __nv_bfloat16>::value;
-      constexpr uint32_t id_s = make_idesc_f16(kTile, kTile, bf16, false, false);
+      constexpr uint32_t id_s = make_idesc_f16(kUnit, kTile, bf16, false, false);
       const bool leader = elect_one();
       uint32_t seq = 0;
       bool ok = true;
       const uint64_t qd = make_sw128_desc(smem_addr(q_smem));
       const uint64_t kd0 = make_sw128_desc(smem_addr(ring)), vd0 = make_sw128_mn_desc(smem_addr(ring), kChunkBytes);
+      auto commit = [&](uint64_t* p) {
+        if constexpr (PAIR)
+          mma_commit2(bar(p));
+        else
+          mma_commit(bar(p));
+      };
+      auto landed = [&](uint32_t s, uint32_t phase) {
+        ok = ok && mbar_wait_fast(bar(&bars->full[s]), phase, abort_flag);
+        tmem_fence_after();
+        return ok;
+      };
       if (leader) ok = mbar_wait_fast(bar(&bars->q_full), 0, abort_flag);
       for (int t = 0; t <= tiles; ++t) {
         if (t < tiles) {
           const uint32_t d = kSCol + (t & 1) * kTile;
           for (int p = 0; p < kslots; ++p, ++seq) {
             const uint32_t s = seq % kSlots, phase = (seq / kSlots) & 1u;
-            const uint64_t ad = qd + (uint64_t)(p * (kSlotBytes >> 4));
+            const uint64_t ad = qd + (uint64_t)(p * (kKeyChunks * kChunkBytes >> 4));
             const uint64_t kd = kd0 + (uint64_t)(s * (kSlotBytes >> 4));
-            if (leader) {
-              ok = ok && mbar_wait_fast(bar(&bars->full[s]), phase, abort_flag);
-              tmem_fence_after();
-              if (ok) {
+            const int n = min(kKeyChunks, nch - kKeyChunks * p);
+            if (leader && landed(s, phase)) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_f16_ss(d, ad + 2 * k, kd + 2 * k, id_s, (p | k) != 0);
-                if (2 * p + 1 < nch) {
+              for (int c = 0; c < kKeyChunks; ++c) {
+                if (c < n) {
 #pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    mma_f16_ss(d, ad + (kChunkBytes >> 4) + 2 * k, kd + (kChunkBytes >> 4) + 2 * k, id_s, 1);
+                  for (int k = 0; k < 4; ++k) {
+                    const uint64_t x = ad + (c * kChunkBytes >> 4) + 2 * k, y = kd + (c * kKeyChunk >> 4) + 2 * k;
+                    if constexpr (PAIR)
+                      mma_f16_ss2(d, x, y, id_s, (p | c | k) != 0);
+                    else
+                      mma_f16_ss(d, x, y, id_s, (p | c | k) != 0);
+                  }
                 }
-                mma_commit(bar(&bars->empty[s]));
               }
+              commit(&bars->empty[s]);
             }
           }
-          if (leader && ok) mma_commit(bar(&bars->s_full[t & 1]));
+          if (leader && ok) commit(&bars->s_full[t & 1]);
         }
         if (t > 0) {
           const int u = t - 1;
           const uint32_t pa = kSCol + (u & 1) * kTile;
           const int steps = (min(kTile, nk - u * kTile) + 15) >> 4;
-          if (leader) ok = ok && mbar_wait_fast(bar(&bars->p_full[u & 1]), (u >> 1) & 1u, abort_flag);
+          if (leader) {
+            if constexpr (PAIR)
+              ok = ok && mbar_wait_peer(bar(&bars->p_full[u & 1]), (u >> 1) & 1u, abort_flag);
+            else
+              ok = ok && mbar_wait_fast(bar(&bars->p_full[u & 1]), (u >> 1) & 1u, abort_flag);
+          }
           for (int p = 0; p < vslots; ++p, ++seq) {
             const uint32_t s = seq % kSlots, phase = (seq / kSlots) & 1u;
-            const uint32_t id_o = 2 * p + 1 < vch ? make_idesc_f16(kTile, 128, bf16, false, true)
-                                                  : make_idesc_f16(kTile, 64, bf16, false, true);
+            // a pair's slot holds half of N = 256 or 128; a CTA's all of N = 128 or 64
+            const bool two = 2 * p + 1 < vch;
+            const uint32_t id_o = two ? make_idesc_f16(kUnit, kUnit, bf16, false, true)
+                                      : make_idesc_f16(kUnit, kUnit / 2, bf16, false, true);
             const uint64_t vd = vd0 + (uint64_t)(s * (kSlotBytes >> 4));
             const uint32_t o = kOCol + p * 128;
-            if (leader) {
-              ok = ok && mbar_wait_fast(bar(&bars->full[s]), phase, abort_flag);
-              tmem_fence_after();
-              if (ok) {
-                if (steps == 8) {
+            if (leader && landed(s, phase)) {
+              auto step = [&](int k) {
+                if constexpr (PAIR)
+                  mma_f16_ts2(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
+                else
+                  mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
+              };
+              if (steps == 8) {
 #pragma unroll
-                  for (int k = 0; k < 8; ++k) mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
-                } else {
-                  for (int k = 0; k < steps; ++k) mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
-                }
-                mma_commit(bar(&bars->empty[s]));
+                for (int k = 0; k < 8; ++k) step(k);
+              } else {
+                for (int k = 0; k < steps; ++k) step(k);
               }
+              commit(&bars->empty[s]);
             }
           }
-          if (leader && ok) mma_commit(bar(&bars->o_done[u & 1]));
+          if (leader && ok) commit(&bars->o_done[u & 1]);
         }
       }
       // no MMA is in flight when TMEM is freed.  The lane that issued waits
       // alone: a lane that spins must not keep its warp from one with work.
       if (leader) {
         volatile int never = 0;
-        mma_commit(bar(&bars->drain));
+        commit(&bars->drain);
         if (!mbar_wait(bar(&bars->drain), 0, &never)) *abort_flag = 1;
       }
     }
@@ -395,27 +463,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int t = 0; t < tiles; ++t) {
       ok = ok && __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->s_full[t & 1]), (t >> 1) & 1u, abort_flag));
-      if ((t + 1) * kTile > vis0 && ok) {
-        // value slots of tile t in the order the producer fills the ring; once
-        // tile t - 1 is multiplied, each slot's previous use is over and its
-        // barrier's parity means this one
-        if (t > 0)
-          ok = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(t - 1) & 1]), ((t - 1) >> 1) & 1u, abort_flag));
+      if (t >= cut0 && ok) {
+        // its values lie in the ring where the producer put them
         const uint32_t s0 = kslots + t * (kslots + vslots) + (t + 1 < tiles ? kslots : 0);
+        ok = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->cut_full[(t - cut0) & 1]), ((t - cut0) >> 1) & 1u,
+                                                    abort_flag));
         const int valid = min(kTile, nk - t * kTile), end = (valid + 15) & ~15;  // the product stops at `end`
         bool found = false;
         for (int c = 0; c < vch && ok; ++c) {
-          const uint32_t q = s0 + (c >> 1), s = q % kSlots;
-          if (!(c & 1))
-            ok = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->full[s]), (q / kSlots) & 1u, abort_flag));
+          const uint32_t s = (s0 + (c >> 1)) % kSlots;
           for (int row = tid - 320; row < end && ok; row += 64)
             found |= clean_row<E>(ring + s * kSlotBytes + (c & 1) * kChunkBytes, row, valid);
         }
-        if (found) bars->poison = 1;
+        if (found) {
+          bars->poison = 1;
+          // the other CTA's rows meet these values too
+          if constexpr (PAIR) store_at(smem_addr(&bars->poison), rank ^ 1, 1);
+        }
         fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR)
+            mbar_arrive_at(bar(&bars->p_full[t & 1]), 0);
+          else
+            p_arrive(t);
+        }
+      } else if (lane == 0) {
+        p_arrive(t);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(&bars->p_full[t & 1]));
       __syncwarp();
     }
   } else {
@@ -425,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3, half = warp >> 2;
     const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const int vis = r < rows ? (a.causal ? (int)max((int64_t)0, min(bd.nk, bd.nk - bd.nq + j0 + r + 1)) : nk) : 0;
+    const int vis = r < rows ? seen(j0 + r) : 0;
     const int ocols = a.dv >> 1, o0 = half * ocols;  // this thread's result columns
     float m = -INFINITY, l = 0.f;
     bool stop = false;
@@ -445,7 +520,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32(src + 32 * h, w);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[32 * h + i] = __uint_as_float(w[i]) * a.c;
+          for (int i = 0; i < 32; ++i) v[32 * h + i] = __uint_as_float(w[i]);
+        }
+        if (a.negative) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] = -v[i];
         }
       }
       const int key0 = t * kTile + half * 64;
@@ -457,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float top = v[0];
 #pragma unroll
       for (int i = 1; i < 64; ++i) top = fmaxf(top, v[i]);
+      top *= a.c;
       // also orders every read of S before the stores of P into its columns
       const bool grow = any_of(stop || top > m + kMaxSlack, 1, kSoftThreads);
       if (grow) {
@@ -489,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t w[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        const float p0 = ex2(v[2 * i] - sub), p1 = ex2(v[2 * i + 1] - sub);
+        const float p0 = ex2(fmaf(v[2 * i], a.c, -sub)), p1 = ex2(fmaf(v[2 * i + 1], a.c, -sub));
         l += p0 + p1;
         w[i] = Elem<E>::pack(p0, p1);
       }
@@ -497,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_st();
       tmem_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(&bars->p_full[b]));
+      if (lane == 0) p_arrive(t);
       __syncwarp();
     }
     if (!stop && tiles > 0)
@@ -526,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = vis > 0 ? __uint_as_float(w[i]) * inv : 0.f;
         if (poison) {
-          for (int k = vis0 / kTile * kTile; k < vis; ++k) {
+          for (int k = cut0 * kTile; k < vis; ++k) {
             const uint16_t* src = a.v + (k0 + k) * a.v_t + head * a.v_h + o0 + o;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -552,20 +632,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_fence_before();
   }
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other may reach its memory
   if (tid == 0 && bars->abort_flag) report(a.status, a.status_host, kStatusWaitTimeout);
   if (warp == 9) {
     tmem_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars->tmem_base), "r"(512) : "memory");
+    tmem_free_all<PAIR>(bars->tmem_base);
   }
+  if constexpr (PAIR) cluster_sync();
 }
 
 bool stride_ok(int64_t s, int64_t count) {
   return s % 8 == 0 && s < (int64_t)1 << 38 && (count > 1 ? s > 0 : s >= 0);
 }
 
-// [tokens][heads][dim] view (strides in elements), box 64 values x 1 head x 128 tokens.
+// [tokens][heads][dim] view (strides in elements), box 64 values x 1 head x box_rows tokens.
 int make_rows_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, int64_t heads, int64_t stride_h,
-                  int64_t tokens, int64_t stride_t) {
+                  int64_t tokens, int64_t stride_t, int box_rows) {
   auto fn = encode_fn();
   if (!fn) {
     set_last_error("glm53_latent_expanded: cuTensorMapEncodeTiled is unavailable");
@@ -573,7 +655,7 @@ int make_rows_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, in
   }
   cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
   cuuint64_t strides[2] = {(cuuint64_t)(stride_h ? stride_h : 8) * 2, (cuuint64_t)(stride_t ? stride_t : 8) * 2};
-  cuuint32_t box[3] = {64, 1, kTile};
+  cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows};
   cuuint32_t step[3] = {1, 1, 1};
   const CUresult r =
       fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
@@ -586,7 +668,7 @@ int make_rows_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, in
   return GLM53_OK;
 }
 
-int make_shared_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, int64_t tokens, int64_t stride_t) {
+int make_shared_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, int64_t tokens, int64_t stride_t, int box_rows) {
   auto fn = encode_fn();
   if (!fn) {
     set_last_error("glm53_latent_expanded: cuTensorMapEncodeTiled is unavailable");
@@ -594,7 +676,7 @@ int make_shared_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, 
   }
   cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)tokens};
   cuuint64_t strides[1] = {(cuuint64_t)(stride_t ? stride_t : 8) * 2};
-  cuuint32_t box[2] = {64, kTile};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
   cuuint32_t step[2] = {1, 1};
   const CUresult r =
       fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base),
@@ -605,6 +687,31 @@ int make_shared_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, 
     return GLM53_ERR_CUDA;
   }
   return GLM53_OK;
+}
+
+template <typename E, bool PAIR>
+int launch(const CUtensorMap& qn, const CUtensorMap& qr, const CUtensorMap& kn, const CUtensorMap& kr,
+           const CUtensorMap& v, const Args& a, cudaStream_t st) {
+  const auto kernel = expanded_kernel<E, PAIR>;
+  const int rc = ensure_max_smem((const void*)kernel, kSmemBytes);
+  if (rc) return rc;
+  // a unit more a request than whole units in all: where rows lie outside every
+  // request, at least one unit a head has no queries and zeroes them
+  constexpr int kCtas = PAIR ? 2 : 1, kUnit = kCtas * kTile;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(((a.Tq + kUnit - 1) / kUnit + a.B) * kCtas), (unsigned)a.H);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, qn, qr, kn, kr, v, a);
+  return check_launch("expanded_kernel");
 }
 
 }  // namespace
@@ -657,24 +764,29 @@ extern "C" int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, in
     return GLM53_ERR_INVALID;
   }
   const bool bf16 = dtype == GLM53_DTYPE_BF16;
+  // Two CTAs take 256 queries as a pair where the requests bring more than 128
+  // on average and the values split into whole chunks: each then reads and
+  // holds half of K and V.  Measured with 64 heads of 256 + 256 values: @PAIR@
+  const bool pair = value_dim % 128 == 0 && Tq > requests * kTile;
+  const int key_rows = pair ? kTile / 2 : kTile;
   CUtensorMap qn, qr, kn, kr, v;
-  int rc = make_rows_map(&qn, q_nope, bf16, nope_dim, heads, qn_stride_h, Tq, qn_stride_t);
+  int rc = make_rows_map(&qn, q_nope, bf16, nope_dim, heads, qn_stride_h, Tq, qn_stride_t, kTile);
   if (rc) return rc;
   qr = kn = kr = v = qn;  // maps that no load reads (no rotary part, no keys)
-  if (rope_dim && (rc = make_rows_map(&qr, q_rope, bf16, rope_dim, heads, qr_stride_h, Tq, qr_stride_t))) return rc;
+  if (rope_dim && (rc = make_rows_map(&qr, q_rope, bf16, rope_dim, heads, qr_stride_h, Tq, qr_stride_t, kTile)))
+    return rc;
   if (Tk) {
-    if ((rc = make_rows_map(&kn, k_nope, bf16, nope_dim, heads, kn_stride_h, Tk, kn_stride_t))) return rc;
-    if ((rc = make_rows_map(&v, values, bf16, value_dim, heads, v_stride_h, Tk, v_stride_t))) return rc;
-    if (rope_dim && (rc = make_shared_map(&kr, k_rope, bf16, rope_dim, Tk, kr_stride_t))) return rc;
+    if ((rc = make_rows_map(&kn, k_nope, bf16, nope_dim, heads, kn_stride_h, Tk, kn_stride_t, key_rows))) return rc;
+    if ((rc = make_rows_map(&v, values, bf16, value_dim, heads, v_stride_h, Tk, v_stride_t, kTile))) return rc;
+    if (rope_dim && (rc = make_shared_map(&kr, k_rope, bf16, rope_dim, Tk, kr_stride_t, key_rows))) return rc;
   }
+  // a masked score is -inf, which a factor of 0 would turn into NaN
+  const float c = std::max(std::fabs(scale) * kLog2e, 1e-37f);
   Args a{Tq, Tk, (int)heads, (int)nope_dim, (int)rope_dim, (int)value_dim, query_starts, key_starts, (int)requests,
-         scale * kLog2e, causal, (const uint16_t*)values, v_stride_t, v_stride_h, (uint16_t*)out, lse, fill_tail,
+         c, scale < 0, causal, (const uint16_t*)values, v_stride_t, v_stride_h, (uint16_t*)out, lse, fill_tail,
          status, status_host};
-  // a tile more a request than whole tiles in all: where rows lie outside every
-  // request, at least one CTA a head has no tile and zeroes them
-  const dim3 grid((unsigned)((Tq + kTile - 1) / kTile + requests), (unsigned)heads);
-  const auto kernel = bf16 ? expanded_kernel<__nv_bfloat16> : expanded_kernel<__half>;
-  if ((rc = ensure_max_smem((const void*)kernel, kSmemBytes))) return rc;
-  kernel<<<grid, kThreads, kSmemBytes, (cudaStream_t)stream>>>(qn, qr, kn, kr, v, a);
-  return check_launch(fn);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (pair)
+    return bf16 ? launch<__nv_bfloat16, true>(qn, qr, kn, kr, v, a, st) : launch<__half, true>(qn, qr, kn, kr, v, a, st);
+  return bf16 ? launch<__nv_bfloat16, false>(qn, qr, kn, kr, v, a, st) : launch<__half, false>(qn, qr, kn, kr, v, a, st);
 }

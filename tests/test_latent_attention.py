@@ -563,6 +563,10 @@ EXPANDED = [
     ([513], [1100], 1, 256, 0, 256, True),
     ([3] * 40, list(range(3, 43)), 1, 128, 64, 64, True),
     ([700], [700], 1, 192, 64, 256, False),
+    ([700, 300, 1000], [701, 1300, 1000], 2, 192, 64, 256, True),
+    ([400, 257], [400, 258], 3, 128, 64, 128, True),
+    ([600, 300], [20, 310], 1, 64, 64, 128, True),
+    ([385], [2000], 1, 128, 0, 256, False),
 ]
 
 
@@ -585,13 +589,42 @@ def test_expanded_matches(dtype, case):
 def test_expanded_scores_that_grow():
     import glm53_flash_mlx_b200 as G
 
-    nq, nk = [260], [900]
-    qn, qr, kn, kr, v, qs, ks = make_expanded(nq, nk, 2, 192, 64, 256, torch.bfloat16, 4)
-    qn = torch.full_like(qn, 0.25)
-    kn = kn.clone()
-    kn[..., :64] = (torch.arange(900, device="cuda") / 900 * 8).to(torch.bfloat16)[:, None, None]
-    out, lse = G.latent_attention_expanded(qn, qr, kn, kr, v, qs, ks, scale=0.5, return_lse=True)
-    check(out, lse, *expanded64(qn, qr, kn, kr, v, nq, nk, 0.5, True, torch.bfloat16))
+    for nq, sign in (([260], 1), ([100], 1), ([260], -1)):
+        nk = [900]
+        qn, qr, kn, kr, v, qs, ks = make_expanded(nq, nk, 2, 192, 64, 256, torch.bfloat16, 4)
+        qn = torch.full_like(qn, 0.25)
+        kn = kn.clone()
+        kn[..., :64] = (torch.arange(900, device="cuda") / 900 * 8).to(torch.bfloat16)[:, None, None] * sign
+        out, lse = G.latent_attention_expanded(qn, qr, kn, kr, v, qs, ks, scale=0.5 * sign, return_lse=True)
+        check(out, lse, *expanded64(qn, qr, kn, kr, v, nq, nk, 0.5 * sign, True, torch.bfloat16))
+    t = make_expanded([150], [300], 2, 128, 64, 128, torch.float16, 5)
+    out, lse = G.latent_attention_expanded(*t, scale=0.0, return_lse=True)  # the mean of what each row sees
+    check(out, lse, *expanded64(*t[:5], [150], [300], 0.0, True, torch.float16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_expanded_masked_keys_and_values_do_not_enter_large(what):
+    """The same with more than 128 queries a request, at every place of a 256-row unit."""
+    import glm53_flash_mlx_b200 as G
+
+    nq, nk = [600, 300], [600, 333]
+    qn, qr, kn, kr, v, qs, ks = make_expanded(nq, nk, 2, 192, 64, 256, torch.bfloat16, 6)
+    clean = G.latent_attention_expanded(qn, qr, kn, kr, v, qs, ks, scale=0.06)
+    bad, hit = v.clone(), torch.zeros_like(clean, dtype=torch.bool)
+    for key, head, col in [(0, 0, 3), (130, 0, 70), (255, 1, 130), (256, 1, 0), (300, 0, 255), (511, 1, 64), (599, 0, 200)]:
+        bad[key, head, col] = what
+        hit[key:600, head, col] = True
+    bad[600 + 332, 1, 255] = what
+    hit[899, 1, 255] = True
+    got = G.latent_attention_expanded(qn, qr, kn, kr, bad, qs, ks, scale=0.06)
+    G.check_latent_status()
+    assert torch.equal(got[~hit], clean[~hit])
+    assert got[hit].isnan().all() if math.isnan(what) else (got[hit] == math.inf).all()
+    kbad = kn.clone()
+    kbad[600:] = math.nan  # the second request's keys
+    got = G.latent_attention_expanded(qn, qr, kbad, kr, v, qs, ks, scale=0.06)
+    assert torch.equal(got[:600], clean[:600]) and got[600:].isnan().all()
 
 
 @pytest.mark.gpu
