@@ -72,7 +72,7 @@ struct Args {
 };
 
 struct __align__(8) Bars {
-  uint64_t q_full, full[kSlots], empty[kSlots], cut_full[2], s_full[2], p_full[2], o_done[2], drain;
+  uint64_t q_full, full[kSlots], empty[kSlots], cut_full[4], s_full[2], p_full[2], o_done[2], drain;
   uint32_t tmem_base;
   int abort_flag;
   int poison;                       // a masked tile holds values that are not finite
@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar(&bars->cut_full[s]), 1);
+      mbar_init(bar(&bars->cut_full[s + 2]), 1);
       mbar_init(bar(&bars->s_full[s]), 1);
       mbar_init(bar(&bars->p_full[s]), kCtas * (kSoftWarps + kCleanWarps));
       mbar_init(bar(&bars->o_done[s]), 1);
@@ -296,7 +297,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- TMA ----------------
     // full[s] counts the bytes of both CTAs of a pair, at rank 0.  The values of
     // a tile that the mask cuts are counted at cut_full of the CTA that holds
-    // (and cleans) them; the product learns of them through p_full.
+    // (and cleans) them; the product learns of them through p_full.  A pair's ring
+    // can hold three such tiles before the first has landed (one slot a tile, no
+    // K behind the last), and a barrier takes one tile at a time: four barriers.
     if (lane == 0 && tiles > 0) {
       auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int z, uint64_t* p) {
         if constexpr (PAIR)
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int per = value ? 2 : kKeyChunks, bytes = value ? kChunkBytes : kKeyChunk;
         const int n = min(per, (value ? vch : nch) - per * part);
         const bool masked = value && tile >= cut0;
-        uint64_t* local = &bars->cut_full[(tile - cut0) & 1];
+        uint64_t* local = &bars->cut_full[(tile - cut0) & 3];
         if (masked) {
           if (part == 0) {
             mbar_expect_tx(bar(local), vch * kChunkBytes);
@@ -358,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         never = 0;
         if (rank == 0) mbar_wait(bar(&bars->q_full), 0, &never);
         never = 0;
-        for (int k = max(0, cut - 2); k < cut; ++k) mbar_wait(bar(&bars->cut_full[k & 1]), (k >> 1) & 1u, &never);
+        for (int k = max(0, cut - 4); k < cut; ++k) mbar_wait(bar(&bars->cut_full[k & 3]), (k >> 2) & 1u, &never);
       }
     }
   } else if (warp == 9) {
@@ -466,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (t >= cut0 && ok) {
         // its values lie in the ring where the producer put them
         const uint32_t s0 = kslots + t * (kslots + vslots) + (t + 1 < tiles ? kslots : 0);
-        ok = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->cut_full[(t - cut0) & 1]), ((t - cut0) >> 1) & 1u,
+        ok = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->cut_full[(t - cut0) & 3]), ((t - cut0) >> 2) & 1u,
                                                     abort_flag));
         const int valid = min(kTile, nk - t * kTile), end = (valid + 15) & ~15;  // the product stops at `end`
         bool found = false;

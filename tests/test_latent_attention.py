@@ -567,6 +567,8 @@ EXPANDED = [
     ([400, 257], [400, 258], 3, 128, 64, 128, True),
     ([600, 300], [20, 310], 1, 64, 64, 128, True),
     ([385], [2000], 1, 128, 0, 256, False),
+    ([200] * 8, [2200] * 8, 4, 192, 64, 256, True),  # three tiles that the mask cuts, loaded one behind the other
+    ([250, 129], [2001, 3333], 2, 128, 64, 128, True),
 ]
 
 
