@@ -251,62 +251,93 @@ __device__ __forceinline__ void write_row(const WriteArgs& a, int64_t t, int lan
   }
 }
 
-// Without queries: a warp a token.  With queries: a block a token, the angles
-// computed once for all heads; the last warp stores the row.
-template <typename E, bool QUERIES>
+// Without queries: a warp a token.  With queries: a block a token, whose last
+// warp forms the angles for all heads and stores the row while the others'
+// loads are on their way (4,096 tokens of 64 heads: @OLD@ us when the loads
+// waited for the angles, @NEW@ us so).
+constexpr int kQueryThreads = 256;
+
+template <typename E>
 __global__ void __launch_bounds__(kWriteThreads) latent_write_kernel(WriteArgs a) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if constexpr (!QUERIES) {
-    const int64_t t = (int64_t)blockIdx.x * (kWriteThreads / 32) + warp;
-    if (t < a.T) write_row<E>(a, t, lane, nullptr);
-  } else {
-    __shared__ float2 turns[kMaxRope / 2];
-    const int64_t t = blockIdx.x;
-    const int half = a.rope >> 1;
-    if (threadIdx.x < half) turns[threadIdx.x] = turn_of(a.positions[t], a.inv_freq[threadIdx.x]);
-    __syncthreads();
-    if (warp == kWriteThreads / 32 - 1) write_row<E>(a, t, lane, turns);
-    const int pieces = a.rope >> 4;  // pairs of 8-value pieces a head
-    for (int i = threadIdx.x; i < a.heads * pieces; i += kWriteThreads) {
-      const int h = i / pieces, v = i - h * pieces;
-      const uint16_t* src = a.q + t * a.q_stride_t + h * a.q_stride_h;
-      uint16_t* dst = a.q_out + (t * a.heads + h) * a.rope;
-      const int e0 = a.interleaved ? 16 * v : 8 * v, e1 = a.interleaved ? e0 + 8 : half + 8 * v;
-      float x[8], y[8];
-      unpack8<E>(*reinterpret_cast<const uint4*>(src + e0), x);
-      unpack8<E>(*reinterpret_cast<const uint4*>(src + e1), y);
-      if (a.interleaved) {
+  const int64_t t = (int64_t)blockIdx.x * (kWriteThreads / 32) + (threadIdx.x >> 5);
+  if (t < a.T) write_row<E>(a, t, threadIdx.x & 31, nullptr);
+}
+
+// The two 8-value pieces that piece pair v of a head turns: values 8 v and
+// rope / 2 + 8 v, or 16 v and 16 v + 8 when neighbours pair up.
+template <typename E>
+__device__ __forceinline__ void turn_pieces(const WriteArgs& a, const float2* turns, int v, uint4& p, uint4& q) {
+  float x[8], y[8];
+  unpack8<E>(p, x);
+  unpack8<E>(q, y);
+  if (a.interleaved) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 c0 = turns[8 * v + j], c1 = turns[8 * v + 4 + j];
-          const float u0 = x[2 * j], w0 = x[2 * j + 1], u1 = y[2 * j], w1 = y[2 * j + 1];
-          x[2 * j] = u0 * c0.x - w0 * c0.y;
-          x[2 * j + 1] = w0 * c0.x + u0 * c0.y;
-          y[2 * j] = u1 * c1.x - w1 * c1.y;
-          y[2 * j + 1] = w1 * c1.x + u1 * c1.y;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float2 cs = turns[8 * v + j];
-          const float u = x[j], w = y[j];
-          x[j] = u * cs.x - w * cs.y;
-          y[j] = w * cs.x + u * cs.y;
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + e0) = pack8<E>(x);
-      *reinterpret_cast<uint4*>(dst + e1) = pack8<E>(y);
+    for (int j = 0; j < 4; ++j) {
+      const float2 c0 = turns[8 * v + j], c1 = turns[8 * v + 4 + j];
+      const float u0 = x[2 * j], w0 = x[2 * j + 1], u1 = y[2 * j], w1 = y[2 * j + 1];
+      x[2 * j] = u0 * c0.x - w0 * c0.y;
+      x[2 * j + 1] = w0 * c0.x + u0 * c0.y;
+      y[2 * j] = u1 * c1.x - w1 * c1.y;
+      y[2 * j + 1] = w1 * c1.x + u1 * c1.y;
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 cs = turns[8 * v + j];
+      const float u = x[j], w = y[j];
+      x[j] = u * cs.x - w * cs.y;
+      y[j] = w * cs.x + u * cs.y;
+    }
+  }
+  p = pack8<E>(x);
+  q = pack8<E>(y);
+}
+
+template <typename E>
+__global__ void __launch_bounds__(kQueryThreads + 32) latent_write_queries_kernel(WriteArgs a) {
+  __shared__ float2 turns[kMaxRope / 2];
+  const int64_t t = blockIdx.x;
+  const int half = a.rope >> 1;
+  if (threadIdx.x >= kQueryThreads) {
+    const int lane = threadIdx.x & 31;
+    const int32_t position = a.positions[t];
+    for (int p = lane; p < half; p += 32) turns[p] = turn_of(position, a.inv_freq[p]);
+    __syncthreads();
+    write_row<E>(a, t, lane, turns);
+    return;
+  }
+  const int pieces = a.rope >> 4, items = a.heads * pieces;  // pairs of pieces: of a head, in all
+  const uint16_t* q = a.q + t * a.q_stride_t;
+  uint16_t* out = a.q_out + t * a.heads * a.rope;
+  auto at = [&](int v, int second) { return a.interleaved ? 16 * v + 8 * second : 8 * v + half * second; };
+  auto load = [&](int i, uint4& x, uint4& y) {
+    const int h = i / pieces, v = i - h * pieces;
+    const uint16_t* src = q + h * a.q_stride_h;
+    x = ldg_stream(reinterpret_cast<const uint4*>(src + at(v, 0)));
+    y = ldg_stream(reinterpret_cast<const uint4*>(src + at(v, 1)));
+  };
+  uint4 x, y;
+  int i = threadIdx.x;
+  if (i < items) load(i, x, y);
+  __syncthreads();
+  while (i < items) {
+    const int h = i / pieces, v = i - h * pieces;
+    turn_pieces<E>(a, turns, v, x, y);
+    uint16_t* dst = out + h * a.rope;
+    *reinterpret_cast<uint4*>(dst + at(v, 0)) = x;
+    *reinterpret_cast<uint4*>(dst + at(v, 1)) = y;
+    i += kQueryThreads;
+    if (i < items) load(i, x, y);
   }
 }
 
 template <typename E>
 void launch_write(const WriteArgs& a, cudaStream_t st) {
   if (a.q) {
-    latent_write_kernel<E, true><<<(unsigned)a.T, kWriteThreads, 0, st>>>(a);
+    latent_write_queries_kernel<E><<<(unsigned)a.T, kQueryThreads + 32, 0, st>>>(a);
   } else {
     const int64_t blocks = (a.T + kWriteThreads / 32 - 1) / (kWriteThreads / 32);
-    latent_write_kernel<E, false><<<(unsigned)blocks, kWriteThreads, 0, st>>>(a);
+    latent_write_kernel<E><<<(unsigned)blocks, kWriteThreads, 0, st>>>(a);
   }
 }
 

@@ -767,10 +767,14 @@ extern "C" int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, in
     return GLM53_ERR_INVALID;
   }
   const bool bf16 = dtype == GLM53_DTYPE_BF16;
-  // Two CTAs take 256 queries as a pair where the requests bring more than 128
-  // on average and the values split into whole chunks: each then reads and
-  // holds half of K and V.  Measured with 64 heads of 256 + 256 values: @PAIR@
-  const bool pair = value_dim % 128 == 0 && Tq > requests * kTile;
+  // Two CTAs take 256 queries as a pair, each reading and holding half of K and
+  // V, where requests are long enough to pay for the pair's hand-shakes and for
+  // units of 256 rows.  Measured, one CTA / a pair: 64 heads of 256 + 256 values,
+  // 1,024 queries and keys 77 / 83 us, 2,048 194 / 188, 512 queries over 4,096
+  // keys 140 / 122, 2,048 over 8,192 856 / 719; 16 heads of 192 + 128 values,
+  // 4 x 512 queries over 512 keys 26 / 33, over 2,512 72.5 / 72.3, 512 over
+  // 4,096 51 / 48.
+  const bool pair = value_dim % 128 == 0 && Tq > requests * kTile && Tk >= requests * 2048;
   const int key_rows = pair ? kTile / 2 : kTile;
   CUtensorMap qn, qr, kn, kr, v;
   int rc = make_rows_map(&qn, q_nope, bf16, nope_dim, heads, qn_stride_h, Tq, qn_stride_t, kTile);

@@ -24,6 +24,7 @@ safe result and the next call of this module raises (``IndexError`` /
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -32,48 +33,67 @@ from . import _native as N
 from .packed import StatusWord, _SYNC_STATUS
 
 _DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_FP16}
-_STATUS: dict[int, StatusWord] = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+# device index -> (status word, its address, the mirror's address, the mirror)
+_STATUS: dict[int, tuple] = {}
 
 
-def _status(dev: torch.device) -> StatusWord:
-    sw = _STATUS.get(dev.index)
-    if sw is None:
+def _status(index: int) -> tuple:
+    entry = _STATUS.get(index)
+    if entry is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("call a latent-attention operator once on this device before capturing it")
-        sw = _STATUS[dev.index] = StatusWord(dev)
-    return sw
+        sw = StatusWord(torch.device("cuda", index))
+        entry = _STATUS[index] = (sw, sw.word.data_ptr(), sw.host.data_ptr(), sw._host_word)
+    return entry
 
 
 def check_latent_status(device: torch.device | int | None = None) -> None:
     """Synchronise and raise for any device-side error of this module's calls so far."""
-    index = torch.cuda.current_device() if device is None else torch.device("cuda", device).index \
-        if isinstance(device, int) else torch.device(device).index
-    sw = _STATUS.get(torch.cuda.current_device() if index is None else index)
-    if sw is not None:
-        sw.check()
-
-
-def _call(name: str, dev: torch.device, *args) -> None:
-    """One C-ABI call on `dev`'s current stream with its status word, whatever the current device is."""
-    sw = _status(dev)
-    sw.raise_pending()
-    status = (sw.word.data_ptr(), sw.host.data_ptr(), N.stream(dev))
-    fn = getattr(N.load_library(), name)
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, *status)
+    if isinstance(device, int):
+        index = device
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, *status)
+        index = None if device is None else torch.device(device).index
+    entry = _STATUS.get(torch.cuda.current_device() if index is None else index)
+    if entry is not None:
+        entry[0].check()
+
+
+def _device(first: torch.Tensor, *rest: torch.Tensor | None) -> int:
+    """The CUDA device index that all tensors share; raises as ``require_cuda`` does otherwise."""
+    index = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        N.require_cuda(first, *rest)
+        raise ValueError("tensors on different devices")
+    return index
+
+
+def _call(name: str, index: int, *args) -> None:
+    """One C-ABI call on the device's current stream with its status word, whatever the current device is."""
+    sw, word, host, mirror = _status(index)
+    if mirror.value:
+        sw.raise_pending()
+    fn = getattr(N.lib() if N._lib is None else N._lib, name)
+    stream = _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, word, host, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, word, host, stream)
     if rc:
         N.check(rc, name)
     if _SYNC_STATUS:
         sw.check()
 
 
-def _int32(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-    return t.contiguous()
+def _int32(t: torch.Tensor, name: str, count: int) -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != count:
+        raise ValueError(f"{name} must be int32 [{count}], got {t.dtype} {list(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _dtype(t: torch.Tensor, name: str) -> int:
@@ -84,28 +104,43 @@ def _dtype(t: torch.Tensor, name: str) -> int:
 
 
 def _same(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
-    if t.dtype != dtype or tuple(t.shape) != shape:
+    if t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
     return t
 
 
-def _pieces(t: torch.Tensor) -> torch.Tensor:
-    """`t` itself where its rows can be read in 16-byte pieces, else a contiguous copy."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0:
-        for s in t.stride()[:-1]:
-            if s <= 0 or s % 8:
+def _pieces(t: torch.Tensor) -> tuple:
+    """(tensor, address, strides but the last): `t` itself where its rows can be read in 16-byte pieces, else a
+    contiguous copy."""
+    *outer, last = t.stride()
+    ptr = t.data_ptr()
+    if last == 1 and not ptr & 15:
+        for s in outer:
+            if s <= 0 or s & 7:
                 break
         else:
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
+            return t, ptr, outer
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), t.stride()[:-1]
+
+
+def _table(t: torch.Tensor, requests: int) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != requests:
+        raise ValueError(f"block_table must be int32 [{requests}, pages], got {t.dtype} {list(t.shape)}")
 
 
 def _output(out: torch.Tensor | None, like: torch.Tensor, shape: tuple) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(shape)
     if not out.is_contiguous():
         raise ValueError("out must be contiguous")
     return _same(out, "out", like.dtype, shape)
+
+
+@functools.lru_cache(maxsize=4096)
+def _absorbed_bytes(T: int, H: int, R: int, index: int) -> int:
+    with torch.cuda.device(index):
+        return N.lib().glm53_latent_absorbed_workspace_bytes(T, H, R)
 
 
 class PagePlan(NamedTuple):
@@ -133,27 +168,30 @@ def plan_pages(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     next call; to release pages, write their ids behind it and add their number.
     """
     B = cached_lens.numel()
-    cached_lens = _int32(cached_lens, "cached_lens", (B,))
-    new_lens = _int32(new_lens, "new_lens", (B,))
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
-        raise ValueError(f"block_table must be int32 [{B}, pages], got {block_table.dtype} {list(block_table.shape)}")
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
-        raise ValueError("block_table is updated in place: its rows must be contiguous")
+    cached_lens = _int32(cached_lens, "cached_lens", B)
+    new_lens = _int32(new_lens, "new_lens", B)
+    _table(block_table, B)
     width = block_table.shape[1]
-    if B > 1 and block_table.stride(0) < width:
+    stride, step = block_table.stride()
+    if width > 1 and step != 1:
+        raise ValueError("block_table is updated in place: its rows must be contiguous")
+    if B <= 1:
+        stride = width
+    elif stride < width:
         raise ValueError("block_table is updated in place: its rows must not overlap")
-    free_pages = _int32(free_pages, "free_pages", (free_pages.numel(),))
-    free_count = _int32(free_count, "free_count", (1,))
+    pages = free_pages.numel()
+    free_pages = _int32(free_pages, "free_pages", pages)
+    free_count = _int32(free_count, "free_count", 1)
     if page_size < 1 or tokens < 0:
         raise ValueError(f"page_size {page_size} and tokens {tokens} must be positive")
-    dev = N.require_cuda(cached_lens, new_lens, block_table, free_pages, free_count)
-    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-    words = torch.empty(tokens + 2 * B + 2, dtype=torch.int32, device=dev)
-    positions, starts, lens, left = words.split([tokens, B + 1, B, 1])
-    _call("glm53_plan_pages", dev, cached_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(),
-          block_table.stride(0) if B > 1 else width, width, free_pages.data_ptr(), free_pages.numel(),
-          free_count.data_ptr(), page_size, tokens, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
-          lens.data_ptr(), left.data_ptr())
+    index = _device(cached_lens, new_lens, block_table, free_pages, free_count)
+    slots = cached_lens.new_empty(tokens, dtype=torch.int64)
+    words = cached_lens.new_empty(tokens + 2 * B + 2)
+    positions, starts, lens, left = words.split_with_sizes([tokens, B + 1, B, 1])
+    at = words.data_ptr()
+    _call("glm53_plan_pages", index, cached_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), stride,
+          width, free_pages.data_ptr(), pages, free_count.data_ptr(), page_size, tokens, slots.data_ptr(), at,
+          at + 4 * tokens, at + 4 * (tokens + B + 1), at + 4 * (tokens + 2 * B + 1))
     return PagePlan(slots, positions, starts, lens, left)
 
 
@@ -183,35 +221,37 @@ def latent_cache_write(kv: torch.Tensor, cache: torch.Tensor, slots: torch.Tenso
     if cache.dim() != 3 or cache.dtype != kv.dtype or cache.shape[2] != width or not cache.is_contiguous():
         raise ValueError(f"cache must be contiguous {kv.dtype} [pages, page_size, {width}], got {cache.dtype} "
                          f"{list(cache.shape)}")
-    if slots.dtype != torch.int64 or tuple(slots.shape) != (T,):
+    if slots.dtype is not torch.int64 or slots.shape != (T,):
         raise ValueError(f"slots must be int64 [{T}], got {slots.dtype} {list(slots.shape)}")
     if (positions is None) != (inv_freq is None):
         raise ValueError("positions and inv_freq come together")
+    wp = pp = fp = None
     if norm_weight is not None:
-        norm_weight = _pieces(_same(norm_weight, "norm_weight", kv.dtype, (latent,)))
+        norm_weight, wp, _ = _pieces(_same(norm_weight, "norm_weight", kv.dtype, (latent,)))
     if positions is not None:
-        positions = _int32(positions, "positions", (T,))
+        positions = _int32(positions, "positions", T)
         inv_freq = _same(inv_freq, "inv_freq", torch.float64, (rope_dim // 2,)).contiguous()
-    rotated = None
+        pp, fp = positions.data_ptr(), inv_freq.data_ptr()
+    rotated = qp = rp = None
     heads = qt = qh = 0
     if queries is not None:
         if positions is None:
             raise ValueError("queries are rotated by positions and inv_freq, which are missing")
-        if queries.dim() != 3 or queries.dtype != kv.dtype or queries.shape[0] != T or queries.shape[2] != rope_dim \
-                or queries.shape[1] < 1:
+        if queries.dim() != 3 or queries.dtype is not kv.dtype or queries.shape[0] != T \
+                or queries.shape[2] != rope_dim or queries.shape[1] < 1:
             raise ValueError(f"queries must be {kv.dtype} [{T}, heads, {rope_dim}], got {queries.dtype} "
                              f"{list(queries.shape)}")
-    dev = N.require_cuda(kv, cache, slots, norm_weight, positions, inv_freq, queries)
+    index = _device(kv, cache, slots, norm_weight, positions, inv_freq, queries)
     if queries is not None:
-        queries = _pieces(queries)
         heads = queries.shape[1]
-        qt, qh = queries.stride(0), queries.stride(1)
-        rotated = torch.empty((T, heads, rope_dim), dtype=kv.dtype, device=dev)
-    kv = _pieces(kv)
-    slots = slots.contiguous()
-    _call("glm53_latent_cache_write", dev, kv.data_ptr(), T, max(kv.stride(0), width), latent, rope_dim, code,
-          N.ptr(norm_weight), eps, N.ptr(positions), N.ptr(inv_freq), interleaved, slots.data_ptr(), cache.data_ptr(),
-          cache.shape[0] * cache.shape[1], N.ptr(queries), heads, qt, qh, N.ptr(rotated))
+        rotated = kv.new_empty((T, heads, rope_dim))
+        rp = rotated.data_ptr()
+        queries, qp, (qt, qh) = _pieces(queries)
+    kv, kp, (kt,) = _pieces(kv)
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
+    _call("glm53_latent_cache_write", index, kp, T, kt if kt > width else width, latent, rope_dim, code, wp, eps, pp, fp,
+          interleaved, slots.data_ptr(), cache.data_ptr(), cache.shape[0] * cache.shape[1], qp, heads, qt, qh, rp)
     return rotated
 
 
@@ -251,32 +291,36 @@ def latent_attention_absorbed(q_latent: torch.Tensor, q_rope: torch.Tensor | Non
     if page_size < 8 or page_size % 8:
         raise ValueError(f"page_size {page_size} must be a positive multiple of 8")
     B = seq_lens.numel()
-    seq_lens = _int32(seq_lens, "seq_lens", (B,))
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
-        raise ValueError(f"block_table must be int32 [{B}, pages], got {block_table.dtype} {list(block_table.shape)}")
+    seq_lens = _int32(seq_lens, "seq_lens", B)
+    _table(block_table, B)
+    sp = None
     if query_starts is not None:
-        query_starts = _int32(query_starts, "query_starts", (B + 1,))
+        query_starts = _int32(query_starts, "query_starts", B + 1)
+        sp = query_starts.data_ptr()
     elif T != B:
         raise ValueError(f"without query_starts there is one token a request: {T} tokens, {B} requests")
-    dev = N.require_cuda(q_latent, q_rope, cache, block_table, seq_lens, query_starts, out)
+    index = _device(q_latent, q_rope, cache, block_table, seq_lens, query_starts, out)
     width = block_table.shape[1]
-    if (width > 1 and block_table.stride(1) != 1) or (B > 1 and block_table.stride(0) < width):
+    stride, step = block_table.stride()
+    if (width > 1 and step != 1) or (B > 1 and stride < width):
         block_table = block_table.clone(memory_format=torch.contiguous_format)
+        stride = width
+    if B <= 1:
+        stride = width
     result = _output(out, q_latent, (T, H, R))
-    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+    lse = q_latent.new_empty((T, H), dtype=torch.float32) if return_lse else None
     if T:
-        q_latent = _pieces(q_latent)
-        qrt = qrh = 0
+        q_latent, lp, (lt, lh) = _pieces(q_latent)
+        rp = None
+        rt = rh = 0
         if rope:
-            q_rope = _pieces(q_rope)
-            qrt, qrh = q_rope.stride(0), q_rope.stride(1)
-        nbytes = N.load_library().glm53_latent_absorbed_workspace_bytes(T, H, R)
+            q_rope, rp, (rt, rh) = _pieces(q_rope)
+        nbytes = _absorbed_bytes(T, H, R, index)
         # from the caching allocator: ordered on this stream, private to a captured graph
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _call("glm53_latent_absorbed", dev, q_latent.data_ptr(), q_latent.stride(0), q_latent.stride(1), N.ptr(q_rope),
-              qrt, qrh, T, H, R, rope, code, cache.data_ptr(), pages, page_size, block_table.data_ptr(),
-              block_table.stride(0) if B > 1 else width, width, seq_lens.data_ptr(), B, N.ptr(query_starts), scale,
-              result.data_ptr(), N.ptr(lse), out is None, ws.data_ptr(), nbytes)
+        ws = q_latent.new_empty((nbytes + 1) // 2)
+        _call("glm53_latent_absorbed", index, lp, lt, lh, rp, rt, rh, T, H, R, rope, code, cache.data_ptr(), pages,
+              page_size, block_table.data_ptr(), stride, width, seq_lens.data_ptr(), B, sp, scale, result.data_ptr(),
+              None if lse is None else lse.data_ptr(), out is None, ws.data_ptr(), nbytes)
     return (result, lse) if return_lse else result
 
 
@@ -320,19 +364,21 @@ def latent_attention_expanded(q_nope: torch.Tensor, q_rope: torch.Tensor | None,
     B = query_starts.numel() - 1
     if B < 0:
         raise ValueError("query_starts must hold requests + 1 entries")
-    query_starts = _int32(query_starts, "query_starts", (B + 1,))
-    key_starts = _int32(key_starts, "key_starts", (B + 1,))
-    dev = N.require_cuda(q_nope, q_rope, k_nope, k_rope, values, query_starts, key_starts, out)
+    query_starts = _int32(query_starts, "query_starts", B + 1)
+    key_starts = _int32(key_starts, "key_starts", B + 1)
+    index = _device(q_nope, q_rope, k_nope, k_rope, values, query_starts, key_starts, out)
     result = _output(out, q_nope, (Tq, H, dv))
-    lse = torch.empty((Tq, H), dtype=torch.float32, device=dev) if return_lse else None
+    lse = q_nope.new_empty((Tq, H), dtype=torch.float32) if return_lse else None
     if Tq:
-        q_nope, k_nope, values = _pieces(q_nope), _pieces(k_nope), _pieces(values)
+        q_nope, qp, (qt, qh) = _pieces(q_nope)
+        k_nope, kp, (kt, kh) = _pieces(k_nope)
+        values, vp, (vt, vh) = _pieces(values)
+        qrp = krp = None
         qrt = qrh = krt = 0
         if dr:
-            q_rope, k_rope = _pieces(q_rope), _pieces(k_rope)
-            qrt, qrh, krt = q_rope.stride(0), q_rope.stride(1), k_rope.stride(0)
-        _call("glm53_latent_expanded", dev, q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1), N.ptr(q_rope), qrt,
-              qrh, k_nope.data_ptr(), k_nope.stride(0), k_nope.stride(1), N.ptr(k_rope), krt, values.data_ptr(),
-              values.stride(0), values.stride(1), Tq, Tk, H, dn, dr, dv, code, query_starts.data_ptr(),
-              key_starts.data_ptr(), B, scale, causal, result.data_ptr(), N.ptr(lse), out is None)
+            q_rope, qrp, (qrt, qrh) = _pieces(q_rope)
+            k_rope, krp, (krt,) = _pieces(k_rope)
+        _call("glm53_latent_expanded", index, qp, qt, qh, qrp, qrt, qrh, kp, kt, kh, krp, krt, vp, vt, vh, Tq, Tk, H, dn,
+              dr, dv, code, query_starts.data_ptr(), key_starts.data_ptr(), B, scale, causal, result.data_ptr(),
+              None if lse is None else lse.data_ptr(), out is None)
     return (result, lse) if return_lse else result
