@@ -653,87 +653,159 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the partial results of units that several CTAs shared:
 //   o = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p,  M the largest m_p,
 // and fills what no CTA wrote (tokens that see nothing; with fill_tail those
-// outside every request).  Few results (WAYS = 16): a block takes a fourth of a
-// (token, head), and each of 16 warps every 16th part of it.  Many (WAYS = 1): a
-// block takes a whole one.
-template <typename E, int WAYS>
-__global__ void __launch_bounds__(WAYS == 1 ? 128 : 32 * WAYS) join_kernel(Args a, int heads) {
-  constexpr int kCols = WAYS == 1 ? 128 : 32;  // float4 columns a block
-  __shared__ float weight[2 * kMaxGrid];
-  __shared__ float4 part[WAYS][kCols];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int t = blockIdx.x, h = blockIdx.y;
+// outside every request).  Bound by latency: the plan is one round to L2, all
+// maxima, sums and the first rows a second.
+
+// Where the parts of unit (t, h) are; false when there is nothing to join.
+struct Parts {
+  int c0, count, row;  // first CTA, parts, row of a slot
+  bool late;           // the first part is not its CTA's first segment
+  __device__ __forceinline__ int64_t slot(int p, int heads) const {
+    return (int64_t)(2 * (c0 + p) + (p == 0 && late ? 1 : 0)) * heads + row;
+  }
+};
+__device__ __forceinline__ bool find_parts(const Args& a, int t, int h, int heads, Parts& q, bool& empty, bool& fill) {
   const int first = a.plan[1 + t], run = a.plan[0], n = first < 0 ? 0 : a.counts[t];
+  empty = n == 0;
+  fill = first >= 0 || a.fill_tail;
+  if (empty) return false;
+  const int g = h / heads, f = first + g * n, c1 = (f + n - 1) / run;
+  q.c0 = f / run;
+  q.count = c1 - q.c0 + 1;
+  q.row = h - g * heads;
+  q.late = f != q.c0 * run;
+  return q.count > 1;
+}
+
+// One warp's weights of all parts into `weight`; returns (1 / sum, lse).
+constexpr int kPartRounds = kMaxGrid / 32;
+__device__ __forceinline__ float2 part_weights(const Args& a, const Parts& q, int heads, float* weight, bool store) {
+  const int lane = threadIdx.x & 31;
+  float m[kPartRounds], l[kPartRounds], top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kPartRounds; ++k) {
+    const int p = lane + 32 * k;
+    m[k] = p < q.count ? a.pm[q.slot(p, heads)] : -INFINITY;
+    l[k] = p < q.count ? a.pl[q.slot(p, heads)] : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < kPartRounds; ++k) top = fmaxf(top, m[k]);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int k = 0; k < kPartRounds; ++k) {
+    const int p = lane + 32 * k;
+    const float w = ex2(m[k] - base);
+    if (store && p < q.count) weight[p] = w;
+    sum = fmaf(l[k], w, sum);
+  }
+  sum = warp_sum(sum);
+  return make_float2(1.f / sum, (base + log2f(sum)) * kLn2);
+}
+
+__device__ __forceinline__ void add_part(float4& o, float w, const float4& x) {
+  o.x = fmaf(w, x.x, o.x);
+  o.y = fmaf(w, x.y, o.y);
+  o.z = fmaf(w, x.z, o.z);
+  o.w = fmaf(w, x.w, o.w);
+}
+template <typename E>
+__device__ __forceinline__ void store_joined(uint16_t* dst, const float4& o, float inv) {
+  *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<E>::pack(o.x * inv, o.y * inv), Elem<E>::pack(o.z * inv, o.w * inv));
+}
+
+// Few results: a block takes 128 values of one (token, head), and each of 16
+// warps every 16th part of them.
+template <typename E>
+__global__ void __launch_bounds__(512) join_few_kernel(Args a, int heads) {
+  __shared__ float weight[kMaxGrid];
+  __shared__ float4 part[16][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int t = blockIdx.x, h = blockIdx.y, way = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = 4 * (blockIdx.z * 32 + lane);
   const int64_t at = (int64_t)t * a.H + h;
-  const int way = threadIdx.x / kCols, col = 4 * (blockIdx.z * kCols + threadIdx.x % kCols);
   const bool mine = col < a.R;
-  if (n == 0) {
-    if (first < 0 && !a.fill_tail) return;
+  Parts q;
+  bool empty, fill;
+  if (!find_parts(a, t, h, heads, q, empty, fill)) {
+    if (!empty || !fill) return;
     if (way == 0 && mine) *reinterpret_cast<uint2*>(a.out + at * a.R + col) = make_uint2(0, 0);
     if (a.lse && threadIdx.x == 0 && blockIdx.z == 0) a.lse[at] = -INFINITY;
     return;
   }
-  const int f = first + (h / heads) * n, c0 = f / run, c1 = (f + n - 1) / run, hl = h % heads;
-  if (c0 == c1) return;
-  // a CTA's first segment is its slot 2 c, a last one that begins a unit 2 c + 1
-  const bool late = f != c0 * run;
-  const int parts = c1 - c0 + 1;
-  auto slot = [&](int p) { return (int64_t)(2 * (c0 + p) + (p == 0 && late ? 1 : 0)) * heads + hl; };
-  // the first rows are on their way while the weights are formed
-  constexpr int kBatch = 6;
-  float4 x[kBatch];
+  constexpr int kBatch = 5;
+  float4 x[kBatch], o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int k = 0; k < kBatch; ++k) {
-    const int p = way + k * WAYS;
-    x[k] = mine && p < parts ? *reinterpret_cast<const float4*>(a.po + slot(p) * a.R + col)
-                             : make_float4(0.f, 0.f, 0.f, 0.f);
+    const int p = way + 16 * k;
+    x[k] = mine && p < q.count ? *reinterpret_cast<const float4*>(a.po + q.slot(p, heads) * a.R + col) : o;
   }
-  const int lane = threadIdx.x & 31;
-  float top = -INFINITY, sum = 0.f;
-  for (int p = lane; p < parts; p += 32) top = fmaxf(top, a.pm[slot(p)]);
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.f : top;
-  for (int p = lane; p < parts; p += 32) {
-    const float w = ex2(a.pm[slot(p)] - base);
-    if (threadIdx.x < 32) weight[p] = w;
-    sum = fmaf(a.pl[slot(p)], w, sum);
-  }
-  sum = warp_sum(sum);
+  const float2 total = part_weights(a, q, heads, weight, way == 0);
   __syncthreads();
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = way; p0 < parts; p0 += kBatch * WAYS) {
+  for (int p0 = way; p0 < q.count; p0 += kBatch * 16) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int p = p0 + k * WAYS, next = p + kBatch * WAYS;
-      const float w = p < parts ? weight[p] : 0.f;
-      o.x = fmaf(w, x[k].x, o.x);
-      o.y = fmaf(w, x[k].y, o.y);
-      o.z = fmaf(w, x[k].z, o.z);
-      o.w = fmaf(w, x[k].w, o.w);
-      x[k] = mine && next < parts ? *reinterpret_cast<const float4*>(a.po + slot(next) * a.R + col)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+      const int p = p0 + 16 * k, next = p + 16 * kBatch;
+      if (p < q.count) add_part(o, weight[p], x[k]);
+      if (mine && next < q.count) x[k] = *reinterpret_cast<const float4*>(a.po + q.slot(next, heads) * a.R + col);
     }
   }
-  if constexpr (WAYS > 1) {
-    part[way][threadIdx.x % kCols] = o;
-    __syncthreads();
-    if (way) return;
+  part[way][lane] = o;
+  __syncthreads();
+  if (way) return;
 #pragma unroll
-    for (int k = 1; k < WAYS; ++k) {
-      const float4 x = part[k][threadIdx.x % kCols];
-      o.x += x.x;
-      o.y += x.y;
-      o.z += x.z;
-      o.w += x.w;
+  for (int k = 1; k < 16; ++k) add_part(o, 1.f, part[k][lane]);
+  if (mine) store_joined<E>(a.out + at * a.R + col, o, total.x);
+  if (a.lse && threadIdx.x == 0 && blockIdx.z == 0) a.lse[at] = total.y;
+}
+
+// Many results: a warp takes one (token, head), 16 values a lane.
+template <typename E>
+__global__ void __launch_bounds__(128) join_many_kernel(Args a, int heads) {
+  __shared__ float weights[4][kMaxGrid];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y * 4 + warp;
+  if (h >= a.H) return;
+  const int64_t at = (int64_t)t * a.H + h;
+  uint16_t* dst = a.out + at * a.R + 4 * lane;
+  Parts q;
+  bool empty, fill;
+  if (!find_parts(a, t, h, heads, q, empty, fill)) {
+    if (!empty || !fill) return;
+    for (int c = 0; c < a.R; c += 128) *reinterpret_cast<uint2*>(dst + c) = make_uint2(0, 0);
+    if (a.lse && lane == 0) a.lse[at] = -INFINITY;
+    return;
+  }
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 x[2][4], o[4];
+  auto load = [&](int p, float4 (&y)[4]) {
+    const float* src = a.po + q.slot(p, heads) * a.R + 4 * lane;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) y[c] = 128 * c < a.R ? *reinterpret_cast<const float4*>(src + 128 * c) : zero;
+  };
+  load(0, x[0]);
+  load(1, x[1]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) o[c] = zero;
+  const float2 total = part_weights(a, q, heads, weights[warp], true);
+  __syncwarp();
+  for (int p0 = 0; p0 < q.count; p0 += 2) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int p = p0 + k;
+      if (p < q.count) {
+        const float w = weights[warp][p];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) add_part(o[c], w, x[k][c]);
+        if (p + 2 < q.count) load(p + 2, x[k]);
+      }
     }
   }
-  if (mine) {
-    const float inv = 1.f / sum;
-    *reinterpret_cast<uint2*>(a.out + at * a.R + col) =
-        make_uint2(Elem<E>::pack(o.x * inv, o.y * inv), Elem<E>::pack(o.z * inv, o.w * inv));
-  }
-  if (a.lse && threadIdx.x == 0 && blockIdx.z == 0) a.lse[at] = (base + log2f(sum)) * kLn2;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (128 * c < a.R) store_joined<E>(dst + 128 * c, o[c], total.x);
+  if (a.lse && lane == 0) a.lse[at] = total.y;
 }
 
 int grid_size() { return std::min(sm_count(), kMaxGrid); }
@@ -773,9 +845,10 @@ int launch(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMap& kv0,
   absorbed_kernel<E, N><<<grid_size(), kThreads, kSmemBytes, st>>>(ql, qr, kv0, kv1, a);
   if ((rc = check_launch("absorbed_kernel"))) return rc;
   if (a.T * a.H <= 512)
-    launch_programmatic(join_kernel<E, 16>, dim3((unsigned)a.T, (unsigned)a.H, 4), dim3(512), 0, st, a, N);
+    launch_programmatic(join_few_kernel<E>, dim3((unsigned)a.T, (unsigned)a.H, (unsigned)(a.R / 128)), dim3(512), 0,
+                        st, a, N);
   else
-    launch_programmatic(join_kernel<E, 1>, dim3((unsigned)a.T, (unsigned)a.H), dim3(128), 0, st, a, N);
+    launch_programmatic(join_many_kernel<E>, dim3((unsigned)a.T, (unsigned)((a.H + 3) / 4)), dim3(128), 0, st, a, N);
   return check_launch("join_kernel");
 }
 
