@@ -29,8 +29,8 @@
 // one CTA's run is finished there; others leave FP32 partial results (at most
 // two a CTA) that a second kernel joins.
 //
-// Roles: warps 0-3 softmax (a 16-key strip each) and epilogue, warp 4 TMA,
-// warp 5 issues S^T, warp 6 issues O^T; in the last three one lane waits and
+// Roles: warps 0-7 softmax (a strip of 16 keys and half of the heads each) and
+// epilogue, warp 8 TMA, warp 9 issues S^T, warp 10 issues O^T; in the last three one lane waits and
 // issues, since a lane that spins must not hold up one with work.  Row maxima are replaced only when a
 // score passes them by 2^8 (latent.cuh).  A token never shares a tile's keys
 // with one that sees fewer, so only rows behind a request's end are masked:
@@ -58,7 +58,8 @@ constexpr int kChunkBytes = kKeys * 128;   // 64 rows of 64 values
 constexpr int kMaxChunks = 9;
 constexpr int kAtomBytes = 1024;           // 8 rows of a chunk
 constexpr int kStageBytes = kMaxChunks * kChunkBytes;
-constexpr int kSoftThreads = 128;
+constexpr int kSoftWarps = 8;
+constexpr int kSoftThreads = kSoftWarps * 32;
 constexpr int kThreads = kSoftThreads + 96;
 constexpr int kMaxGrid = 256;              // parts a join block holds weights of, halved
 constexpr int kSCol = 256;                 // TMEM: O^T at 0..255, two S^T tiles behind
@@ -206,13 +207,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       n += tiles_of(q, a.G);
       if (q.bad && blockIdx.x == 0) report(a.status, a.status_host, kStatusBadGeometry);
     }
-    if (warp == 5) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                       smem_addr(&bars->tmem_base)),
-                   "r"(512)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    } else if (warp == 4 && lane == 0) {
+    if (warp == 9) {
+      tmem_alloc_all<false>(smem_addr(&bars->tmem_base));
+    } else if (warp == 8 && lane == 0) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&ql_map)) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qr_map)) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kv0_map)) : "memory");
@@ -228,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_init(bar(&bars->empty[b][h]), 1);
         }
         mbar_init(bar(&bars->s_full[b]), 1);
-        mbar_init(bar(&bars->p_full[b]), 4);
+        mbar_init(bar(&bars->p_full[b]), kSoftWarps);
         mbar_init(bar(&bars->drain[b]), 1);
       }
       mbar_init(bar(&bars->o_done), 1);
@@ -295,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Segment sg;
   uint32_t n = 0;  // tiles so far, over all segments
 
-  if (warp == 4) {
+  if (warp == 8) {
     // ---------------- TMA ----------------
     // Lane 0 waits and issues; the lanes look up a tile's boxes side by side.
     const int boxes = kKeys / a.box, box_groups = a.box / 8;
@@ -303,19 +300,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t queries = 0;  // Q tiles asked for
     int at_half = 0;
     while (next_segment(a, cur, sg)) {
-      if (lane == 0) {
-        if (queries) ok = ok && mbar_wait_fast(bar(&bars->q_empty), (queries - 1) & 1u, abort_flag);
-        if (ok) {
-          ++queries;
-          mbar_expect_tx(bar(&bars->q_full), (a.R + a.r) / 64 * (N * 128));
-          for (int c = 0; c < a.R / 64; ++c)
-            tma_load_3d(smem_addr(q_smem + c * (N * 128)), &ql_map, c * 64, sg.g * N, sg.token, bar(&bars->q_full));
-          if (a.r)
-            tma_load_3d(smem_addr(q_smem + a.R / 64 * (N * 128)), &qr_map, 0, sg.g * N, sg.token,
-                        bar(&bars->q_full));
-        }
-      }
-      __syncwarp();
       // lane k looks up box k of a tile: rows pos .. pos + box of the request
       const int32_t* row = a.table + sg.request * a.table_stride;
       auto place = [&](int t) {  // group of eight rows in the cache, -1 for none
@@ -330,6 +314,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         return (id * a.page + (pos - at * a.page)) / 8;
       };
       int next = place(sg.tile);
+      if (lane == 0) {
+        if (queries) ok = ok && mbar_wait_fast(bar(&bars->q_empty), (queries - 1) & 1u, abort_flag);
+        if (ok) {
+          ++queries;
+          mbar_expect_tx(bar(&bars->q_full), (a.R + a.r) / 64 * (N * 128));
+          for (int c = 0; c < a.R / 64; ++c)
+            tma_load_3d(smem_addr(q_smem + c * (N * 128)), &ql_map, c * 64, sg.g * N, sg.token, bar(&bars->q_full));
+          if (a.r)
+            tma_load_3d(smem_addr(q_smem + a.R / 64 * (N * 128)), &qr_map, 0, sg.g * N, sg.token,
+                        bar(&bars->q_full));
+        }
+      }
+      __syncwarp();
       for (int t = sg.tile; t < sg.tile + sg.n; ++t) {
         const int count = __popc(__ballot_sync(0xffffffffu, next >= 0));
         int y[8];
@@ -372,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncwarp();
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // ---------------- S^T = rows . Q^T ----------------
     // All lanes walk the loops, so that descriptors stay uniform; one waits and issues.
     const bool leader = elect_one();
@@ -415,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait(bar(&bars->drain[0]), 0, &never)) *abort_flag = 1;
     }
     __syncwarp();
-  } else if (warp == 6) {
+  } else if (warp == 10) {
     // ---------------- O^T += c^T . P^T ----------------
     const bool leader = elect_one();
     constexpr uint32_t id_o = make_idesc_f16(128, N, bf16, true, true);
@@ -463,14 +460,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ---------------- softmax, epilogue ----------------
-    // this thread's keys of a tile: k0 and k0 + 8; its heads: 8 j + h0 + {0, 1}
-    const int k0 = 16 * warp + (lane >> 2), h0 = 2 * (lane & 3);
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    // this thread's keys of a tile: k0 and k0 + 8; its heads: h0 + 8 j + {0, 1}
+    constexpr int kHalf = N / 2, kOwn = N / 8;  // heads of a warp, of a thread
+    const int strip = warp & 3, side = warp >> 2;
+    const int k0 = 16 * strip + (lane >> 2), h0 = side * kHalf + 2 * (lane & 3);
+    const uint32_t lanes = (uint32_t)(strip * 32) << 16;
     bool stop = false;
     for (int segment = 0; !stop && next_segment(a, cur, sg); ++segment) {
-      float m[N / 4], l[N / 4];
+      float m[kOwn], l[kOwn];
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
+      for (int i = 0; i < kOwn; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.f;
       }
@@ -478,19 +477,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t b = n & 1, use = n >> 1;
         if (!mbar_wait_warp(bar(&bars->s_full[b]), use & 1u, abort_flag)) stop = true;
         const int valid = min(kKeys, sg.visible - (sg.tile + t) * kKeys);
-        float v[N / 2];
+        float v[2 * kOwn];
         bool grow = stop;
         if (!stop) {
           tmem_fence_after();
-          uint32_t w[N / 2];
-          tmem_ld16_frag(lanes + kSCol + b * N, w);
+          uint32_t w[2 * kOwn];
+          tmem_ld16_frag(lanes + kSCol + b * N + side * kHalf, w);
           tmem_wait_ld();
           const bool in0 = k0 < valid, in1 = k0 + 8 < valid;
 #pragma unroll
-          for (int i = 0; i < N / 2; ++i)
+          for (int i = 0; i < 2 * kOwn; ++i)
             v[i] = ((i & 2) ? in1 : in0) ? __uint_as_float(w[i]) * a.c : -INFINITY;
 #pragma unroll
-          for (int i = 0; i < N / 4; ++i) {
+          for (int i = 0; i < kOwn; ++i) {
             const int e = (i >> 1) * 4 + (i & 1);
             grow |= fmaxf(v[e], v[e + 2]) > m[i] + kMaxSlack;
           }
@@ -510,29 +509,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           stop = any_of(stop, 1, kSoftThreads);
           if (stop) break;
 #pragma unroll
-          for (int i = 0; i < N / 4; ++i) {
+          for (int i = 0; i < kOwn; ++i) {
             const int e = (i >> 1) * 4 + (i & 1);
             float x = fmaxf(v[e], v[e + 2]);
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            if (lane < 4) bars->xchg[warp][8 * (i >> 1) + h0 + (i & 1)] = x;
+            if (lane < 4) bars->xchg[strip][8 * (i >> 1) + h0 + (i & 1)] = x;
           }
           bar_sync(1, kSoftThreads);
 #pragma unroll
-          for (int i = 0; i < N / 4; ++i) {
+          for (int i = 0; i < kOwn; ++i) {
             const int h = 8 * (i >> 1) + h0 + (i & 1);
             const float top = fmaxf(m[i], fmaxf(fmaxf(bars->xchg[0][h], bars->xchg[1][h]),
                                                 fmaxf(bars->xchg[2][h], bars->xchg[3][h])));
             const float f = top == m[i] ? 1.f : ex2(m[i] - top);
             m[i] = top;
             l[i] *= f;
-            if (tid < 4) bars->factor[h] = f;
+            if (strip == 0 && lane < 4) bars->factor[h] = f;
           }
           bar_sync(1, kSoftThreads);
           if (t > 0 && mbar_wait_warp(bar(&bars->o_done), (n - 1) & 1u, abort_flag)) {
             tmem_fence_after();
-            for (int o = 0; o < groups * N; o += 16) {
+            for (int o = 16 * side; o < groups * N; o += 32) {
               uint32_t w[16];
               tmem_ld16(lanes + o, w);
               tmem_wait_ld();
@@ -545,9 +544,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // P^T: rows of keys, 64 heads of 2 bytes, 128-byte swizzle
-        uint32_t p0[N / 8], p1[N / 8];
+        uint32_t p0[kOwn / 2], p1[kOwn / 2];
 #pragma unroll
-        for (int j = 0; j < N / 8; ++j) {
+        for (int j = 0; j < kOwn / 2; ++j) {
           const float s0 = m[2 * j] == -INFINITY ? 0.f : m[2 * j], s1 = m[2 * j + 1] == -INFINITY ? 0.f : m[2 * j + 1];
           const float a0 = ex2(v[4 * j] - s0), a1 = ex2(v[4 * j + 1] - s1);
           const float b0 = ex2(v[4 * j + 2] - s0), b1 = ex2(v[4 * j + 3] - s1);
@@ -558,8 +557,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (n > 0) mbar_wait_warp(bar(&bars->o_done), (n - 1) & 1u, abort_flag);  // P^T of the last tile is read
 #pragma unroll
-        for (int j = 0; j < N / 8; ++j) {
-          uint8_t* at = p_smem + k0 * 128 + ((j ^ (k0 & 7)) << 4) + 2 * h0;
+        for (int j = 0; j < kOwn / 2; ++j) {
+          uint8_t* at = p_smem + k0 * 128 + (((side * (kHalf / 8) + j) ^ (k0 & 7)) << 4) + 4 * (lane & 3);
           *reinterpret_cast<uint32_t*>(at) = p0[j];
           *reinterpret_cast<uint32_t*>(at + 8 * 128) = p1[j];
         }
@@ -573,17 +572,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (stop) break;
       // row sums over the 64 keys of every strip
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
+      for (int i = 0; i < kOwn; ++i) {
         float x = l[i];
         x += __shfl_xor_sync(0xffffffffu, x, 4);
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
-        if (lane < 4) bars->xchg[warp][8 * (i >> 1) + h0 + (i & 1)] = x;
+        if (lane < 4) bars->xchg[strip][8 * (i >> 1) + h0 + (i & 1)] = x;
       }
       bar_sync(1, kSoftThreads);
-      if (tid < 4) {
+      if (strip == 0 && lane < 4) {
 #pragma unroll
-        for (int i = 0; i < N / 4; ++i) bars->top[8 * (i >> 1) + h0 + (i & 1)] = m[i];
+        for (int i = 0; i < kOwn; ++i) bars->top[8 * (i >> 1) + h0 + (i & 1)] = m[i];
       }
       bar_sync(1, kSoftThreads);
       const int heads = min(N, a.H - sg.g * N);
@@ -607,11 +606,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       // bytes a warp in FP32; for the 16-bit result lane pairs exchange values
       const int odd = lane & 1;
 #pragma unroll 2
-      for (int o = 0; o < groups * N; o += 16) {
+      for (int o = 16 * side; o < groups * N; o += 32) {
         uint32_t w[16];
         tmem_ld16(lanes + o, w);
         const int hb = o & (N - 1), lim = heads - hb;
-        const int64_t col = (int64_t)(o / N) * 128 + tid;
+        const int64_t col = (int64_t)(o / N) * 128 + strip * 32 + lane;
         tmem_wait_ld();
         if (!whole) {
           float* part = a.po + (slot * N + hb) * a.R + col;
@@ -644,9 +643,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if (tid == 0 && bars->abort_flag) report(a.status, a.status_host, kStatusWaitTimeout);
-  if (warp == 5) {
+  if (warp == 9) {
     tmem_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars->tmem_base), "r"(512) : "memory");
+    tmem_free_all<false>(bars->tmem_base);
   }
 }
 
