@@ -173,6 +173,7 @@ SIGNATURES: dict[str, tuple] = {
         [_vp, _i64, _i64, _i64, _i64, _int, _vp, _f, _vp, _vp, _int, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp,
          _vp, _vp, _vp],
     ),
+    "glm53_latent_call": (_int, [_int, ctypes.c_char_p]),
     "glm53_latent_absorbed_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "glm53_latent_absorbed": (
         _int,

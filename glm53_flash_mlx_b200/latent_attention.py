@@ -25,6 +25,7 @@ safe result and the next call of this module raises (``IndexError`` /
 from __future__ import annotations
 
 import functools
+import struct
 from typing import NamedTuple
 
 import torch
@@ -72,22 +73,38 @@ def _device(first: torch.Tensor, *rest: torch.Tensor | None) -> int:
     return index
 
 
-def _call(name: str, index: int, *args) -> None:
-    """One C-ABI call on the device's current stream with its status word, whatever the current device is."""
-    sw, word, host, mirror = _status(index)
-    if mirror.value:
-        sw.raise_pending()
-    fn = getattr(N.lib() if N._lib is None else N._lib, name)
-    stream = _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, word, host, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, word, host, stream)
-    if rc:
-        N.check(rc, name)
-    if _SYNC_STATUS:
-        sw.check()
+class _Entry:
+    """One C-ABI entry point, called through ``glm53_latent_call``: a word per argument (``floats`` names the
+    positions that hold floating-point values; 0 stands for NULL) costs a third of converting each of them."""
+
+    def __init__(self, number: int, count: int, floats: tuple = ()):
+        self.number = number
+        # three more words: status, its mirror, the stream
+        self.pack = struct.Struct("".join("d" if i in floats else "q" for i in range(count + 3))).pack
+
+    def __call__(self, index: int, *args) -> None:
+        """Call on the device's current stream with its status word, whatever the current device is."""
+        sw, word, host, mirror = _status(index)
+        if mirror.value:
+            sw.raise_pending()
+        lib = N._lib or N.lib()
+        stream = _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
+        words = self.pack(*args, word, host, stream)
+        if torch.cuda.current_device() == index:
+            rc = lib.glm53_latent_call(self.number, words)
+        else:
+            with torch.cuda.device(index):
+                rc = lib.glm53_latent_call(self.number, words)
+        if rc:
+            N.check(rc, "glm53_latent_call")
+        if _SYNC_STATUS:
+            sw.check()
+
+
+_PLAN_PAGES = _Entry(0, 16)
+_CACHE_WRITE = _Entry(1, 19, floats=(7,))
+_ABSORBED = _Entry(2, 26, floats=(20,))
+_EXPANDED = _Entry(3, 29, floats=(24,))
 
 
 def _int32(t: torch.Tensor, name: str, count: int) -> torch.Tensor:
@@ -189,7 +206,7 @@ def plan_pages(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     words = cached_lens.new_empty(tokens + 2 * B + 2)
     positions, starts, lens, left = words.split_with_sizes([tokens, B + 1, B, 1])
     at = words.data_ptr()
-    _call("glm53_plan_pages", index, cached_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), stride,
+    _PLAN_PAGES(index, cached_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), stride,
           width, free_pages.data_ptr(), pages, free_count.data_ptr(), page_size, tokens, slots.data_ptr(), at,
           at + 4 * tokens, at + 4 * (tokens + B + 1), at + 4 * (tokens + 2 * B + 1))
     return PagePlan(slots, positions, starts, lens, left)
@@ -225,15 +242,15 @@ def latent_cache_write(kv: torch.Tensor, cache: torch.Tensor, slots: torch.Tenso
         raise ValueError(f"slots must be int64 [{T}], got {slots.dtype} {list(slots.shape)}")
     if (positions is None) != (inv_freq is None):
         raise ValueError("positions and inv_freq come together")
-    wp = pp = fp = None
+    wp = pp = fp = 0
     if norm_weight is not None:
         norm_weight, wp, _ = _pieces(_same(norm_weight, "norm_weight", kv.dtype, (latent,)))
     if positions is not None:
         positions = _int32(positions, "positions", T)
         inv_freq = _same(inv_freq, "inv_freq", torch.float64, (rope_dim // 2,)).contiguous()
         pp, fp = positions.data_ptr(), inv_freq.data_ptr()
-    rotated = qp = rp = None
-    heads = qt = qh = 0
+    rotated = None
+    qp = rp = heads = qt = qh = 0
     if queries is not None:
         if positions is None:
             raise ValueError("queries are rotated by positions and inv_freq, which are missing")
@@ -250,7 +267,7 @@ def latent_cache_write(kv: torch.Tensor, cache: torch.Tensor, slots: torch.Tenso
     kv, kp, (kt,) = _pieces(kv)
     if not slots.is_contiguous():
         slots = slots.contiguous()
-    _call("glm53_latent_cache_write", index, kp, T, kt if kt > width else width, latent, rope_dim, code, wp, eps, pp, fp,
+    _CACHE_WRITE(index, kp, T, kt if kt > width else width, latent, rope_dim, code, wp, eps, pp, fp,
           interleaved, slots.data_ptr(), cache.data_ptr(), cache.shape[0] * cache.shape[1], qp, heads, qt, qh, rp)
     return rotated
 
@@ -293,7 +310,7 @@ def latent_attention_absorbed(q_latent: torch.Tensor, q_rope: torch.Tensor | Non
     B = seq_lens.numel()
     seq_lens = _int32(seq_lens, "seq_lens", B)
     _table(block_table, B)
-    sp = None
+    sp = 0
     if query_starts is not None:
         query_starts = _int32(query_starts, "query_starts", B + 1)
         sp = query_starts.data_ptr()
@@ -311,16 +328,15 @@ def latent_attention_absorbed(q_latent: torch.Tensor, q_rope: torch.Tensor | Non
     lse = q_latent.new_empty((T, H), dtype=torch.float32) if return_lse else None
     if T:
         q_latent, lp, (lt, lh) = _pieces(q_latent)
-        rp = None
-        rt = rh = 0
+        rp = rt = rh = 0
         if rope:
             q_rope, rp, (rt, rh) = _pieces(q_rope)
         nbytes = _absorbed_bytes(T, H, R, index)
         # from the caching allocator: ordered on this stream, private to a captured graph
         ws = q_latent.new_empty((nbytes + 1) // 2)
-        _call("glm53_latent_absorbed", index, lp, lt, lh, rp, rt, rh, T, H, R, rope, code, cache.data_ptr(), pages,
+        _ABSORBED(index, lp, lt, lh, rp, rt, rh, T, H, R, rope, code, cache.data_ptr(), pages,
               page_size, block_table.data_ptr(), stride, width, seq_lens.data_ptr(), B, sp, scale, result.data_ptr(),
-              None if lse is None else lse.data_ptr(), out is None, ws.data_ptr(), nbytes)
+              0 if lse is None else lse.data_ptr(), out is None, ws.data_ptr(), nbytes)
     return (result, lse) if return_lse else result
 
 
@@ -373,12 +389,11 @@ def latent_attention_expanded(q_nope: torch.Tensor, q_rope: torch.Tensor | None,
         q_nope, qp, (qt, qh) = _pieces(q_nope)
         k_nope, kp, (kt, kh) = _pieces(k_nope)
         values, vp, (vt, vh) = _pieces(values)
-        qrp = krp = None
-        qrt = qrh = krt = 0
+        qrp = krp = qrt = qrh = krt = 0
         if dr:
             q_rope, qrp, (qrt, qrh) = _pieces(q_rope)
             k_rope, krp, (krt,) = _pieces(k_rope)
-        _call("glm53_latent_expanded", index, qp, qt, qh, qrp, qrt, qrh, kp, kt, kh, krp, krt, vp, vt, vh, Tq, Tk, H, dn,
+        _EXPANDED(index, qp, qt, qh, qrp, qrt, qrh, kp, kt, kh, krp, krt, vp, vt, vh, Tq, Tk, H, dn,
               dr, dv, code, query_starts.data_ptr(), key_starts.data_ptr(), B, scale, causal, result.data_ptr(),
-              None if lse is None else lse.data_ptr(), out is None)
+              0 if lse is None else lse.data_ptr(), out is None)
     return (result, lse) if return_lse else result

@@ -794,6 +794,16 @@ int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, int64_t qn_st
                           int causal, void* out, float* lse, int fill_tail, uint32_t* status, uint32_t* status_host,
                           void* stream);
 
+/* The four entry points above for bindings that pay for every argument they
+ * convert: the arguments of `entry` (GLM53_LATENT_*) in their order, one 64-bit
+ * word each (integers sign-extended, pointers, floats as doubles), 8-byte
+ * aligned. */
+#define GLM53_LATENT_PLAN_PAGES 0
+#define GLM53_LATENT_CACHE_WRITE 1
+#define GLM53_LATENT_ABSORBED 2
+#define GLM53_LATENT_EXPANDED 3
+int glm53_latent_call(int entry, const void* words);
+
 #ifdef __cplusplus
 }
 #endif

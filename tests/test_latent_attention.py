@@ -156,6 +156,26 @@ def test_expanded_refuses(bad):
     assert lib().glm53_latent_expanded(*expanded_args(**bad)) == 1
 
 
+@pytest.mark.parametrize("entry,make,bads", [
+    (0, plan_args, [dict(B=-1), dict(page=0), dict(out=ONE)]),
+    (1, write_args, [dict(dtype=2), dict(R=12), dict(kv=8), dict(qo=None)]),
+    (2, absorbed_args, [dict(T=3), dict(scale=math.nan), dict(wsb=1), dict(width=5)]),
+    (3, expanded_args, [dict(dv=32), dict(scale=math.inf), dict(B=70000), dict(qs=None)]),
+])
+def test_packed_call_refuses_alike(entry, make, bads):
+    import struct
+
+    names = ["glm53_plan_pages", "glm53_latent_cache_write", "glm53_latent_absorbed", "glm53_latent_expanded"]
+    for bad in bads:
+        args = make(**bad)
+        rc = getattr(lib(), names[entry])(*args)
+        why = lib().glm53_last_error()
+        words = b"".join(struct.pack("d" if isinstance(a, float) else "q", a or 0) for a in args)
+        assert lib().glm53_latent_call(entry, words) == rc == 1
+        assert lib().glm53_last_error() == why
+    assert lib().glm53_latent_call(9, b"\0" * 400) == 1 and lib().glm53_latent_call(entry, None) == 1
+
+
 def test_python_refuses_before_the_device():
     import glm53_flash_mlx_b200 as G
 
