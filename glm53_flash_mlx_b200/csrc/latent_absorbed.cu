@@ -62,6 +62,7 @@ constexpr int kSoftWarps = 8;
 constexpr int kSoftThreads = kSoftWarps * 32;
 constexpr int kThreads = kSoftThreads + 96;
 constexpr int kMaxGrid = 256;              // parts a join block holds weights of, halved
+constexpr int kFewTokens = 64;             // of a request, planned by one thread
 constexpr int kSCol = 256;                 // TMEM: O^T at 0..255, two S^T tiles behind
 
 struct Args {
@@ -251,15 +252,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int run = max(1, (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x));
     const int64_t begin = (int64_t)blockIdx.x * run;
     if (blockIdx.x == 0) {
+      // what the join looks up: every token's first tile and tiles.  A request
+      // with many tokens leaves only its first one's, and the block fills the rest.
       if (tid == 0) a.plan[0] = run;
+      bool many = false;
       int f = before;
       for (int i = i0; i < i1; ++i) {
         const Request q = request_at(a, i);
+        if (q.nq > kFewTokens) {
+          many = true;
+          a.plan[1 + q.q0] = f;
+          f += tiles_of(q, a.G);
+          continue;
+        }
         for (int j = 0; j < q.nq; ++j) {
           const int k = tiles_of(visible_of(q, j));
           a.plan[1 + q.q0 + j] = f;
           a.counts[q.q0 + j] = k;
           f += k * a.G;
+        }
+      }
+      if (__syncthreads_or(many)) {
+        for (int i = 0; i < a.B; ++i) {
+          const Request q = request_at(a, i);
+          if (q.nq <= kFewTokens) continue;
+          const int at = *(volatile int32_t*)(a.plan + 1 + q.q0);
+          const int64_t skipped = tiles_up_to((int64_t)q.len - q.nq);
+          __syncthreads();
+          for (int j = tid; j < q.nq; j += kThreads) {
+            a.plan[1 + q.q0 + j] = at + (int)(tiles_up_to((int64_t)q.len - q.nq + j) - skipped) * a.G;
+            a.counts[q.q0 + j] = tiles_of(visible_of(q, j));
+          }
         }
       }
     }
@@ -272,8 +295,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           f += all;
           continue;
         }
-        int j = 0;
-        while (begin >= f + tiles_of(visible_of(q, j)) * a.G) f += tiles_of(visible_of(q, j++)) * a.G;
+        // the last token whose first tile is not behind `begin`
+        const int64_t skipped = tiles_up_to((int64_t)q.len - q.nq);
+        auto first_of = [&](int j) { return f + (int)(tiles_up_to((int64_t)q.len - q.nq + j) - skipped) * a.G; };
+        int j = 0, hi = q.nq;
+        while (hi - j > 1) {
+          const int mid = (j + hi) >> 1;
+          if (first_of(mid) <= begin)
+            j = mid;
+          else
+            hi = mid;
+        }
+        f = first_of(j);
         const int k = tiles_of(visible_of(q, j)), rest = (int)(begin - f);
         const int g = a.G == 1 ? 0 : rest / k;
         bars->cursor = Cursor{i, j, g, rest - g * k, min(run, total - (int)begin)};

@@ -146,12 +146,27 @@ def _table(t: torch.Tensor, requests: int) -> None:
         raise ValueError(f"block_table must be int32 [{requests}, pages], got {t.dtype} {list(t.shape)}")
 
 
-def _output(out: torch.Tensor | None, like: torch.Tensor, shape: tuple) -> torch.Tensor:
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses that `t`'s elements lie in."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _output(out: torch.Tensor | None, shape: tuple, like: torch.Tensor, *rest: torch.Tensor | None) -> torch.Tensor:
     if out is None:
         return like.new_empty(shape)
     if not out.is_contiguous():
         raise ValueError("out must be contiguous")
-    return _same(out, "out", like.dtype, shape)
+    _same(out, "out", like.dtype, shape)
+    a, b = _span(out)
+    for t in (like, *rest):
+        if t is not None:
+            c, d = _span(t)
+            if a < d and c < b:
+                raise ValueError("out must not overlap an input")
+    return out
 
 
 @functools.lru_cache(maxsize=4096)
@@ -226,7 +241,8 @@ def latent_cache_write(kv: torch.Tensor, cache: torch.Tensor, slots: torch.Tenso
     ``interleaved``.  Unlike ``rms_norm`` the row is rounded once, at its store.
     ``cache`` [pages, page_size, latent + rope] is contiguous; ``slots`` int64
     [tokens] (``PagePlan.slots``): a negative slot stores nothing; slots are
-    distinct (of two tokens with one slot either row stays).  ``queries``
+    distinct (of two tokens with one slot either row stays).  ``kv`` and ``queries`` lie
+    outside the cache.  ``queries``
     [tokens, heads, rope_dim] are rotated likewise into a new tensor, which is
     returned (None without queries).
     """
@@ -324,7 +340,7 @@ def latent_attention_absorbed(q_latent: torch.Tensor, q_rope: torch.Tensor | Non
         stride = width
     if B <= 1:
         stride = width
-    result = _output(out, q_latent, (T, H, R))
+    result = _output(out, (T, H, R), q_latent, q_rope, cache)
     lse = q_latent.new_empty((T, H), dtype=torch.float32) if return_lse else None
     if T:
         q_latent, lp, (lt, lh) = _pieces(q_latent)
@@ -383,7 +399,7 @@ def latent_attention_expanded(q_nope: torch.Tensor, q_rope: torch.Tensor | None,
     query_starts = _int32(query_starts, "query_starts", B + 1)
     key_starts = _int32(key_starts, "key_starts", B + 1)
     index = _device(q_nope, q_rope, k_nope, k_rope, values, query_starts, key_starts, out)
-    result = _output(out, q_nope, (Tq, H, dv))
+    result = _output(out, (Tq, H, dv), q_nope, q_rope, k_nope, k_rope, values)
     lse = q_nope.new_empty((Tq, H), dtype=torch.float32) if return_lse else None
     if Tq:
         q_nope, qp, (qt, qh) = _pieces(q_nope)

@@ -747,7 +747,8 @@ int glm53_plan_pages(const int32_t* cached_lens, const int32_t* new_lens, int64_
  * (2 i, 2 i + 1) when interleaved), computed in FP32 and rounded once.
  * kv [tokens, latent_dim + rope_dim], rows kv_stride apart; slots int64: < 0
  * skips the token, >= cache_rows sets GLM53_STATUS_BAD_PAGE and skips it.  Two
- * tokens with one slot leave either row.  queries (optional)
+ * tokens with one slot leave either row.  kv and queries overlap neither the
+ * cache nor queries_out.  queries (optional)
  * [tokens, heads, rope_dim]: turned likewise into queries_out (contiguous). */
 int glm53_latent_cache_write(const void* kv, int64_t tokens, int64_t kv_stride, int64_t latent_dim, int64_t rope_dim,
                              int dtype, const void* norm_weight, float eps, const int32_t* positions,
@@ -765,7 +766,8 @@ int glm53_latent_cache_write(const void* kv, int64_t tokens, int64_t kv_stride, 
  * request's tokens sees all seq_lens rows, each earlier one a row less.  A
  * token that sees no row gives 0 and lse -inf.  Tokens behind
  * query_starts[requests] are zeroed when fill_tail is set, else left as they
- * were.  A page id outside the cache sets GLM53_STATUS_BAD_PAGE, a length
+ * were.  out overlaps no input.  The workspace (256-byte aligned, contents of no
+ * account) belongs to one call at a time.  A page id outside the cache sets GLM53_STATUS_BAD_PAGE, a length
  * outside the table GLM53_STATUS_BAD_GEOMETRY. */
 size_t glm53_latent_absorbed_workspace_bytes(int64_t tokens, int64_t heads, int64_t latent_dim);
 int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, int64_t ql_stride_h, const void* q_rope,

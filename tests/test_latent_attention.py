@@ -455,6 +455,8 @@ ABSORBED = [
     ([9000], [1], 64, 512, 64, 64, False),
     ([2500] * 3 + [1, 0, 70], [1] * 6, 32, 512, 0, 16, False),
     (list(range(0, 400)), [1] * 400, 8, 128, 64, 16, False),
+    ([300, 20, 90], [300, 1, 70], 4, 128, 64, 32, False),   # a prompt's worth of tokens in one request
+    ([50, 700], [80, 65], 70, 128, 0, 16, True),            # more tokens than rows; two groups of heads
 ]
 
 
@@ -510,6 +512,19 @@ def test_absorbed_padded_batch_keeps_or_zeroes_the_rest():
     got = G.latent_attention_absorbed(pad(ql), pad(qr), cache, table, n, scale=0.05, query_starts=starts, out=given)
     assert got is given and torch.equal(given[:3], want) and (given[3:] == 7).all()
     G.check_latent_status()
+
+
+@pytest.mark.gpu
+def test_outputs_that_overlap_inputs_are_refused():
+    import glm53_flash_mlx_b200 as G
+
+    ql, qr, cache, table, n, _, _ = make_absorbed([100, 30], [1, 1], 16, 512, 64, 16, torch.bfloat16, 9)
+    with pytest.raises(ValueError, match="overlap"):
+        G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05, out=ql)
+    t = make_expanded([40], [40], 2, 128, 64, 128, torch.bfloat16, 8)
+    with pytest.raises(ValueError, match="overlap"):
+        v = t[4].contiguous()
+        G.latent_attention_expanded(*t[:4], v, *t[5:], scale=0.07, out=v)
 
 
 @pytest.mark.gpu
