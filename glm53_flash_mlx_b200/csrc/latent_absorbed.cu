@@ -68,6 +68,7 @@ constexpr int kSCol = 256;                 // TMEM: O^T at 0..255, two S^T tiles
 struct Args {
   int64_t T;
   int H, R, r, G;  // G groups of 64 heads
+  const uint16_t* cache;
   int64_t pages;
   int page, box;   // rows of a page, rows of a TMA box: gcd(page, 64)
   int half[2];     // chunks of the two halves of a row: whole 128-value groups, the rotary part last
@@ -365,7 +366,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         int y[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) y[k] = __shfl_sync(0xffffffffu, next, k);
-        next = place(t + 1);  // read ahead of the waits below
+        // The next tile is looked up ahead of the waits below, and its rows, one
+        // run of memory a box, go into L2 by then: a freed stage is refilled from
+        // there, and memory is read in order (64 requests of 6,000-8,192 rows:
+        // 119.4 -> 111.7 us; two tiles ahead 115.4, three 122.2; as tensor boxes,
+        // 128 bytes of a row at a time, no gain).
+        next = place(t + 1);
+        if (next >= 0 && next < a.pages * a.page / 8)
+          prefetch_l2(a.cache + (int64_t)next * 8 * (a.R + a.r), a.box * (a.R + a.r) * 2);
         if (lane == 0 && ok) {
           const uint32_t b = n & 1, use = n >> 1;
           for (at_half = 0; at_half < halves; ++at_half) {
@@ -995,6 +1003,7 @@ extern "C" int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, 
   a.R = (int)latent_dim;
   a.r = (int)rope_dim;
   a.G = (int)((heads + unit - 1) / unit);
+  a.cache = (const uint16_t*)cache;
   a.pages = pages;
   a.page = (int)page_size;
   a.box = box;

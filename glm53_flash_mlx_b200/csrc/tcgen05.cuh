@@ -233,6 +233,11 @@ __device__ __forceinline__ void tmem_ld16_frag(uint32_t taddr, uint32_t (&v)[16]
       : "r"(taddr)
       : "memory");
 }
+// Brings `bytes` (a multiple of 16) at a 16-byte aligned address into L2.
+__device__ __forceinline__ void prefetch_l2(const void* at, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(bytes) : "memory");
+}
+
 // True in one lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
