@@ -68,18 +68,15 @@ struct Args {
   uint16_t* out;
   float* lse;
   int fill_tail;
+  int persistent;  // CTAs walk the units; otherwise one a CTA (pair), units in x, heads in y
   uint32_t *status, *status_host;
 };
 
 struct __align__(8) Bars {
-  uint64_t q_full, full[kSlots], empty[kSlots], cut_full[4], s_full[2], p_full[2], o_done[2], drain;
+  uint64_t q_full, q_empty, full[kSlots], empty[kSlots], cut_full[4], s_full[2], p_full[2], o_done[2], drain;
   uint32_t tmem_base;
   int abort_flag;
-  int poison;                       // a masked tile holds values that are not finite
-  int found;                        // this CTA has a query tile
-  int first;                        // its first query row in the request
-  int64_t q0, k0, nq, nk;           // the request's rows
-  int warp_sum[kThreads / 32];
+  int poison[2];  // by unit parity: the unit (from 1) with values that are not finite in a masked tile
 };
 
 // alignment slack, Q, ring, barriers, two floats a row
@@ -109,6 +106,54 @@ __device__ __forceinline__ Bounds bounds_of(const Args& a, int i) {
     b.k0 = b.nk = 0;
   }
   return b;
+}
+
+// One head's queries [first, first + rows of a unit) of a request, and what
+// they see.  A unit is 128 queries, 256 for a pair of CTAs.
+struct Unit {
+  int q0, nq, k0, nk;
+  int first, head;
+
+  // keys that query j of the request sees
+  __device__ __forceinline__ int seen(const Args& a, int j) const {
+    return a.causal ? max(0, (int)min((int64_t)nk, (int64_t)nk - nq + j + 1)) : nk;
+  }
+};
+
+// Query tile `x` over all requests (in order; a request's last tile, which sees
+// the most keys, first); by a converged warp.  False when there are fewer.
+template <int ROWS>
+__device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u, bool report_bad) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int r0 = 0; r0 < a.B; r0 += 32) {
+    Bounds b{};
+    int n = 0;
+    if (r0 + lane < a.B) {
+      b = bounds_of(a, r0 + lane);
+      n = (int)((b.nq + ROWS - 1) / ROWS);
+      if (report_bad && b.bad) report(a.status, a.status_host, kStatusBadGeometry);
+    }
+    int s = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    const int lo = base + s - n;
+    const uint32_t mine = __ballot_sync(0xffffffffu, x >= lo && x < lo + n);
+    if (mine) {
+      const int src = __ffs(mine) - 1;
+      u.q0 = __shfl_sync(0xffffffffu, (int)b.q0, src);
+      u.nq = __shfl_sync(0xffffffffu, (int)b.nq, src);
+      u.k0 = __shfl_sync(0xffffffffu, (int)b.k0, src);
+      u.nk = __shfl_sync(0xffffffffu, (int)b.nk, src);
+      u.first = __shfl_sync(0xffffffffu, (n - 1 - (x - lo)) * ROWS, src);
+      return true;
+    }
+    base += __shfl_sync(0xffffffffu, s, 31);
+  }
+  return false;
 }
 
 // Infinities and NaN: the exponent bits are all ones.
@@ -155,6 +200,28 @@ __device__ __forceinline__ bool clean_row(uint8_t* chunk, int row, int valid) {
   return true;
 }
 
+// Lane 4 k + e of a quad holds p[i]; afterwards p[i] is what lane 4 k + i held
+// in p[e].
+__device__ __forceinline__ uint4 shfl_xor4(uint4 v, int mask) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, mask), __shfl_xor_sync(0xffffffffu, v.y, mask),
+                    __shfl_xor_sync(0xffffffffu, v.z, mask), __shfl_xor_sync(0xffffffffu, v.w, mask));
+}
+__device__ __forceinline__ void quad_transpose(uint4 (&p)[4], int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const uint4 got = shfl_xor4(odd ? p[i] : p[i + 1], 1);
+    p[i] = odd ? got : p[i];
+    p[i + 1] = odd ? p[i + 1] : got;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint4 got = shfl_xor4(high ? p[i] : p[i + 2], 2);
+    p[i] = high ? got : p[i];
+    p[i + 2] = high ? p[i + 2] : got;
+  }
+}
+
 template <typename E, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     expanded_kernel(const __grid_constant__ CUtensorMap qn_map, const __grid_constant__ CUtensorMap qr_map,
@@ -166,17 +233,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* ring = smem + 4 * kChunkBytes;
   Bars* bars = reinterpret_cast<Bars*>(ring + kSlots * kSlotBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int head = blockIdx.y;
   constexpr int kCtas = PAIR ? 2 : 1, kUnit = kCtas * kTile;  // queries a CTA or pair takes
   const int rank = PAIR ? (int)cluster_rank() : 0;
-  const int unit = (int)blockIdx.x / kCtas;
   auto bar = [&](uint64_t* p) { return smem_addr(p); };
 
   if (tid == 0) {
-    bars->found = 0;
     bars->abort_flag = 0;
-    bars->poison = 0;
+    bars->poison[0] = bars->poison[1] = 0;
     mbar_init(bar(&bars->q_full), 1);
+    mbar_init(bar(&bars->q_empty), 1);
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(bar(&bars->full[s]), 1);
       mbar_init(bar(&bars->empty[s]), 1);
@@ -202,96 +267,48 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncwarp();
 
-  // which request and query tile: count tiles over the requests, a block's
-  // worth at a time
-  int base = 0;
-  for (int r0 = 0; r0 < a.B; r0 += kThreads) {
-    int n = 0;
-    Bounds b{};
-    if (r0 + tid < a.B) {
-      b = bounds_of(a, r0 + tid);
-      n = (int)((b.nq + kUnit - 1) / kUnit);
-      if (b.bad && blockIdx.x == 0 && head == 0) report(a.status, a.status_host, kStatusBadGeometry);
+  // The CTA's units in order, by a converged warp: every role walks them itself.
+  // Walking CTAs take all heads of one query tile before the next tile, so that
+  // a round of the grid holds units of like length.
+  auto next_unit = [&](int i, Unit& u) {
+    const bool scan = warp == 0 && blockIdx.y == 0 && i == 0;
+    if (a.persistent) {
+      const int64_t at = blockIdx.x + (int64_t)i * gridDim.x;
+      const int64_t x = at / a.H;
+      u.head = (int)(at - x * a.H);
+      return x < INT32_MAX && find_tile<kUnit>(a, (int)x, u, scan);
     }
-    int s = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += x;
-    }
-    if (lane == 31) bars->warp_sum[warp] = s;
-    __syncthreads();
-    int before = base;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += bars->warp_sum[w];
-      base += bars->warp_sum[w];
-    }
-    const int lo = before + s - n;
-    if (unit >= lo && unit < lo + n) {
-      bars->found = 1;
-      // the later query tiles see more keys: they go first
-      bars->first = (n - 1 - (unit - lo)) * kUnit;
-      bars->q0 = b.q0;
-      bars->nq = b.nq;
-      bars->k0 = b.k0;
-      bars->nk = b.nk;
-    }
-    if (base > unit) break;
-    __syncthreads();
-  }
+    u.head = blockIdx.y;
+    return i == 0 && find_tile<kUnit>(a, blockIdx.x / kCtas, u, scan);
+  };
   tmem_fence_before();
   __syncthreads();
   if constexpr (PAIR) cluster_sync();  // the other CTA's barriers are set up
   tmem_fence_after();
-  if (!bars->found) {
-    if (warp == 9) tmem_free_all<PAIR>(bars->tmem_base);
-    // surplus CTAs zero the rows outside every request
-    if (a.fill_tail) {
-      int64_t lo = a.B ? a.q_starts[a.B] : 0, hi = a.B ? a.q_starts[0] : 0;
-      lo = lo < 0 ? 0 : lo;
-      hi = hi < 0 ? 0 : (hi > a.Tq ? a.Tq : hi);
-      const int64_t rows = hi + (a.Tq > lo ? a.Tq - lo : 0);
-      const int pieces = a.dv >> 3;
-      const int64_t step = (int64_t)(gridDim.x - base * kCtas) * kThreads;
-      for (int64_t i = (int64_t)(blockIdx.x - base * kCtas) * kThreads + tid; i < rows * pieces; i += step) {
-        const int64_t k = i / pieces, row = k < hi ? k : lo + (k - hi);
-        const int64_t at = row * a.H + head;
-        reinterpret_cast<uint4*>(a.out + at * a.dv)[i - k * pieces] = make_uint4(0, 0, 0, 0);
-        if (a.lse && i == k * pieces) a.lse[at] = -INFINITY;
-      }
-    }
-    if constexpr (PAIR) cluster_sync();
-    return;
-  }
-  const Bounds bd{bars->q0, bars->nq, bars->k0, bars->nk, false};
-  const int first = bars->first, j0 = first + rank * kTile;
-  const int rows = (int)max((int64_t)0, min(bd.nq - j0, (int64_t)kTile));  // of this CTA
-  const int nk = (int)bd.nk;
-  // keys that query j of the request sees
-  auto seen = [&](int64_t j) {
-    return a.causal ? (int)max((int64_t)0, min(bd.nk, bd.nk - bd.nq + j + 1)) : nk;
-  };
-  const int vis0 = seen(j0);       // of this CTA's first row
-  const int unit_vis0 = seen(first);  // of the unit's first row
-  const int cut0 = unit_vis0 / kTile;  // first tile that the mask cuts for some row of the unit
-  const int tiles = (seen(min(bd.nq, (int64_t)first + kUnit) - 1) + kTile - 1) / kTile;
+
   // A pair holds half the keys of a K tile (64 rows, four chunks a slot) and
   // half the values of a V tile in each CTA.
   constexpr int kKeyRows = kTile / kCtas, kKeyChunk = kKeyRows * 128, kKeyChunks = kSlotBytes / kKeyChunk;
   const int nch = (a.dn + a.dr) / 64, kslots = (nch + kKeyChunks - 1) / kKeyChunks;
   const int vch = a.dv / 64 / kCtas, vslots = (vch + 1) / 2;
-  const int64_t q0 = bd.q0 + j0, k0 = bd.k0;
+  // key tiles of a unit, and the first of them that the mask cuts for some row
+  auto tiles_of = [&](const Unit& u) {
+    return (u.seen(a, (int)min((int64_t)u.nq, (int64_t)u.first + kUnit) - 1) + kTile - 1) / kTile;
+  };
+  auto cut_of = [&](const Unit& u) { return u.seen(a, u.first) / kTile; };
 
   constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's
   volatile int* abort_flag = &bars->abort_flag;
 
-  auto p_arrive = [&](int t) {
+  auto p_arrive = [&](uint32_t g) {
     if constexpr (PAIR)
-      mbar_arrive_at_relaxed(bar(&bars->p_full[t & 1]), 0);
+      mbar_arrive_at_relaxed(bar(&bars->p_full[g & 1]), 0);
     else
-      mbar_arrive(bar(&bars->p_full[t & 1]));
+      mbar_arrive(bar(&bars->p_full[g & 1]));
   };
+  // Running over all units: g key tiles, seq ring slots, cut tiles that the mask
+  // cuts.  Tile g's S, P and product use the barriers g & 1, phase (g >> 1) & 1.
+  uint32_t g = 0;
 
   if (warp == 8) {
     // ---------------- TMA ----------------
@@ -300,97 +317,114 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (and cleans) them; the product learns of them through p_full.  A pair's ring
     // can hold three such tiles before the first has landed (one slot a tile, no
     // K behind the last), and a barrier takes one tile at a time: four barriers.
-    if (lane == 0 && tiles > 0) {
-      auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int z, uint64_t* p) {
-        if constexpr (PAIR)
-          tma_load_3d_at(dst, map, x, head, z, bar(p), 0);
-        else
-          tma_load_3d(dst, map, x, head, z, bar(p));
-      };
-      if (rank == 0) mbar_expect_tx(bar(&bars->q_full), kCtas * nch * kChunkBytes);
-      for (int c = 0; c < nch; ++c) {
-        const bool rope = c * 64 >= a.dn;
-        load(smem_addr(q_smem + c * kChunkBytes), rope ? &qr_map : &qn_map, rope ? 0 : c * 64, (int)q0, &bars->q_full);
-      }
-      uint32_t seq = 0;
-      int cut = 0;  // value tiles that the mask cuts, so far
-      bool ok = true;
-      auto slot = [&](bool value, int tile, int part) {
-        const uint32_t s = seq % kSlots;
-        if (seq >= kSlots) ok = mbar_wait_fast(bar(&bars->empty[s]), (seq / kSlots - 1) & 1u, abort_flag);
-        if (!ok) return;
-        const int per = value ? 2 : kKeyChunks, bytes = value ? kChunkBytes : kKeyChunk;
-        const int n = min(per, (value ? vch : nch) - per * part);
-        const bool masked = value && tile >= cut0;
-        uint64_t* local = &bars->cut_full[(tile - cut0) & 3];
-        if (masked) {
-          if (part == 0) {
-            mbar_expect_tx(bar(local), vch * kChunkBytes);
-            ++cut;
-          }
-          if (rank == 0) mbar_arrive(bar(&bars->full[s]));
-        } else if (rank == 0) {
-          mbar_expect_tx(bar(&bars->full[s]), kCtas * n * bytes);
-        }
-        for (int c = 0; c < n; ++c) {
-          const uint32_t dst = smem_addr(ring + s * kSlotBytes + c * bytes);
-          const int x = (per * part + c) * 64, z = (int)(k0 + (int64_t)tile * kTile);
-          if (masked)
-            tma_load_3d(dst, &v_map, rank * vch * 64 + x, head, z, bar(local));
-          else if (value)
-            load(dst, &v_map, rank * vch * 64 + x, z, &bars->full[s]);
-          else if (x < a.dn)
-            load(dst, &kn_map, x, z + rank * kKeyRows, &bars->full[s]);
-          else if constexpr (PAIR)
-            tma_load_2d_at(dst, &kr_map, 0, z + rank * kKeyRows, bar(&bars->full[s]), 0);
+    uint32_t seq = 0, queries = 0;
+    int cut = 0;
+    bool ok = true;
+    Unit u;
+    for (int i = 0; next_unit(i, u); ++i) {
+      const int tiles = tiles_of(u), cut0 = cut_of(u);
+      if (lane == 0 && tiles > 0 && ok) {
+        auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int z, uint64_t* p) {
+          if constexpr (PAIR)
+            tma_load_3d_at(dst, map, x, u.head, z, bar(p), 0);
           else
-            tma_load_2d(dst, &kr_map, 0, z, bar(&bars->full[s]));
+            tma_load_3d(dst, map, x, u.head, z, bar(p));
+        };
+        if (queries) ok = mbar_wait_fast(bar(&bars->q_empty), (queries - 1) & 1u, abort_flag);
+        if (ok) {
+          ++queries;
+          if (rank == 0) mbar_expect_tx(bar(&bars->q_full), kCtas * nch * kChunkBytes);
+          for (int c = 0; c < nch; ++c) {
+            const bool rope = c * 64 >= a.dn;
+            load(smem_addr(q_smem + c * kChunkBytes), rope ? &qr_map : &qn_map, rope ? 0 : c * 64,
+                 u.q0 + u.first + rank * kTile, &bars->q_full);
+          }
         }
-        ++seq;
-      };
-      for (int t = 0; t <= tiles && ok; ++t) {
-        for (int p = 0; p < kslots && ok && t < tiles; ++p) slot(false, t, p);
-        for (int p = 0; p < vslots && ok && t > 0; ++p) slot(true, t - 1, p);
+        auto slot = [&](bool value, int tile, int part) {
+          const uint32_t s = seq % kSlots;
+          if (seq >= kSlots) ok = mbar_wait_fast(bar(&bars->empty[s]), (seq / kSlots - 1) & 1u, abort_flag);
+          if (!ok) return;
+          const int per = value ? 2 : kKeyChunks, bytes = value ? kChunkBytes : kKeyChunk;
+          const int n = min(per, (value ? vch : nch) - per * part);
+          const bool masked = value && tile >= cut0;
+          if (masked && part == 0) ++cut;
+          uint64_t* local = &bars->cut_full[(cut - 1) & 3];
+          if (masked) {
+            if (part == 0) mbar_expect_tx(bar(local), vch * kChunkBytes);
+            if (rank == 0) mbar_arrive(bar(&bars->full[s]));
+          } else if (rank == 0) {
+            mbar_expect_tx(bar(&bars->full[s]), kCtas * n * bytes);
+          }
+          for (int c = 0; c < n; ++c) {
+            const uint32_t dst = smem_addr(ring + s * kSlotBytes + c * bytes);
+            const int x = (per * part + c) * 64, z = u.k0 + tile * kTile;
+            if (masked)
+              tma_load_3d(dst, &v_map, rank * vch * 64 + x, u.head, z, bar(local));
+            else if (value)
+              load(dst, &v_map, rank * vch * 64 + x, z, &bars->full[s]);
+            else if (x < a.dn)
+              load(dst, &kn_map, x, z + rank * kKeyRows, &bars->full[s]);
+            else if constexpr (PAIR)
+              tma_load_2d_at(dst, &kr_map, 0, z + rank * kKeyRows, bar(&bars->full[s]), 0);
+            else
+              tma_load_2d(dst, &kr_map, 0, z, bar(&bars->full[s]));
+          }
+          ++seq;
+        };
+        for (int t = 0; t <= tiles && ok; ++t) {
+          for (int p = 0; p < kslots && ok && t < tiles; ++p) slot(false, t, p);
+          for (int p = 0; p < vslots && ok && t > 0; ++p) slot(true, t - 1, p);
+        }
       }
-      if (!ok) {
-        // copies still in flight write this CTA's (this pair's) shared memory:
-        // wait for them; a pair leaves together
-        volatile int never = 0;
-        for (uint32_t k = seq > kSlots ? seq - kSlots : 0; k < seq && rank == 0; ++k)
-          mbar_wait(bar(&bars->full[k % kSlots]), (k / kSlots) & 1u, &never);
+      __syncwarp();
+    }
+    if (!ok) {
+      // copies still in flight write this CTA's (this pair's) shared memory: wait
+      // for them; a pair leaves together
+      volatile int never = 0;
+      for (uint32_t k = seq > kSlots ? seq - kSlots : 0; k < seq && rank == 0; ++k) {
         never = 0;
-        if (rank == 0) mbar_wait(bar(&bars->q_full), 0, &never);
+        mbar_wait(bar(&bars->full[k % kSlots]), (k / kSlots) & 1u, &never);
+      }
+      never = 0;
+      if (rank == 0 && queries) mbar_wait(bar(&bars->q_full), (queries - 1) & 1u, &never);
+      for (int k = max(0, cut - 4); k < cut; ++k) {
         never = 0;
-        for (int k = max(0, cut - 4); k < cut; ++k) mbar_wait(bar(&bars->cut_full[k & 3]), (k >> 2) & 1u, &never);
+        mbar_wait(bar(&bars->cut_full[k & 3]), (k >> 2) & 1u, &never);
       }
     }
+    __syncwarp();
   } else if (warp == 9) {
     // ---------------- MMA ----------------
     // All lanes walk the loops, so that descriptors stay in uniform registers;
     // one elected lane waits and issues the unrolled MMAs of a slot.
-    if (tiles > 0 && rank == 0) {
-      constexpr bool bf16 = std::is_same<E, __nv_bfloat16>::value;
-      constexpr uint32_t id_s = make_idesc_f16(kUnit, kTile, bf16, false, false);
-      const bool leader = elect_one();
-      uint32_t seq = 0;
-      bool ok = true;
-      const uint64_t qd = make_sw128_desc(smem_addr(q_smem));
-      const uint64_t kd0 = make_sw128_desc(smem_addr(ring)), vd0 = make_sw128_mn_desc(smem_addr(ring), kChunkBytes);
-      auto commit = [&](uint64_t* p) {
-        if constexpr (PAIR)
-          mma_commit2(bar(p));
-        else
-          mma_commit(bar(p));
-      };
-      auto landed = [&](uint32_t s, uint32_t phase) {
-        ok = ok && mbar_wait_fast(bar(&bars->full[s]), phase, abort_flag);
-        tmem_fence_after();
-        return ok;
-      };
-      if (leader) ok = mbar_wait_fast(bar(&bars->q_full), 0, abort_flag);
+    constexpr bool bf16 = std::is_same<E, __nv_bfloat16>::value;
+    constexpr uint32_t id_s = make_idesc_f16(kUnit, kTile, bf16, false, false);
+    const bool leader = elect_one() && rank == 0;
+    uint32_t seq = 0, queries = 0;
+    bool ok = true;
+    const uint64_t qd = make_sw128_desc(smem_addr(q_smem));
+    const uint64_t kd0 = make_sw128_desc(smem_addr(ring)), vd0 = make_sw128_mn_desc(smem_addr(ring), kChunkBytes);
+    auto commit = [&](uint64_t* p) {
+      if constexpr (PAIR)
+        mma_commit2(bar(p));
+      else
+        mma_commit(bar(p));
+    };
+    auto landed = [&](uint32_t s, uint32_t phase) {
+      ok = ok && mbar_wait_fast(bar(&bars->full[s]), phase, abort_flag);
+      tmem_fence_after();
+      return ok;
+    };
+    Unit u;
+    for (int i = 0; next_unit(i, u); ++i) {
+      const int tiles = tiles_of(u);
+      if (tiles == 0) continue;
+      if (leader) ok = ok && mbar_wait_fast(bar(&bars->q_full), queries & 1u, abort_flag);
+      ++queries;
       for (int t = 0; t <= tiles; ++t) {
         if (t < tiles) {
-          const uint32_t d = kSCol + (t & 1) * kTile;
+          const uint32_t d = kSCol + ((g + t) & 1) * kTile;
           for (int p = 0; p < kslots; ++p, ++seq) {
             const uint32_t s = seq % kSlots, phase = (seq / kSlots) & 1u;
             const uint64_t ad = qd + (uint64_t)(p * (kKeyChunks * kChunkBytes >> 4));
@@ -413,17 +447,21 @@ __global__ void __launch_bounds__(kThreads, 1)
               commit(&bars->empty[s]);
             }
           }
-          if (leader && ok) commit(&bars->s_full[t & 1]);
+          if (leader && ok) {
+            commit(&bars->s_full[(g + t) & 1]);
+            if (t + 1 == tiles) commit(&bars->q_empty);
+          }
         }
         if (t > 0) {
-          const int u = t - 1;
-          const uint32_t pa = kSCol + (u & 1) * kTile;
-          const int steps = (min(kTile, nk - u * kTile) + 15) >> 4;
+          const uint32_t v = g + t - 1;  // the tile whose values are multiplied
+          const uint32_t pa = kSCol + (v & 1) * kTile;
+          const int steps = (min(kTile, u.nk - (t - 1) * kTile) + 15) >> 4;
+          const bool more = t > 1;  // adds to what is there
           if (leader) {
             if constexpr (PAIR)
-              ok = ok && mbar_wait_peer(bar(&bars->p_full[u & 1]), (u >> 1) & 1u, abort_flag);
+              ok = ok && mbar_wait_peer(bar(&bars->p_full[v & 1]), (v >> 1) & 1u, abort_flag);
             else
-              ok = ok && mbar_wait_fast(bar(&bars->p_full[u & 1]), (u >> 1) & 1u, abort_flag);
+              ok = ok && mbar_wait_fast(bar(&bars->p_full[v & 1]), (v >> 1) & 1u, abort_flag);
           }
           for (int p = 0; p < vslots; ++p, ++seq) {
             const uint32_t s = seq % kSlots, phase = (seq / kSlots) & 1u;
@@ -436,9 +474,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (leader && landed(s, phase)) {
               auto step = [&](int k) {
                 if constexpr (PAIR)
-                  mma_f16_ts2(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
+                  mma_f16_ts2(o, pa + 8 * k, vd + 128 * k, id_o, more || k);
                 else
-                  mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, (u | k) != 0);
+                  mma_f16_ts(o, pa + 8 * k, vd + 128 * k, id_o, more || k);
               };
               if (steps == 8) {
 #pragma unroll
@@ -449,52 +487,65 @@ __global__ void __launch_bounds__(kThreads, 1)
               commit(&bars->empty[s]);
             }
           }
-          if (leader && ok) commit(&bars->o_done[u & 1]);
+          if (leader && ok) commit(&bars->o_done[v & 1]);
         }
       }
-      // no MMA is in flight when TMEM is freed.  The lane that issued waits
-      // alone: a lane that spins must not keep its warp from one with work.
-      if (leader) {
-        volatile int never = 0;
-        commit(&bars->drain);
-        if (!mbar_wait(bar(&bars->drain), 0, &never)) *abort_flag = 1;
-      }
+      g += tiles;
+    }
+    __syncwarp();
+    // no MMA is in flight when TMEM is freed.  The lane that issued waits alone:
+    // a lane that spins must not keep its warp from one with work.
+    if (leader) {
+      volatile int never = 0;
+      commit(&bars->drain);
+      if (!mbar_wait(bar(&bars->drain), 0, &never)) *abort_flag = 1;
     }
     __syncwarp();
   } else if (warp >= 10) {
     // ---------------- values of the tiles that the mask cuts ----------------
     bool ok = true;
-    for (int t = 0; t < tiles; ++t) {
-      ok = ok && __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->s_full[t & 1]), (t >> 1) & 1u, abort_flag));
-      if (t >= cut0 && ok) {
-        // its values lie in the ring where the producer put them
-        const uint32_t s0 = kslots + t * (kslots + vslots) + (t + 1 < tiles ? kslots : 0);
-        ok = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->cut_full[(t - cut0) & 3]), ((t - cut0) >> 2) & 1u,
-                                                    abort_flag));
-        const int valid = min(kTile, nk - t * kTile), end = (valid + 15) & ~15;  // the product stops at `end`
-        bool found = false;
-        for (int c = 0; c < vch && ok; ++c) {
-          const uint32_t s = (s0 + (c >> 1)) % kSlots;
-          for (int row = tid - 320; row < end && ok; row += 64)
-            found |= clean_row<E>(ring + s * kSlotBytes + (c & 1) * kChunkBytes, row, valid);
+    uint32_t seq = 0;
+    int cut = 0, units = 0;
+    Unit u;
+    for (int i = 0; next_unit(i, u); ++i) {
+      const int tiles = tiles_of(u), cut0 = cut_of(u);
+      if (tiles == 0) continue;
+      ++units;
+      for (int t = 0; t < tiles; ++t) {
+        const uint32_t v = g + t;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->s_full[v & 1]), (v >> 1) & 1u, abort_flag));
+        if (t >= cut0 && ok) {
+          // its values lie in the ring where the producer put them
+          const uint32_t s0 = seq + kslots + t * (kslots + vslots) + (t + 1 < tiles ? kslots : 0);
+          ok = __all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->cut_full[cut & 3]), (cut >> 2) & 1u, abort_flag));
+          ++cut;
+          const int valid = min(kTile, u.nk - t * kTile), end = (valid + 15) & ~15;  // the product stops at `end`
+          bool found = false;
+          for (int c = 0; c < vch && ok; ++c) {
+            const uint32_t s = (s0 + (c >> 1)) % kSlots;
+            for (int row = tid - 320; row < end && ok; row += 64)
+              found |= clean_row<E>(ring + s * kSlotBytes + (c & 1) * kChunkBytes, row, valid);
+          }
+          if (found) {
+            bars->poison[units & 1] = units;
+            // the other CTA's rows meet these values too
+            if constexpr (PAIR) store_at(smem_addr(&bars->poison[units & 1]), rank ^ 1, units);
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (PAIR)
+              mbar_arrive_at(bar(&bars->p_full[v & 1]), 0);
+            else
+              p_arrive(v);
+          }
+        } else if (lane == 0) {
+          p_arrive(v);
         }
-        if (found) {
-          bars->poison = 1;
-          // the other CTA's rows meet these values too
-          if constexpr (PAIR) store_at(smem_addr(&bars->poison), rank ^ 1, 1);
-        }
-        fence_async_shared();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR)
-            mbar_arrive_at(bar(&bars->p_full[t & 1]), 0);
-          else
-            p_arrive(t);
-        }
-      } else if (lane == 0) {
-        p_arrive(t);
       }
-      __syncwarp();
+      g += tiles;
+      seq += tiles * (kslots + vslots);
     }
   } else {
     // ---------------- softmax, epilogue ----------------
@@ -503,14 +554,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3, half = warp >> 2;
     const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const int vis = r < rows ? seen(j0 + r) : 0;
     const int ocols = a.dv >> 1, o0 = half * ocols;  // this thread's result columns
-    float m = -INFINITY, l = 0.f;
-    bool stop = false;
     float* xchg = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 1024);  // [2][128]
+    bool stop = false;
+    int units = 0;
+    Unit u;
+    for (int i = 0; !stop && next_unit(i, u); ++i) {
+    const int tiles = tiles_of(u), j0 = u.first + rank * kTile;
+    const int vis = j0 + r < u.nq ? u.seen(a, j0 + r) : 0, vis0 = u.seen(a, j0);
+    float m = -INFINITY, l = 0.f;
+    if (tiles > 0) ++units;
     for (int t = 0; t < tiles; ++t) {
-      const int b = t & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->s_full[b]), (t >> 1) & 1u, abort_flag))) {
+      const uint32_t v_ = g + t, b = v_ & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->s_full[b]), (v_ >> 1) & 1u, abort_flag))) {
         stop = true;
       }
       float v[64];
@@ -554,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l *= f;
         if (t > 0) {
           // (a warp whose wait gives up goes on: all stop at the next tile)
-          if (__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(t - 1) & 1]), ((t - 1) >> 1) & 1u, abort_flag))) {
+          if (__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(v_ - 1) & 1]), ((v_ - 1) >> 1) & 1u, abort_flag))) {
             tmem_fence_after();
             for (int o = 0; o < ocols; o += 32) {
               uint32_t w[32];
@@ -580,25 +636,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_st();
       tmem_fence_before();
       __syncwarp();
-      if (lane == 0) p_arrive(t);
+      if (lane == 0) p_arrive(v_);
       __syncwarp();
     }
+    g += tiles;
     if (!stop && tiles > 0)
-      stop = !__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(tiles - 1) & 1]), ((tiles - 1) >> 1) & 1u, abort_flag));
+      stop = !__all_sync(0xffffffffu, mbar_wait_fast(bar(&bars->o_done[(g - 1) & 1]), ((g - 1) >> 1) & 1u, abort_flag));
     stop = any_of(stop, 1, kSoftThreads);
     if (!stop) {
       tmem_fence_after();
       xchg[half * kTile + r] = l;
       bar_sync(1, kSoftThreads);
       l = xchg[r] + xchg[kTile + r];
-      const bool poison = bars->poison != 0;
+      const bool poison = tiles > 0 && bars->poison[units & 1] == units;
       const float inv = 1.f / l;
-      const int64_t at = (q0 + r) * a.H + head;
-      if (r < rows && a.lse && half == 0)
+      const bool mine = j0 + r < u.nq;
+      const int64_t at = (int64_t)(u.q0 + j0 + r) * a.H + u.head;
+      if (mine && a.lse && half == 0)
         a.lse[at] = vis > 0 ? ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2 : -INFINITY;
-      // 16-bit rows into the Q buffer (every S is done), pieces of 16 bytes
-      // swizzled by row, then whole rows to memory
-      const int row_bytes = a.dv * 2;
       for (int o = 0; o < ocols; o += 32) {
         uint32_t w[32];
         if (tiles > 0) {
@@ -609,33 +664,47 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = vis > 0 ? __uint_as_float(w[i]) * inv : 0.f;
         if (poison) {
-          for (int k = cut0 * kTile; k < vis; ++k) {
-            const uint16_t* src = a.v + (k0 + k) * a.v_t + head * a.v_h + o0 + o;
+          for (int k = cut_of(u) * kTile; k < vis; ++k) {
+            const uint16_t* src = a.v + (int64_t)(u.k0 + k) * a.v_t + u.head * a.v_h + o0 + o;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (not_finite<E>(src[i])) f[i] += Elem<E>::to_float(src[i]);
           }
         }
+        // four lanes exchange their rows' four pieces, so that a store of the quad
+        // is 64 bytes of one row
+        uint4 p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(q_smem + r * row_bytes + 16 * (((o0 + o) / 8 + i) ^ (r & 7))) =
-              make_uint4(Elem<E>::pack(f[8 * i], f[8 * i + 1]), Elem<E>::pack(f[8 * i + 2], f[8 * i + 3]),
-                         Elem<E>::pack(f[8 * i + 4], f[8 * i + 5]), Elem<E>::pack(f[8 * i + 6], f[8 * i + 7]));
-      }
-      bar_sync(1, kSoftThreads);
-      const int pieces = a.dv >> 3;
-      uint4* out = reinterpret_cast<uint4*>(a.out + (q0 * a.H + head) * a.dv);
-      if (lane < pieces) {
-#pragma unroll 4
-        for (int row = warp; row < rows; row += kSoftWarps)
-          out[(int64_t)row * a.H * pieces + lane] =
-              *reinterpret_cast<const uint4*>(q_smem + row * row_bytes + 16 * (lane ^ (row & 7)));
+          p[i] = make_uint4(Elem<E>::pack(f[8 * i], f[8 * i + 1]), Elem<E>::pack(f[8 * i + 2], f[8 * i + 3]),
+                            Elem<E>::pack(f[8 * i + 4], f[8 * i + 5]), Elem<E>::pack(f[8 * i + 6], f[8 * i + 7]));
+        quad_transpose(p, lane);
+        const int row = r & ~3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j0 + row + i < u.nq)
+            *reinterpret_cast<uint4*>(a.out + ((int64_t)(u.q0 + j0 + row + i) * a.H + u.head) * a.dv + o0 + o +
+                                      8 * (lane & 3)) = p[i];
       }
     }
     tmem_fence_before();
+    }
   }
   __syncthreads();
   if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other may reach its memory
+  if (a.fill_tail) {
+    // rows outside every request, by all CTAs
+    const int64_t lo = a.B ? max(0, a.q_starts[a.B]) : 0, hi = a.B ? min(a.Tq, (int64_t)max(0, a.q_starts[0])) : 0;
+    const int64_t rows = hi + max((int64_t)0, a.Tq - lo);
+    const int pieces = a.dv >> 3;
+    const int64_t step = (int64_t)gridDim.x * gridDim.y * kThreads;
+    for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + tid; i < rows * a.H * pieces; i += step) {
+      const int64_t k = i / (a.H * pieces), rest = i - k * a.H * pieces;
+      const int64_t row = k < hi ? k : lo + (k - hi), at = row * a.H + rest / pieces;
+      reinterpret_cast<uint4*>(a.out + at * a.dv)[rest % pieces] = make_uint4(0, 0, 0, 0);
+      if (a.lse && rest % pieces == 0) a.lse[at] = -INFINITY;
+    }
+  }
   if (tid == 0 && bars->abort_flag) report(a.status, a.status_host, kStatusWaitTimeout);
   if (warp == 9) {
     tmem_fence_after();
@@ -698,11 +767,17 @@ int launch(const CUtensorMap& qn, const CUtensorMap& qr, const CUtensorMap& kn, 
   const auto kernel = expanded_kernel<E, PAIR>;
   const int rc = ensure_max_smem((const void*)kernel, kSmemBytes);
   if (rc) return rc;
-  // a unit more a request than whole units in all: where rows lie outside every
-  // request, at least one unit a head has no queries and zeroes them
+  // Units at most: one more a request than whole units in all.
   constexpr int kCtas = PAIR ? 2 : 1, kUnit = kCtas * kTile;
+  const int64_t units = (a.Tq + kUnit - 1) / kUnit + a.B;
+  Args b = a;
+  // A CTA an SM walks the units (the next one's queries and keys load, and its
+  // first scores form, under the results of the last) where the search for a
+  // unit, 32 requests a step, is short; pairs and larger batches take one each.
+  b.persistent = !PAIR && a.B <= 256;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(((a.Tq + kUnit - 1) / kUnit + a.B) * kCtas), (unsigned)a.H);
+  cfg.gridDim = b.persistent ? dim3((unsigned)std::min<int64_t>(sm_count(), units * a.H))
+                             : dim3((unsigned)(units * kCtas), (unsigned)a.H);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = st;
@@ -713,7 +788,7 @@ int launch(const CUtensorMap& qn, const CUtensorMap& qr, const CUtensorMap& kn, 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = PAIR ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kernel, qn, qr, kn, kr, v, a);
+  cudaLaunchKernelEx(&cfg, kernel, qn, qr, kn, kr, v, b);
   return check_launch("expanded_kernel");
 }
 
@@ -790,7 +865,7 @@ extern "C" int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, in
   // a masked score is -inf, which a factor of 0 would turn into NaN
   const float c = std::max(std::fabs(scale) * kLog2e, 1e-37f);
   Args a{Tq, Tk, (int)heads, (int)nope_dim, (int)rope_dim, (int)value_dim, query_starts, key_starts, (int)requests,
-         c, scale < 0, causal, (const uint16_t*)values, v_stride_t, v_stride_h, (uint16_t*)out, lse, fill_tail,
+         c, scale < 0, causal, (const uint16_t*)values, v_stride_t, v_stride_h, (uint16_t*)out, lse, fill_tail, 0,
          status, status_host};
   const cudaStream_t st = (cudaStream_t)stream;
   if (pair)
