@@ -19,10 +19,19 @@
 // 64 KB, and one ring of five 32 KB slots that K and V halves (128 keys x 128
 // values) share in the order the MMAs take them.
 //
+// One CTA alone moves 128 KB into shared memory a tile and its MMAs read
+// 192 KB there: 2,560 cycles at 128 bytes each, more than the MMAs need.  For
+// long requests two CTAs work as a pair (cta_group::2, M = 256): each holds its
+// 128 queries, half the keys of a K tile and half the values of a V tile, and
+// rank 0 issues for both (2,048 queries over 8,192 keys, 64 heads of 256 + 256:
+// 856 us alone, 715 as pairs, 1,345 TFLOP/s).  For short ones a CTA an SM walks
+// the units instead, so that the set-up of one runs under the results of the
+// last.  Both rules are at the launch.
+//
 // Roles: warps 0-7 softmax (two threads a row, 64 keys each) and epilogue,
-// warp 8 TMA, warp 9 MMA, warps 10 and 11 clean values (below).  Every mbarrier wait is bounded; a CTA that gives up
-// sets GLM53_STATUS_WAIT_TIMEOUT, waits for its copies and MMAs, frees its
-// TMEM and exits.
+// warp 8 TMA, warp 9 MMA, warps 10 and 11 clean values (below).  Every mbarrier
+// wait is bounded; a CTA that gives up sets GLM53_STATUS_WAIT_TIMEOUT, waits for
+// its copies and MMAs, frees its TMEM and exits.
 //
 // Masked places must not enter, whatever they hold.  Masked scores are
 // replaced before the maximum.  A masked weight is 0, but 0 x NaN is not, so on
@@ -68,7 +77,7 @@ struct Args {
   uint16_t* out;
   float* lse;
   int fill_tail;
-  int persistent;  // CTAs walk the units; otherwise one a CTA (pair), units in x, heads in y
+  int persistent;  // CTAs walk the units; else one a CTA (pair), units in x, heads in y
   uint32_t *status, *status_host;
 };
 
@@ -771,10 +780,16 @@ int launch(const CUtensorMap& qn, const CUtensorMap& qr, const CUtensorMap& kn, 
   constexpr int kCtas = PAIR ? 2 : 1, kUnit = kCtas * kTile;
   const int64_t units = (a.Tq + kUnit - 1) / kUnit + a.B;
   Args b = a;
-  // A CTA an SM walks the units (the next one's queries and keys load, and its
-  // first scores form, under the results of the last) where the search for a
-  // unit, 32 requests a step, is short; pairs and larger batches take one each.
-  b.persistent = !PAIR && a.B <= 256;
+  // A CTA an SM walks the units: the next one's queries and keys load, and its
+  // first scores form, under the results of the last.  64 heads, walking / one
+  // unit a CTA: 16 x 150 queries and keys of 256 + 256 values 136 / 164 us,
+  // 4 x 512 92 / 111, 1 x 2,048 of 256 + 192 172 / 182.  All heads of a query
+  // tile come before the next tile, so one request's keys and values of all
+  // heads should stay in L2 (126 MB): over 8,192 keys of 256 + 192 values
+  // (402 MB) 947 / 772, of 192 + 64 (201 MB) 615 / 543.  The search for a unit
+  // takes 32 requests a step.  A pair's units are long and stay one each.
+  const double held = 2.0 * a.Tk / a.B * a.H * (a.dn + a.dv);
+  b.persistent = !PAIR && a.B <= 256 && held <= 126e6;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = b.persistent ? dim3((unsigned)std::min<int64_t>(sm_count(), units * a.H))
                              : dim3((unsigned)(units * kCtas), (unsigned)a.H);
@@ -844,11 +859,11 @@ extern "C" int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, in
   const bool bf16 = dtype == GLM53_DTYPE_BF16;
   // Two CTAs take 256 queries as a pair, each reading and holding half of K and
   // V, where requests are long enough to pay for the pair's hand-shakes and for
-  // units of 256 rows.  Measured, one CTA / a pair: 64 heads of 256 + 256 values,
-  // 1,024 queries and keys 77 / 83 us, 2,048 194 / 188, 512 queries over 4,096
-  // keys 140 / 122, 2,048 over 8,192 856 / 719; 16 heads of 192 + 128 values,
-  // 4 x 512 queries over 512 keys 26 / 33, over 2,512 72.5 / 72.3, 512 over
-  // 4,096 51 / 48.
+  // units of 256 rows.  Measured, CTAs alone / pairs: 64 heads of 256 + 256
+  // values, 1,024 queries and keys 72 / 83 us, 2,048 194 / 188, 512 queries over
+  // 4,096 keys 140 / 122, 2,048 over 8,192 856 / 715; 16 heads of 192 + 128
+  // values, 4 x 512 queries over 512 keys 24 / 33, over 2,512 72.5 / 72.3, 512
+  // over 4,096 51 / 48.
   const bool pair = value_dim % 128 == 0 && Tq > requests * kTile && Tk >= requests * 2048;
   const int key_rows = pair ? kTile / 2 : kTile;
   CUtensorMap qn, qr, kn, kr, v;
