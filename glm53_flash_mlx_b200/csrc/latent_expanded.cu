@@ -81,10 +81,23 @@ struct Args {
   uint32_t *status, *status_host;
 };
 
+// One head's queries [first, first + rows of a unit) of a request, and what
+// they see.  A unit is 128 queries, 256 for a pair of CTAs.
+struct Unit {
+  int q0, nq, k0, nk;
+  int first, head;
+
+  // keys that query j of the request sees
+  __device__ __forceinline__ int seen(const Args& a, int j) const {
+    return a.causal ? max(0, (int)min((int64_t)nk, (int64_t)nk - nq + j + 1)) : nk;
+  }
+};
+
 struct __align__(8) Bars {
   uint64_t q_full, q_empty, full[kSlots], empty[kSlots], cut_full[4], s_full[2], p_full[2], o_done[2], drain;
   uint32_t tmem_base;
   int abort_flag;
+  Unit unit;      // the softmax warps' unit
   int poison[2];  // by unit parity: the unit (from 1) with values that are not finite in a masked tile
 };
 
@@ -116,18 +129,6 @@ __device__ __forceinline__ Bounds bounds_of(const Args& a, int i) {
   }
   return b;
 }
-
-// One head's queries [first, first + rows of a unit) of a request, and what
-// they see.  A unit is 128 queries, 256 for a pair of CTAs.
-struct Unit {
-  int q0, nq, k0, nk;
-  int first, head;
-
-  // keys that query j of the request sees
-  __device__ __forceinline__ int seen(const Args& a, int j) const {
-    return a.causal ? max(0, (int)min((int64_t)nk, (int64_t)nk - nq + j + 1)) : nk;
-  }
-};
 
 // Query tile `x` over all requests (in order; a request's last tile, which sees
 // the most keys, first); by a converged warp.  False when there are fewer.
@@ -567,10 +568,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* xchg = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 1024);  // [2][128]
     bool stop = false;
     int units = 0;
-    Unit u;
-    for (int i = 0; !stop && next_unit(i, u); ++i) {
-    const int tiles = tiles_of(u), j0 = u.first + rank * kTile;
-    const int vis = j0 + r < u.nq ? u.seen(a, j0 + r) : 0, vis0 = u.seen(a, j0);
+    for (int i = 0; !stop; ++i) {
+    int tiles, vis, vis0;
+    {
+      Unit u;
+      if (!next_unit(i, u)) break;
+      // kept in shared memory for the epilogue: registers are short in between
+      if (tid == 0) bars->unit = u;
+      const int j0 = u.first + rank * kTile;
+      tiles = tiles_of(u);
+      vis = j0 + r < u.nq ? u.seen(a, j0 + r) : 0;
+      vis0 = u.seen(a, j0);
+    }
     float m = -INFINITY, l = 0.f;
     if (tiles > 0) ++units;
     for (int t = 0; t < tiles; ++t) {
@@ -655,6 +664,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!stop) {
       tmem_fence_after();
       xchg[half * kTile + r] = l;
+      const Unit u = bars->unit;
+      const int j0 = u.first + rank * kTile;
       bar_sync(1, kSoftThreads);
       l = xchg[r] + xchg[kTile + r];
       const bool poison = tiles > 0 && bars->poison[units & 1] == units;
