@@ -749,6 +749,59 @@ def test_two_graphs_and_a_side_stream():
 
 
 @pytest.mark.gpu
+def test_calls_at_once_on_several_streams():
+    """Both attention forms, a store and a plan, eager and as replayed graphs, on streams of their own at the
+    same time: every result is the one that the call gives alone."""
+    import glm53_flash_mlx_b200 as G
+
+    dev = "cuda"
+    a = make_absorbed([3000, 900, 5, 0], [1, 2, 1, 1], 64, 512, 64, 64, torch.bfloat16, 1)
+    b = make_absorbed([700] * 9, [1] * 9, 16, 512, 64, 16, torch.float16, 2)
+    e = make_expanded([300, 150], [300, 700], 8, 192, 64, 256, torch.bfloat16, 3)
+    f = make_expanded([520], [4200], 4, 192, 64, 256, torch.bfloat16, 4)  # CTA pairs
+    kv = torch.randn((40, 576), device=dev).bfloat16()
+    slots = torch.randperm(64, device=dev)[:40]
+    cached, new, table, free = make_plan_case(50, 16, 60, 8)
+
+    def store():
+        cache = torch.zeros((4, 16, 576), dtype=torch.bfloat16, device=dev)
+        G.latent_cache_write(kv, cache, slots)
+        return cache
+
+    def plan():
+        return run_plan(cached, new, table, free, len(free), 16, sum(new))[0].slots
+
+    calls = [lambda: G.latent_attention_absorbed(*a[:5], scale=0.06, query_starts=a[5]),
+             lambda: G.latent_attention_absorbed(*b[:5], scale=0.06),
+             lambda: G.latent_attention_expanded(*e, scale=0.06),
+             lambda: G.latent_attention_expanded(*f, scale=0.06), store, plan]
+    alone = [c() for c in calls]
+    torch.cuda.synchronize()
+    graphs = []
+    for c in calls[:5]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = c()
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in range(len(calls) + len(graphs))]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(c())
+        for s, (g, _) in zip(streams[len(calls):], graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    G.check_latent_status()
+    for i, x in enumerate(got):
+        assert torch.equal(x, alone[i % len(calls)]), i
+    for (_, out), want in zip(graphs, alone):
+        assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
 def test_a_prompt_and_its_decode_together():
     """Plan, store, expand and attend a ragged prompt batch, then decode a token each: both forms give the
     layer's attention, and the output projection reads the result."""
