@@ -30,13 +30,18 @@
 // two a CTA) that a second kernel joins.
 //
 // Roles: warps 0-7 softmax (a strip of 16 keys and half of the heads each) and
-// epilogue, warp 8 TMA, warp 9 issues S^T, warp 10 issues O^T; in the last three one lane waits and
-// issues, since a lane that spins must not hold up one with work.  Row maxima are replaced only when a
-// score passes them by 2^8 (latent.cuh).  A token never shares a tile's keys
-// with one that sees fewer, so only rows behind a request's end are masked:
-// their scores are replaced, and their values cleared in shared memory (a zero
-// weight does not remove a NaN) up to the 16 rows that an MMA takes.
-// Every mbarrier wait is bounded, as in the expanded form.
+// epilogue, warp 8 TMA, warp 9 issues S^T, warp 10 issues O^T; in the last
+// three one lane waits and issues, since a lane that spins must not hold up one
+// with work.  Row maxima are replaced only when a score passes them by 2^8
+// (latent.cuh).  A token never shares a unit with one that sees fewer rows, so
+// only rows behind its own last one are masked: their scores are replaced, and
+// their values cleared in shared memory (a zero weight does not remove a NaN)
+// up to the 16 rows that an MMA takes.  Every mbarrier wait is bounded, as in
+// the expanded form.
+//
+// 64 requests of 6,000-8,192 rows, 64 heads: 112 us, 4.75 TB/s of rows (72% of
+// the measured copy); bound by the life of a stage: load, S^T, softmax and O^T
+// of a tile follow one another, and two tiles fit beside Q.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -61,7 +66,7 @@ constexpr int kStageBytes = kMaxChunks * kChunkBytes;
 constexpr int kSoftWarps = 8;
 constexpr int kSoftThreads = kSoftWarps * 32;
 constexpr int kThreads = kSoftThreads + 96;
-constexpr int kMaxGrid = 256;              // parts a join block holds weights of, halved
+constexpr int kMaxGrid = 256;              // CTAs, and so parts of a result, at most
 constexpr int kFewTokens = 64;             // of a request, planned by one thread
 constexpr int kSCol = 256;                 // TMEM: O^T at 0..255, two S^T tiles behind
 
