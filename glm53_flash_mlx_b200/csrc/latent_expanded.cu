@@ -24,7 +24,8 @@
 // long requests two CTAs work as a pair (cta_group::2, M = 256): each holds its
 // 128 queries, half the keys of a K tile and half the values of a V tile, and
 // rank 0 issues for both (2,048 queries over 8,192 keys, 64 heads of 256 + 256:
-// 856 us alone, 715 as pairs, 1,345 TFLOP/s).  For short ones a CTA an SM walks
+// 856 us alone, 715 to 771 as pairs by the clock that the power limit leaves,
+// 1,250 to 1,345 TFLOP/s).  For short ones a CTA an SM walks
 // the units instead, so that the set-up of one runs under the results of the
 // last.  Both rules are at the launch.
 //
