@@ -280,6 +280,8 @@ def latent_cache_write(kv: torch.Tensor, cache: torch.Tensor, slots: torch.Tenso
         rotated = kv.new_empty((T, heads, rope_dim))
         rp = rotated.data_ptr()
         queries, qp, (qt, qh) = _pieces(queries)
+    if T > 1 and kv.stride(0) < width:  # overlapping rows
+        kv = kv.clone(memory_format=torch.contiguous_format)
     kv, kp, (kt,) = _pieces(kv)
     if not slots.is_contiguous():
         slots = slots.contiguous()

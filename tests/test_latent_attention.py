@@ -389,6 +389,18 @@ def test_write_reports_a_slot_outside_the_cache():
     assert (cache.view(32, 576)[1] == 1).all() and cache.float().sum() == 576
 
 
+@pytest.mark.gpu
+def test_write_reads_overlapping_rows():
+    import glm53_flash_mlx_b200 as G
+
+    run = torch.randn(576 + 8 * 4, device="cuda").to(torch.bfloat16)
+    kv = run.unfold(0, 576, 8)  # five rows, each eight values behind the last
+    cache = torch.zeros((1, 16, 576), dtype=torch.bfloat16, device="cuda")
+    G.latent_cache_write(kv, cache, torch.arange(5, device="cuda"))
+    G.check_latent_status()
+    assert torch.equal(cache[0, :5], kv)
+
+
 # --- absorbed form ---------------------------------------------------------
 
 
