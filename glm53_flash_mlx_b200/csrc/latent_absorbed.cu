@@ -95,16 +95,16 @@ struct Args {
 
 struct Request {
   int q0, nq, len;
-  bool bad;
+  bool bad, disorder;  // disorder: bounds outside the tokens or descending
 };
 __device__ __forceinline__ Request request_at(const Args& a, int i) {
-  Request q{i, 1, a.lens[i], false};
+  Request q{i, 1, a.lens[i], false, false};
   if (a.starts) {
     q.q0 = a.starts[i];
     const int64_t n = (int64_t)a.starts[i + 1] - q.q0;
     q.nq = (int)n;
     if (q.q0 < 0 || n < 0 || q.q0 + n > a.T) {
-      q.bad = true;
+      q.bad = q.disorder = true;
       q.nq = 0;
     }
   }
@@ -207,11 +207,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   // tiles of all requests, this CTA's run of them, and where it begins
   {
     const int per = (a.B + kThreads - 1) / kThreads;
-    const int i0 = min(a.B, tid * per), i1 = min(a.B, i0 + per);
+    const int i0 = min(a.B, tid * per);
+    int i1 = min(a.B, i0 + per);
     int n = 0;
+    bool disorder = false;
     for (int i = i0; i < i1; ++i) {
       const Request q = request_at(a, i);
       n += tiles_of(q, a.G);
+      disorder |= q.disorder;
       if (q.bad && blockIdx.x == 0) report(a.status, a.status_host, kStatusBadGeometry);
     }
     if (warp == 9) {
@@ -248,12 +251,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 31) bars->warp_sum[warp] = s;
     if (blockIdx.x == 0)
       for (int64_t t = tid; t < a.T; t += kThreads) a.plan[1 + t] = -1;
-    __syncthreads();
+    // starts out of order, with which two requests could hold one token: no plan
+    const bool none = __syncthreads_or(disorder);
     int total = 0, before = s - n;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) before += bars->warp_sum[w];
       total += bars->warp_sum[w];
+    }
+    if (none) {
+      total = 0;
+      i1 = i0;
     }
     const int run = max(1, (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x));
     const int64_t begin = (int64_t)blockIdx.x * run;

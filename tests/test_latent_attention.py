@@ -562,6 +562,26 @@ def test_absorbed_reports_bad_pages_and_lengths():
         assert torch.equal(got[0], want[0]) and (got[1] == 0).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts", [[0, 40, 0, 40, 0, 40], [0, 10, 50, 30, 35, 40], [-1, 1, 2, 3, 4, 5],
+                                    [0, 10, 20, 30, 40, 41], [40, 30, 20, 10, 5, 0]])
+def test_absorbed_starts_out_of_order_bound_no_token(starts):
+    import glm53_flash_mlx_b200 as G
+
+    lens = [3000, 100, 2000, 40, 500]
+    ql, qr, cache, table, n, _, _ = make_absorbed(lens, [8] * 5, 16, 512, 64, 16, torch.bfloat16, 11)
+    bad = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    out, lse = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05, query_starts=bad, return_lse=True)
+    with pytest.raises(RuntimeError):
+        G.check_latent_status()
+    assert (out == 0).all() and (lse == -math.inf).all()
+    given = torch.ones_like(out)
+    G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05, query_starts=bad, out=given)
+    with pytest.raises(RuntimeError):
+        G.check_latent_status()
+    assert (given == 1).all()
+
+
 # --- expanded form ---------------------------------------------------------
 
 
