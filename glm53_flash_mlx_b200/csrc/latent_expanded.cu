@@ -134,7 +134,7 @@ __device__ __forceinline__ Bounds bounds_of(const Args& a, int i) {
 // Query tile `x` over all requests (in order; a request's last tile, which sees
 // the most keys, first); by a converged warp.  False when there are fewer.
 template <int ROWS>
-__device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u, bool report_bad) {
+__device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u) {
   const int lane = threadIdx.x & 31;
   int base = 0;
   for (int r0 = 0; r0 < a.B; r0 += 32) {
@@ -143,7 +143,6 @@ __device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u, bool re
     if (r0 + lane < a.B) {
       b = bounds_of(a, r0 + lane);
       n = (int)((b.nq + ROWS - 1) / ROWS);
-      if (report_bad && b.bad) report(a.status, a.status_host, kStatusBadGeometry);
     }
     int s = n;
 #pragma unroll
@@ -282,15 +281,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Walking CTAs take all heads of one query tile before the next tile, so that
   // a round of the grid holds units of like length.
   auto next_unit = [&](int i, Unit& u) {
-    const bool scan = warp == 0 && blockIdx.y == 0 && i == 0;
     if (a.persistent) {
       const int64_t at = blockIdx.x + (int64_t)i * gridDim.x;
       const int64_t x = at / a.H;
       u.head = (int)(at - x * a.H);
-      return x < INT32_MAX && find_tile<kUnit>(a, (int)x, u, scan);
+      return x < INT32_MAX && find_tile<kUnit>(a, (int)x, u);
     }
     u.head = blockIdx.y;
-    return i == 0 && find_tile<kUnit>(a, blockIdx.x / kCtas, u, scan);
+    return i == 0 && find_tile<kUnit>(a, blockIdx.x / kCtas, u);
   };
   tmem_fence_before();
   __syncthreads();
@@ -405,6 +403,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
+    if (blockIdx.y == 0)
+      for (int64_t i = (int64_t)blockIdx.x * 32 + lane; i < a.B; i += (int64_t)gridDim.x * 32)
+        if (bounds_of(a, (int)i).bad) report(a.status, a.status_host, kStatusBadGeometry);
   } else if (warp == 9) {
     // ---------------- MMA ----------------
     // All lanes walk the loops, so that descriptors stay in uniform registers;

@@ -788,7 +788,9 @@ int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, int64_t ql_
  * it) and lse FP32 [query_tokens, heads], contiguous; rows that see no key and
  * rows outside every request as in glm53_latent_absorbed.  nope_dim, value_dim
  * multiples of 64, rope_dim 0 or 64, nope_dim + rope_dim and value_dim at most
- * 256.  Starts outside the rows set GLM53_STATUS_BAD_GEOMETRY. */
+ * 256.  Starts that descend or leave the rows set GLM53_STATUS_BAD_GEOMETRY:
+ * such a request has no keys, or no queries (what its rows of out hold is not
+ * defined). */
 int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, int64_t qn_stride_h, const void* q_rope,
                           int64_t qr_stride_t, int64_t qr_stride_h, const void* k_nope, int64_t kn_stride_t,
                           int64_t kn_stride_h, const void* k_rope, int64_t kr_stride_t, const void* values,

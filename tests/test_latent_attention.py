@@ -672,6 +672,27 @@ def test_expanded_scores_that_grow():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,nq,nk,H,at", [(100, 40, 60, 16, 90), (3, 300, 2200, 2, 1), (300, 3, 5, 4, 250)])
+@pytest.mark.parametrize("which", ["queries", "keys"])
+def test_expanded_reports_starts_of_any_request(B, nq, nk, H, at, which):
+    """However many units come before it; the requests beside it keep their results."""
+    import glm53_flash_mlx_b200 as G
+
+    *t, qs, ks = make_expanded([nq] * B, [nk] * B, H, 128, 64, 128, torch.bfloat16, 7)
+    want = G.latent_attention_expanded(*t, qs, ks, scale=0.07)
+    bad = (qs if which == "queries" else ks).clone()
+    bad[at + 1] = -1  # the end of request `at`, the start of the next
+    out = torch.ones_like(want)
+    G.latent_attention_expanded(*t, *((bad, ks) if which == "queries" else (qs, bad)), scale=0.07, out=out)
+    with pytest.raises(RuntimeError):
+        G.check_latent_status()
+    first, last = at * nq, (at + 2) * nq
+    assert torch.equal(out[:first], want[:first]) and torch.equal(out[last:], want[last:])
+    if which == "keys":
+        assert (out[first:last] == 0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what", [math.nan, math.inf])
 def test_expanded_masked_keys_and_values_do_not_enter_large(what):
     """The same with more than 128 queries a request, at every place of a 256-row unit."""
