@@ -401,6 +401,27 @@ def test_write_reads_overlapping_rows():
     assert torch.equal(cache[0, :5], kv)
 
 
+@pytest.mark.gpu
+def test_write_refuses_rows_of_the_cache():
+    import glm53_flash_mlx_b200 as G
+
+    cache = torch.zeros((4, 16, 576), dtype=torch.bfloat16, device="cuda")
+    slots, pos = torch.arange(3, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda")
+    freq = torch.ones(32, dtype=torch.float64, device="cuda")
+    rows = cache.view(64, 576)
+    for at in (0, 61):
+        with pytest.raises(ValueError, match="outside the cache"):
+            G.latent_cache_write(rows[at:at + 3], cache, slots)
+        with pytest.raises(ValueError, match="outside the cache"):
+            G.latent_cache_write(torch.ones_like(rows[:3]), cache, slots, positions=pos, inv_freq=freq,
+                                 queries=rows[at:at + 3, 512:].unsqueeze(1))
+    # the rows beside a cache that is a part of a larger buffer are not in it
+    G.latent_cache_write(rows[45:48], cache[3:], slots)
+    G.latent_cache_write(rows[16:19], cache[:1], slots)
+    G.latent_cache_write(rows[48:48], cache, slots[:0])
+    G.check_latent_status()
+
+
 # --- absorbed form ---------------------------------------------------------
 
 
