@@ -199,20 +199,46 @@ __device__ __forceinline__ float2 turn_of(int32_t position, double inv_freq) {
   return make_float2(c, s);
 }
 
+// What a warp loads of token t's row, all at once: the slot, the first 512
+// latent values and the first rotary pair a lane, raw.
+struct Row {
+  int64_t slot;
+  uint4 raw[2];
+  uint16_t u, w;
+};
+// where rotary pair p lies in a row
+__device__ __forceinline__ int2 pair_at(const WriteArgs& a, int p) {
+  const int e = a.latent + (a.interleaved ? 2 * p : p);
+  return make_int2(e, e + (a.interleaved ? 1 : a.rope >> 1));
+}
+__device__ __forceinline__ Row load_row(const WriteArgs& a, int64_t t, int lane) {
+  Row row;
+  const uint16_t* x = a.kv + t * a.kv_stride;
+  row.slot = a.slots[t];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 32 * i < a.latent >> 3) row.raw[i] = reinterpret_cast<const uint4*>(x)[lane + 32 * i];
+  if (lane < a.rope >> 1) {
+    const int2 e = pair_at(a, lane);
+    row.u = x[e.x];
+    row.w = x[e.y];
+  }
+  return row;
+}
+
 template <typename E>
-__device__ __forceinline__ void write_row(const WriteArgs& a, int64_t t, int lane, const float2* turns) {
-  const int64_t slot = a.slots[t];
-  if (slot < 0) return;
-  if (slot >= a.cache_rows) {
+__device__ __forceinline__ void write_row(const WriteArgs& a, int64_t t, int lane, const float2* turns,
+                                          const Row& row) {
+  if (row.slot < 0) return;
+  if (row.slot >= a.cache_rows) {
     if (lane == 0) report(a.status, a.status_host, kStatusBadPage);
     return;
   }
   const uint16_t* x = a.kv + t * a.kv_stride;
-  uint16_t* y = a.cache + slot * (a.latent + a.rope);
+  uint16_t* y = a.cache + row.slot * (a.latent + a.rope);
   const uint4* xv = reinterpret_cast<const uint4*>(x);
   const int vecs = a.latent >> 3;
-  // the first 512 values stay in registers, raw; what is beyond is read again
-  uint4 raw[2];
+  // what is beyond the first 512 values is read again
   float sq = 0.f;
   auto square = [&](uint4 w) {
     float f[8];
@@ -220,14 +246,11 @@ __device__ __forceinline__ void write_row(const WriteArgs& a, int64_t t, int lan
 #pragma unroll
     for (int j = 0; j < 8; ++j) sq = fmaf(f[j], f[j], sq);
   };
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + 32 * i < vecs) raw[i] = xv[lane + 32 * i];
   float r = 1.f;
   if (a.weight) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (lane + 32 * i < vecs) square(raw[i]);
+      if (lane + 32 * i < vecs) square(row.raw[i]);
     for (int v = lane + 64; v < vecs; v += 32) square(xv[v]);
     r = 1.0f / sqrtf(warp_sum(sq) / (float)a.latent + a.eps);
   }
@@ -244,19 +267,19 @@ __device__ __forceinline__ void write_row(const WriteArgs& a, int64_t t, int lan
   };
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (lane + 32 * i < vecs) store(lane + 32 * i, raw[i]);
+    if (lane + 32 * i < vecs) store(lane + 32 * i, row.raw[i]);
   for (int v = lane + 64; v < vecs; v += 32) store(v, xv[v]);
-  const int half = a.rope >> 1;
-  for (int p = lane; p < half; p += 32) {
-    const int e0 = a.latent + (a.interleaved ? 2 * p : p), e1 = e0 + (a.interleaved ? 1 : half);
-    const float u = Elem<E>::to_float(x[e0]), w = Elem<E>::to_float(x[e1]);
+  for (int p = lane; p < a.rope >> 1; p += 32) {
+    const int2 e = pair_at(a, p);
+    const uint16_t u16 = p == lane ? row.u : x[e.x], w16 = p == lane ? row.w : x[e.y];
     if (a.positions) {
+      const float u = Elem<E>::to_float(u16), w = Elem<E>::to_float(w16);
       const float2 cs = turns ? turns[p] : turn_of(a.positions[t], a.inv_freq[p]);
-      y[e0] = Elem<E>::from_float(u * cs.x - w * cs.y);
-      y[e1] = Elem<E>::from_float(w * cs.x + u * cs.y);
+      y[e.x] = Elem<E>::from_float(u * cs.x - w * cs.y);
+      y[e.y] = Elem<E>::from_float(w * cs.x + u * cs.y);
     } else {
-      y[e0] = x[e0];
-      y[e1] = x[e1];
+      y[e.x] = u16;
+      y[e.y] = w16;
     }
   }
 }
@@ -270,7 +293,8 @@ constexpr int kQueryThreads = 256;
 template <typename E>
 __global__ void __launch_bounds__(kWriteThreads) latent_write_kernel(WriteArgs a) {
   const int64_t t = (int64_t)blockIdx.x * (kWriteThreads / 32) + (threadIdx.x >> 5);
-  if (t < a.T) write_row<E>(a, t, threadIdx.x & 31, nullptr);
+  const int lane = threadIdx.x & 31;
+  if (t < a.T) write_row<E>(a, t, lane, nullptr, load_row(a, t, lane));
 }
 
 // The two 8-value pieces that piece pair v of a head turns: values 8 v and
@@ -311,9 +335,10 @@ __global__ void __launch_bounds__(kQueryThreads + 32, 6) latent_write_queries_ke
   if (threadIdx.x >= kQueryThreads) {
     const int lane = threadIdx.x & 31;
     const int32_t position = a.positions[t];
+    const Row row = load_row(a, t, lane);
     for (int p = lane; p < half; p += 32) turns[p] = turn_of(position, a.inv_freq[p]);
     __syncthreads();
-    write_row<E>(a, t, lane, turns);
+    write_row<E>(a, t, lane, turns, row);
     return;
   }
   const int pieces = a.rope >> 4, items = a.heads * pieces;  // pairs of pieces: of a head, in all
