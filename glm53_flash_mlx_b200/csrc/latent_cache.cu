@@ -287,8 +287,13 @@ __device__ __forceinline__ void write_row(const WriteArgs& a, int64_t t, int lan
 // Without queries: a warp a token.  With queries: a block a token, whose last
 // warp forms the angles for all heads and stores the row while the others'
 // loads are on their way (4,096 tokens of 64 heads, 77 MB: 29.3 us when the
-// loads waited for the angles, 19.7 us so, 17.9 us with six blocks an SM).
-constexpr int kQueryThreads = 256;
+// loads waited for the angles, 16.1 us so).  A piece pair a thread is quickest
+// while the blocks run at once, blocks of fewer threads when they take turns,
+// with more tokens' angles and loads on their way.  64 heads, 256 / 64 threads
+// beside that warp: 1 token 2.9 / 3.3 us, 888 (6 blocks an SM) 4.6 / 4.8, 1,500
+// 7.2 / 6.1, 4,096 16.1 / 12.7, 16,384 68 / 53; 16 heads, 64 pairs: 600 3.4 / 3.1.
+constexpr int kWideQueries = 256, kWideBlocks = 6;
+constexpr int kNarrowQueries = 64, kNarrowBlocks = 16;
 
 template <typename E>
 __global__ void __launch_bounds__(kWriteThreads) latent_write_kernel(WriteArgs a) {
@@ -327,12 +332,13 @@ __device__ __forceinline__ void turn_pieces(const WriteArgs& a, const float2* tu
   q = pack8<E>(y);
 }
 
-template <typename E>
-__global__ void __launch_bounds__(kQueryThreads + 32, 6) latent_write_queries_kernel(WriteArgs a) {
+// QUERIES: threads that turn queries
+template <typename E, int QUERIES, int BLOCKS>
+__global__ void __launch_bounds__(QUERIES + 32, BLOCKS) latent_write_queries_kernel(WriteArgs a) {
   __shared__ float2 turns[kMaxRope / 2];
   const int64_t t = blockIdx.x;
   const int half = a.rope >> 1;
-  if (threadIdx.x >= kQueryThreads) {
+  if (threadIdx.x >= QUERIES) {
     const int lane = threadIdx.x & 31;
     const int32_t position = a.positions[t];
     const Row row = load_row(a, t, lane);
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(kQueryThreads + 32, 6) latent_write_queries_ke
     uint16_t* dst = out + h * a.rope;
     *reinterpret_cast<uint4*>(dst + at(v, 0)) = x;
     *reinterpret_cast<uint4*>(dst + at(v, 1)) = y;
-    i += kQueryThreads;
+    i += QUERIES;
     if (i < items) load(i, x, y);
   }
 }
@@ -369,7 +375,10 @@ __global__ void __launch_bounds__(kQueryThreads + 32, 6) latent_write_queries_ke
 template <typename E>
 void launch_write(const WriteArgs& a, cudaStream_t st) {
   if (a.q) {
-    latent_write_queries_kernel<E><<<(unsigned)a.T, kQueryThreads + 32, 0, st>>>(a);
+    if ((int64_t)a.heads * (a.rope >> 4) > kNarrowQueries && a.T <= (int64_t)kWideBlocks * sm_count())
+      latent_write_queries_kernel<E, kWideQueries, kWideBlocks><<<(unsigned)a.T, kWideQueries + 32, 0, st>>>(a);
+    else
+      latent_write_queries_kernel<E, kNarrowQueries, kNarrowBlocks><<<(unsigned)a.T, kNarrowQueries + 32, 0, st>>>(a);
   } else {
     const int64_t blocks = (a.T + kWriteThreads / 32 - 1) / (kWriteThreads / 32);
     latent_write_kernel<E><<<(unsigned)blocks, kWriteThreads, 0, st>>>(a);

@@ -340,7 +340,7 @@ def rounded_close(got, want, scale):
 @pytest.mark.parametrize("T,latent,rope,heads,norm,interleaved,page", [
     (1, 512, 64, 64, True, False, 64), (9, 512, 64, 5, True, True, 16), (130, 512, 64, 0, True, False, 48),
     (17, 8, 16, 1, True, False, 3), (33, 1024, 256, 3, False, True, 16), (8, 512, 0, 0, True, False, 16),
-    (5, 256, 64, 0, False, False, 16)])
+    (5, 256, 64, 0, False, False, 16), (1000, 512, 64, 64, True, False, 64), (1111, 128, 128, 9, True, True, 16)])
 def test_write_matches(dtype, T, latent, rope, heads, norm, interleaved, page):
     import glm53_flash_mlx_b200 as G
 
