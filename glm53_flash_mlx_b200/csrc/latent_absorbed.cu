@@ -768,12 +768,12 @@ __device__ __forceinline__ void store_joined(uint16_t* dst, const float4& o, flo
   *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<E>::pack(o.x * inv, o.y * inv), Elem<E>::pack(o.z * inv, o.w * inv));
 }
 
-// Few results: a block takes 128 values of one (token, head), and each of 16
-// warps every 16th part of them.
-template <typename E>
-__global__ void __launch_bounds__(512) join_few_kernel(Args a, int heads) {
+// Few results: a block takes 128 values of one (token, head), and each of its
+// WAYS warps every WAYS-th part of them.
+template <typename E, int WAYS>
+__global__ void __launch_bounds__(32 * WAYS) join_few_kernel(Args a, int heads) {
   __shared__ float weight[kMaxGrid];
-  __shared__ float4 part[16][32];
+  __shared__ float4 part[WAYS][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int t = blockIdx.x, h = blockIdx.y, way = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col = 4 * (blockIdx.z * 32 + lane);
@@ -791,15 +791,15 @@ __global__ void __launch_bounds__(512) join_few_kernel(Args a, int heads) {
   float4 x[kBatch], o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int k = 0; k < kBatch; ++k) {
-    const int p = way + 16 * k;
+    const int p = way + WAYS * k;
     x[k] = mine && p < q.count ? *reinterpret_cast<const float4*>(a.po + q.slot(p, heads) * a.R + col) : o;
   }
   const float2 total = part_weights(a, q, heads, weight, way == 0);
   __syncthreads();
-  for (int p0 = way; p0 < q.count; p0 += kBatch * 16) {
+  for (int p0 = way; p0 < q.count; p0 += kBatch * WAYS) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int p = p0 + 16 * k, next = p + 16 * kBatch;
+      const int p = p0 + WAYS * k, next = p + WAYS * kBatch;
       if (p < q.count) add_part(o, weight[p], x[k]);
       if (mine && next < q.count) x[k] = *reinterpret_cast<const float4*>(a.po + q.slot(next, heads) * a.R + col);
     }
@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(512) join_few_kernel(Args a, int heads) {
   __syncthreads();
   if (way) return;
 #pragma unroll
-  for (int k = 1; k < 16; ++k) add_part(o, 1.f, part[k][lane]);
+  for (int k = 1; k < WAYS; ++k) add_part(o, 1.f, part[k][lane]);
   if (mine) store_joined<E>(a.out + at * a.R + col, o, total.x);
   if (a.lse && threadIdx.x == 0 && blockIdx.z == 0) a.lse[at] = total.y;
 }
@@ -897,9 +897,29 @@ int launch(const CUtensorMap& ql, const CUtensorMap& qr, const CUtensorMap& kv0,
   if (rc) return rc;
   absorbed_kernel<E, N><<<grid_size(), kThreads, kSmemBytes, st>>>(ql, qr, kv0, kv1, a);
   if ((rc = check_launch("absorbed_kernel"))) return rc;
-  if (a.T * a.H <= 512)
-    launch_programmatic(join_few_kernel<E>, dim3((unsigned)a.T, (unsigned)a.H, (unsigned)(a.R / 128)), dim3(512), 0,
-                        st, a, N);
+  // How many warps share a result: many while there are few results, which then
+  // have many parts.  1,000 / 12,000 rows each, whole calls, us by warps:
+  //   results         16           8            4            2            1
+  //   1 x 64      15.5 / 20.8  15.5 / 22.1  15.9 / 25.4  16.6 / 28.9  20.3 / 70.3
+  //   2 x 64      18.6 / 29.3  15.5 / 25.3  16.1 / 27.8  16.8 / 31.6  20.5 / 58.4
+  //   4 x 64      24.0 / 38.3  18.4 / 32.1  16.4 / 30.5  17.5 / 33.0  23.8 / 47.7
+  //   8 x 64      35.4 / 61.6  23.9 / 50.0  18.8 / 44.7  17.9 / 45.0  25.6 / 52.1
+  //   16 x 64     52.6 / 96.2  34.6 / 77.5  24.7 / 67.5  20.5 / 62.6  21.9 / 65.9
+  //   24 x 64     75.2 / 132   48.7 / 104   35.3 / 90.1  29.0 / 83.8  26.5 / 82.0
+  //   16 x 16     21.9 / 57.9  17.3 / 52.7  15.5 / 51.5  15.7 / 50.8  18.4 / 56.1
+  //   4 x 128     35.2 / 57.2  23.9 / 46.0  18.8 / 40.6  17.9 / 39.9  25.9 / 49.2
+  // Two warps no longer pay where a unit has two or three parts: 64 x 16 27.4 / 148
+  // with two, 25.8 / 146 with one.
+  const int64_t results = a.T * a.H;
+  const dim3 pieces((unsigned)a.T, (unsigned)a.H, (unsigned)(a.R / 128));
+  if (results <= 64)
+    launch_programmatic(join_few_kernel<E, 16>, pieces, dim3(512), 0, st, a, N);
+  else if (results <= 128)
+    launch_programmatic(join_few_kernel<E, 8>, pieces, dim3(256), 0, st, a, N);
+  else if (results <= 384)
+    launch_programmatic(join_few_kernel<E, 4>, pieces, dim3(128), 0, st, a, N);
+  else if (results <= 1024 && 3 * a.T * a.G <= grid_size())
+    launch_programmatic(join_few_kernel<E, 2>, pieces, dim3(64), 0, st, a, N);
   else
     launch_programmatic(join_many_kernel<E>, dim3((unsigned)a.T, (unsigned)((a.H + 3) / 4)), dim3(128), 0, st, a, N);
   return check_launch("join_kernel");
