@@ -99,6 +99,7 @@ struct __align__(8) Bars {
   uint32_t tmem_base;
   int abort_flag;
   Unit unit;      // the softmax warps' unit
+  int walk[kSoftWarps][2];  // where each softmax warp's search for a unit stands (MANY)
   int poison[2];  // by unit parity: the unit (from 1) with values that are not finite in a masked tile
 };
 
@@ -132,12 +133,13 @@ __device__ __forceinline__ Bounds bounds_of(const Args& a, int i) {
 }
 
 // Query tile `x` over all requests (in order; a request's last tile, which sees
-// the most keys, first); by a converged warp.  False when there are fewer.
+// the most keys, first); by a converged warp.  False when there are fewer.  The
+// search begins at request `r0`, whose first tile is `base`, and leaves both for
+// the next, which must not look for an earlier tile.
 template <int ROWS>
-__device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u) {
+__device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u, int& r0, int& base) {
   const int lane = threadIdx.x & 31;
-  int base = 0;
-  for (int r0 = 0; r0 < a.B; r0 += 32) {
+  for (; r0 < a.B; r0 += 32) {
     Bounds b{};
     int n = 0;
     if (r0 + lane < a.B) {
@@ -232,7 +234,7 @@ __device__ __forceinline__ void quad_transpose(uint4 (&p)[4], int lane) {
   }
 }
 
-template <typename E, bool PAIR>
+template <typename E, bool PAIR, bool MANY>
 __global__ void __launch_bounds__(kThreads, 1)
     expanded_kernel(const __grid_constant__ CUtensorMap qn_map, const __grid_constant__ CUtensorMap qr_map,
                     const __grid_constant__ CUtensorMap kn_map, const __grid_constant__ CUtensorMap kr_map,
@@ -280,15 +282,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   // The CTA's units in order, by a converged warp: every role walks them itself.
   // Walking CTAs take all heads of one query tile before the next tile, so that
   // a round of the grid holds units of like length.
-  auto next_unit = [&](int i, Unit& u) {
+  auto next_unit = [&](int i, Unit& u, int& r0, int& base) {
     if (a.persistent) {
       const int64_t at = blockIdx.x + (int64_t)i * gridDim.x;
       const int64_t x = at / a.H;
       u.head = (int)(at - x * a.H);
-      return x < INT32_MAX && find_tile<kUnit>(a, (int)x, u);
+      return x < INT32_MAX && find_tile<kUnit>(a, (int)x, u, r0, base);
     }
     u.head = blockIdx.y;
-    return i == 0 && find_tile<kUnit>(a, blockIdx.x / kCtas, u);
+    return i == 0 && find_tile<kUnit>(a, blockIdx.x / kCtas, u, r0, base);
   };
   tmem_fence_before();
   __syncthreads();
@@ -330,7 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int cut = 0;
     bool ok = true;
     Unit u;
-    for (int i = 0; next_unit(i, u); ++i) {
+    int r0 = 0, base = 0;
+    for (int i = 0; next_unit(i, u, r0, base); ++i) {
       const int tiles = tiles_of(u), cut0 = cut_of(u);
       if (lane == 0 && tiles > 0 && ok) {
         auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int z, uint64_t* p) {
@@ -429,7 +432,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       return ok;
     };
     Unit u;
-    for (int i = 0; next_unit(i, u); ++i) {
+    int r0 = 0, base = 0;
+    for (int i = 0; next_unit(i, u, r0, base); ++i) {
       const int tiles = tiles_of(u);
       if (tiles == 0) continue;
       if (leader) ok = ok && mbar_wait_fast(bar(&bars->q_full), queries & 1u, abort_flag);
@@ -519,7 +523,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t seq = 0;
     int cut = 0, units = 0;
     Unit u;
-    for (int i = 0; next_unit(i, u); ++i) {
+    int r0 = 0, base = 0;
+    for (int i = 0; next_unit(i, u, r0, base); ++i) {
       const int tiles = tiles_of(u), cut0 = cut_of(u);
       if (tiles == 0) continue;
       ++units;
@@ -570,11 +575,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* xchg = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 1024);  // [2][128]
     bool stop = false;
     int units = 0;
+    if constexpr (MANY) {
+      if (lane == 0) bars->walk[warp][0] = bars->walk[warp][1] = 0;
+      __syncwarp();
+    }
     for (int i = 0; !stop; ++i) {
     int tiles, vis, vis0;
     {
       Unit u;
-      if (!next_unit(i, u)) break;
+      int r0 = 0, base = 0;
+      if constexpr (MANY) {
+        r0 = bars->walk[warp][0];
+        base = bars->walk[warp][1];
+      }
+      if (!next_unit(i, u, r0, base)) break;
+      if constexpr (MANY) {
+        __syncwarp();
+        if (lane == 0) {
+          bars->walk[warp][0] = r0;
+          bars->walk[warp][1] = base;
+        }
+        __syncwarp();
+      }
       // kept in shared memory for the epilogue: registers are short in between
       if (tid == 0) bars->unit = u;
       const int j0 = u.first + rank * kTile;
@@ -783,10 +805,10 @@ int make_shared_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, 
   return GLM53_OK;
 }
 
-template <typename E, bool PAIR>
+template <typename E, bool PAIR, bool MANY = false>
 int launch(const CUtensorMap& qn, const CUtensorMap& qr, const CUtensorMap& kn, const CUtensorMap& kr,
            const CUtensorMap& v, const Args& a, cudaStream_t st) {
-  const auto kernel = expanded_kernel<E, PAIR>;
+  const auto kernel = expanded_kernel<E, PAIR, MANY>;
   const int rc = ensure_max_smem((const void*)kernel, kSmemBytes);
   if (rc) return rc;
   // Units at most: one more a request than whole units in all.
@@ -799,10 +821,11 @@ int launch(const CUtensorMap& qn, const CUtensorMap& qr, const CUtensorMap& kn, 
   // 4 x 512 92 / 111, 1 x 2,048 of 256 + 192 172 / 182.  All heads of a query
   // tile come before the next tile, so one request's keys and values of all
   // heads should stay in L2 (126 MB): over 8,192 keys of 256 + 192 values
-  // (402 MB) 947 / 772, of 192 + 64 (201 MB) 615 / 543.  The search for a unit
-  // takes 32 requests a step.  A pair's units are long and stay one each.
+  // (402 MB) 947 / 772, of 192 + 64 (201 MB) 615 / 543.  Many short requests, one
+  // unit a CTA / walking: 300 of 100 queries and keys 2,230 / 1,026, 2,000 of 3 and
+  // 20 19,960 / 5,640.  A pair's units are long and stay one each.
   const double held = 2.0 * a.Tk / a.B * a.H * (a.dn + a.dv);
-  b.persistent = !PAIR && a.B <= 256 && held <= 126e6;
+  b.persistent = !PAIR && held <= 126e6;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = b.persistent ? dim3((unsigned)std::min<int64_t>(sm_count(), units * a.H))
                              : dim3((unsigned)(units * kCtas), (unsigned)a.H);
@@ -898,5 +921,13 @@ extern "C" int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, in
   const cudaStream_t st = (cudaStream_t)stream;
   if (pair)
     return bf16 ? launch<__nv_bfloat16, true>(qn, qr, kn, kr, v, a, st) : launch<__half, true>(qn, qr, kn, kr, v, a, st);
+  // Softmax warps whose search for a unit goes on where it stood, for many
+  // requests: 64 heads, from the start / so, 200 requests of 20 queries and 40
+  // keys 658 / 605 us, 300 1,049 / 902, 2,000 of 3 and 20 16,400 / 5,640; but
+  // spilled registers cost 8 requests of 512 154 / 159, five ragged ones of 16
+  // heads 31.3 / 32.0.
+  if (requests > 128)
+    return bf16 ? launch<__nv_bfloat16, false, true>(qn, qr, kn, kr, v, a, st)
+                : launch<__half, false, true>(qn, qr, kn, kr, v, a, st);
   return bf16 ? launch<__nv_bfloat16, false>(qn, qr, kn, kr, v, a, st) : launch<__half, false>(qn, qr, kn, kr, v, a, st);
 }
