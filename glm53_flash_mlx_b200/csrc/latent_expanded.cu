@@ -900,7 +900,16 @@ extern "C" int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, in
   // 4,096 keys 140 / 122, 2,048 over 8,192 856 / 715; 16 heads of 192 + 128
   // values, 4 x 512 queries over 512 keys 24 / 33, over 2,512 72.5 / 72.3, 512
   // over 4,096 51 / 48.
-  const bool pair = value_dim % 128 == 0 && Tq > requests * kTile && Tk >= requests * 2048;
+  // With one query tile a request a pair's second half of rows is empty, but two
+  // SMs read its keys: worth it for wide rows while there are SMs for all pairs.
+  // Alone / pairs, 128 queries over 8,192 keys: 64 heads of 256 + 256 values
+  // 137 / 118, 8 heads 119 / 95 (over 2,048 37 / 33), 64 heads of 256 + 128
+  // values 97.5 / 98.8, 96 heads 104 / 212.
+  const bool one_tile = Tq <= requests * kTile;
+  const bool pair = value_dim % 128 == 0 &&
+                    (one_tile ? nope_dim + rope_dim + value_dim > 448 && 2 * requests * heads <= sm_count() &&
+                                    Tk >= requests * 2560
+                              : Tk >= requests * 2048);
   const int key_rows = pair ? kTile / 2 : kTile;
   CUtensorMap qn, qr, kn, kr, v;
   int rc = make_rows_map(&qn, q_nope, bf16, nope_dim, heads, qn_stride_h, Tq, qn_stride_t, kTile);

@@ -657,6 +657,8 @@ EXPANDED = [
     ([385], [2000], 1, 128, 0, 256, False),
     ([200] * 8, [2200] * 8, 4, 192, 64, 256, True),  # three tiles that the mask cuts, loaded one behind the other
     ([250, 129], [2001, 3333], 2, 128, 64, 128, True),
+    ([1], [3000], 2, 192, 64, 256, True),
+    ([100, 28], [2600, 2700], 3, 192, 64, 256, True),  # one query tile a request, long keys
     ([5] * 150 + [140] + [2, 0] * 100, [9] * 150 + [150] + [2, 3] * 100, 2, 64, 64, 64, True),  # many requests
 ]
 
