@@ -705,9 +705,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Joins the partial results of units that several CTAs shared:
 //   o = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p,  M the largest m_p,
-// and fills what no CTA wrote (tokens that see nothing; with fill_tail those
-// outside every request).  Bound by latency: the plan is one round to L2, all
-// maxima, sums and the first rows a second.
+// and fills what no CTA wrote: tokens that see nothing, and of those outside
+// every request the log-sums, with fill_tail the results too.  Bound by latency:
+// the plan is one round to L2, all maxima, sums and the first rows a second.
 
 // Where the parts of unit (t, h) are; false when there is nothing to join.
 struct Parts {
@@ -782,8 +782,8 @@ __global__ void __launch_bounds__(32 * WAYS) join_few_kernel(Args a, int heads) 
   Parts q;
   bool empty, fill;
   if (!find_parts(a, t, h, heads, q, empty, fill)) {
-    if (!empty || !fill) return;
-    if (way == 0 && mine) *reinterpret_cast<uint2*>(a.out + at * a.R + col) = make_uint2(0, 0);
+    if (!empty) return;
+    if (fill && way == 0 && mine) *reinterpret_cast<uint2*>(a.out + at * a.R + col) = make_uint2(0, 0);
     if (a.lse && threadIdx.x == 0 && blockIdx.z == 0) a.lse[at] = -INFINITY;
     return;
   }
@@ -825,8 +825,8 @@ __global__ void __launch_bounds__(128) join_many_kernel(Args a, int heads) {
   Parts q;
   bool empty, fill;
   if (!find_parts(a, t, h, heads, q, empty, fill)) {
-    if (!empty || !fill) return;
-    for (int c = 0; c < a.R; c += 128) *reinterpret_cast<uint2*>(dst + c) = make_uint2(0, 0);
+    if (!empty) return;
+    for (int c = 0; c < a.R && fill; c += 128) *reinterpret_cast<uint2*>(dst + c) = make_uint2(0, 0);
     if (a.lse && lane == 0) a.lse[at] = -INFINITY;
     return;
   }

@@ -736,16 +736,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other may reach its memory
-  if (a.fill_tail) {
-    // rows outside every request, by all CTAs
+  if (a.fill_tail || a.lse) {
+    // rows outside every request, by all CTAs: their log-sums, with fill_tail the results too
     const int64_t lo = a.B ? max(0, a.q_starts[a.B]) : 0, hi = a.B ? min(a.Tq, (int64_t)max(0, a.q_starts[0])) : 0;
     const int64_t rows = hi + max((int64_t)0, a.Tq - lo);
-    const int pieces = a.dv >> 3;
+    const int pieces = a.fill_tail ? a.dv >> 3 : 1;
     const int64_t step = (int64_t)gridDim.x * gridDim.y * kThreads;
     for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + tid; i < rows * a.H * pieces; i += step) {
       const int64_t k = i / (a.H * pieces), rest = i - k * a.H * pieces;
       const int64_t row = k < hi ? k : lo + (k - hi), at = row * a.H + rest / pieces;
-      reinterpret_cast<uint4*>(a.out + at * a.dv)[rest % pieces] = make_uint4(0, 0, 0, 0);
+      if (a.fill_tail) reinterpret_cast<uint4*>(a.out + at * a.dv)[rest % pieces] = make_uint4(0, 0, 0, 0);
       if (a.lse && rest % pieces == 0) a.lse[at] = -INFINITY;
     }
   }

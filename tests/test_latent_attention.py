@@ -547,6 +547,33 @@ def test_absorbed_padded_batch_keeps_or_zeroes_the_rest():
     G.check_latent_status()
 
 
+def stale(*shape):
+    """Leaves blocks of this size that hold other values to the allocator."""
+    blocks = [torch.full(shape, 7.0, device="cuda") for _ in range(8)]
+    del blocks
+
+
+@pytest.mark.gpu
+def test_absorbed_log_sums_behind_the_last_token_of_a_given_result():
+    import glm53_flash_mlx_b200 as G
+
+    lens, queries = [100, 30, 5], [2, 1, 0]
+    ql, qr, cache, table, n, starts, _ = make_absorbed(lens, queries, 16, 512, 64, 16, torch.bfloat16, 9)
+    ql, qr = (torch.cat([x, x[:2], x[:2]]) for x in (ql, qr))
+    for starts in (starts, starts + 2):  # four tokens behind the last request; two before the first and behind the last
+        first = int(starts[0])
+        want, lse = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05, query_starts=starts, return_lse=True)
+        given = torch.full_like(want, 7.0)
+        stale(7, 16)
+        got, again = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05, query_starts=starts, out=given,
+                                                 return_lse=True)
+        outside = torch.ones(7, dtype=torch.bool, device="cuda")
+        outside[first:first + 3] = False
+        assert (again[outside] == -math.inf).all() and torch.equal(again, lse)
+        assert (given[outside] == 7).all() and torch.equal(given[~outside], want[~outside])
+    G.check_latent_status()
+
+
 @pytest.mark.gpu
 def test_outputs_that_overlap_inputs_are_refused():
     import glm53_flash_mlx_b200 as G
@@ -790,6 +817,27 @@ def test_expanded_rows_outside_every_request():
     with pytest.raises(RuntimeError):
         G.check_latent_status()
     assert torch.equal(got[:40], want[:40]) and (got[40:] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nk", [[60, 30], [4500, 30]])  # CTAs alone, CTA pairs
+def test_expanded_log_sums_behind_the_last_query_of_a_given_result(nk):
+    import glm53_flash_mlx_b200 as G
+
+    nq = [240, 30]
+    *t, qs, ks = make_expanded(nq, nk, 3, 128, 64, 128, torch.bfloat16, 8)
+    t[0], t[1] = (torch.cat([x, x[:5]]) for x in t[:2])
+    for qs in (qs, qs + 2):  # five queries behind the last request; two before the first and three behind the last
+        first = int(qs[0])
+        want, lse = G.latent_attention_expanded(*t, qs, ks, scale=0.07, return_lse=True)
+        given = torch.full_like(want, 7.0)
+        stale(275, 3)
+        got, again = G.latent_attention_expanded(*t, qs, ks, scale=0.07, out=given, return_lse=True)
+        outside = torch.ones(275, dtype=torch.bool, device="cuda")
+        outside[first:first + 270] = False
+        assert (again[outside] == -math.inf).all() and torch.equal(again, lse)
+        assert (given[outside] == 7).all() and torch.equal(given[~outside], want[~outside])
+    G.check_latent_status()
 
 
 # --- streams, graphs, together ---------------------------------------------
