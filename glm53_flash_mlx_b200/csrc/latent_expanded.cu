@@ -62,6 +62,7 @@ constexpr int kSoftWarps = 8;
 constexpr int kSoftThreads = kSoftWarps * 32;
 constexpr int kCleanWarps = 2;
 constexpr int kThreads = kSoftThreads + 128;
+constexpr int kFillCtas = 512;             // CTAs that fill rows outside every request, at most
 constexpr int kOCol = 0;     // TMEM: O at 0..255, S tiles at 256 and 384
 constexpr int kSCol = 256;
 
@@ -94,12 +95,19 @@ struct Unit {
   }
 };
 
+// Where a search for a query tile stands: at request `r0`, whose first tile is
+// `base`; `top`, once a start out of order was met, is the
+// largest valid start before it (below), else -1.
+struct Walk {
+  int r0 = 0, base = 0, top = -1;
+};
+
 struct __align__(8) Bars {
   uint64_t q_full, q_empty, full[kSlots], empty[kSlots], cut_full[4], s_full[2], p_full[2], o_done[2], drain;
   uint32_t tmem_base;
   int abort_flag;
   Unit unit;      // the softmax warps' unit
-  int walk[kSoftWarps][2];  // where each softmax warp's search for a unit stands (MANY)
+  Walk walk[kSoftWarps];  // where each softmax warp's search for a unit stands (MANY)
   int poison[2];  // by unit parity: the unit (from 1) with values that are not finite in a masked tile
 };
 
@@ -112,7 +120,7 @@ static_assert(kSmemBytes <= 232448, "227 KB a CTA");
 // key bounds as no keys.
 struct Bounds {
   int64_t q0, nq, k0, nk;
-  bool bad;
+  bool bad, ordered;  // ordered: the query bounds are valid
 };
 __device__ __forceinline__ Bounds bounds_of(const Args& a, int i) {
   Bounds b;
@@ -120,11 +128,9 @@ __device__ __forceinline__ Bounds bounds_of(const Args& a, int i) {
   b.nq = (int64_t)a.q_starts[i + 1] - b.q0;
   b.k0 = a.k_starts[i];
   b.nk = (int64_t)a.k_starts[i + 1] - b.k0;
-  b.bad = false;
-  if (b.q0 < 0 || b.nq < 0 || b.q0 + b.nq > a.Tq) {
-    b.bad = true;
-    b.nq = 0;
-  }
+  b.ordered = b.q0 >= 0 && b.nq >= 0 && b.q0 + b.nq <= a.Tq;
+  b.bad = !b.ordered;
+  if (!b.ordered) b.nq = 0;
   if (b.k0 < 0 || b.nk < 0 || b.k0 + b.nk > a.Tk) {
     b.bad = true;
     b.k0 = b.nk = 0;
@@ -132,19 +138,46 @@ __device__ __forceinline__ Bounds bounds_of(const Args& a, int i) {
   return b;
 }
 
+// Where query starts descend or leave the rows, the requests that keep their
+// queries are those with bounds in order that begin at or behind every valid
+// start before them: no two of them share a row.
+__device__ __forceinline__ bool valid_start(const Args& a, int64_t v) { return v >= 0 && v <= a.Tq; }
+
+// By a converged warp, 32 requests a step, `b` those of this lane (all 0 behind
+// the last) and `top` the largest valid start before the step (the step's first
+// start is as large where all before it is in order): whether this lane's request
+// keeps its queries.
+__device__ __forceinline__ bool keeps_queries(const Args& a, const Bounds& b, int& top) {
+  const int lane = threadIdx.x & 31;
+  int most = valid_start(a, b.q0) ? (int)b.q0 : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, most, o);
+    if (lane >= o) most = max(most, y);
+  }
+  most = max(most, top);
+  top = __shfl_sync(0xffffffffu, most, 31);
+  return b.ordered && b.q0 >= most;
+}
+
 // Query tile `x` over all requests (in order; a request's last tile, which sees
 // the most keys, first); by a converged warp.  False when there are fewer.  The
-// search begins at request `r0`, whose first tile is `base`, and leaves both for
-// the next, which must not look for an earlier tile.
+// next search goes on from `w` and must not look for an earlier tile.
 template <int ROWS>
-__device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u, int& r0, int& base) {
+__device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u, Walk& w) {
   const int lane = threadIdx.x & 31;
-  for (; r0 < a.B; r0 += 32) {
+  for (; w.r0 < a.B; w.r0 += 32) {
     Bounds b{};
     int n = 0;
-    if (r0 + lane < a.B) {
-      b = bounds_of(a, r0 + lane);
+    const bool real = w.r0 + lane < a.B;
+    if (real) {
+      b = bounds_of(a, w.r0 + lane);
       n = (int)((b.nq + ROWS - 1) / ROWS);
+    }
+    int top = w.top;
+    if (top >= 0 || __any_sync(0xffffffffu, real && !b.ordered)) {
+      top = max(top, 0);
+      if (!keeps_queries(a, b, top)) n = 0;
     }
     int s = n;
 #pragma unroll
@@ -152,7 +185,7 @@ __device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u, int& r0
       const int y = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += y;
     }
-    const int lo = base + s - n;
+    const int lo = w.base + s - n;
     const uint32_t mine = __ballot_sync(0xffffffffu, x >= lo && x < lo + n);
     if (mine) {
       const int src = __ffs(mine) - 1;
@@ -163,7 +196,8 @@ __device__ __forceinline__ bool find_tile(const Args& a, int x, Unit& u, int& r0
       u.first = __shfl_sync(0xffffffffu, (n - 1 - (x - lo)) * ROWS, src);
       return true;
     }
-    base += __shfl_sync(0xffffffffu, s, 31);
+    w.base += __shfl_sync(0xffffffffu, s, 31);
+    w.top = top;
   }
   return false;
 }
@@ -282,15 +316,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   // The CTA's units in order, by a converged warp: every role walks them itself.
   // Walking CTAs take all heads of one query tile before the next tile, so that
   // a round of the grid holds units of like length.
-  auto next_unit = [&](int i, Unit& u, int& r0, int& base) {
+  auto next_unit = [&](int i, Unit& u, Walk& w) {
     if (a.persistent) {
       const int64_t at = blockIdx.x + (int64_t)i * gridDim.x;
       const int64_t x = at / a.H;
       u.head = (int)(at - x * a.H);
-      return x < INT32_MAX && find_tile<kUnit>(a, (int)x, u, r0, base);
+      return x < INT32_MAX && find_tile<kUnit>(a, (int)x, u, w);
     }
     u.head = blockIdx.y;
-    return i == 0 && find_tile<kUnit>(a, blockIdx.x / kCtas, u, r0, base);
+    return i == 0 && find_tile<kUnit>(a, blockIdx.x / kCtas, u, w);
   };
   tmem_fence_before();
   __syncthreads();
@@ -332,8 +366,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int cut = 0;
     bool ok = true;
     Unit u;
-    int r0 = 0, base = 0;
-    for (int i = 0; next_unit(i, u, r0, base); ++i) {
+    Walk w;
+    for (int i = 0; next_unit(i, u, w); ++i) {
       const int tiles = tiles_of(u), cut0 = cut_of(u);
       if (lane == 0 && tiles > 0 && ok) {
         auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int z, uint64_t* p) {
@@ -432,8 +466,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       return ok;
     };
     Unit u;
-    int r0 = 0, base = 0;
-    for (int i = 0; next_unit(i, u, r0, base); ++i) {
+    Walk w;
+    for (int i = 0; next_unit(i, u, w); ++i) {
       const int tiles = tiles_of(u);
       if (tiles == 0) continue;
       if (leader) ok = ok && mbar_wait_fast(bar(&bars->q_full), queries & 1u, abort_flag);
@@ -523,8 +557,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t seq = 0;
     int cut = 0, units = 0;
     Unit u;
-    int r0 = 0, base = 0;
-    for (int i = 0; next_unit(i, u, r0, base); ++i) {
+    Walk w;
+    for (int i = 0; next_unit(i, u, w); ++i) {
       const int tiles = tiles_of(u), cut0 = cut_of(u);
       if (tiles == 0) continue;
       ++units;
@@ -576,25 +610,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool stop = false;
     int units = 0;
     if constexpr (MANY) {
-      if (lane == 0) bars->walk[warp][0] = bars->walk[warp][1] = 0;
+      if (lane == 0) bars->walk[warp] = Walk{};
       __syncwarp();
     }
     for (int i = 0; !stop; ++i) {
     int tiles, vis, vis0;
     {
       Unit u;
-      int r0 = 0, base = 0;
-      if constexpr (MANY) {
-        r0 = bars->walk[warp][0];
-        base = bars->walk[warp][1];
-      }
-      if (!next_unit(i, u, r0, base)) break;
+      Walk w;
+      if constexpr (MANY) w = bars->walk[warp];
+      if (!next_unit(i, u, w)) break;
       if constexpr (MANY) {
         __syncwarp();
-        if (lane == 0) {
-          bars->walk[warp][0] = r0;
-          bars->walk[warp][1] = base;
-        }
+        if (lane == 0) bars->walk[warp] = w;
         __syncwarp();
       }
       // kept in shared memory for the epilogue: registers are short in between
@@ -734,19 +762,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_fence_before();
     }
   }
-  __syncthreads();
+  // Rows outside every request: their log-sums, with fill_tail the results too.
+  // The warps that are done early look whether all starts are in order.
+  const int64_t cta = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  const int64_t ctas = min((int64_t)gridDim.x * gridDim.y, (int64_t)kFillCtas);
+  const bool fills = (a.fill_tail || a.lse) && cta < ctas;
+  bool unordered = false;
+  if (fills && warp >= 10)
+    for (int i = tid - 320; i < a.B; i += 64) unordered |= !bounds_of(a, i).ordered;
+  const bool disorder = __syncthreads_or(unordered);
   if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other may reach its memory
-  if (a.fill_tail || a.lse) {
-    // rows outside every request, by all CTAs: their log-sums, with fill_tail the results too
-    const int64_t lo = a.B ? max(0, a.q_starts[a.B]) : 0, hi = a.B ? min(a.Tq, (int64_t)max(0, a.q_starts[0])) : 0;
-    const int64_t rows = hi + max((int64_t)0, a.Tq - lo);
+  if (fills) {
     const int pieces = a.fill_tail ? a.dv >> 3 : 1;
-    const int64_t step = (int64_t)gridDim.x * gridDim.y * kThreads;
-    for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + tid; i < rows * a.H * pieces; i += step) {
-      const int64_t k = i / (a.H * pieces), rest = i - k * a.H * pieces;
-      const int64_t row = k < hi ? k : lo + (k - hi), at = row * a.H + rest / pieces;
-      if (a.fill_tail) reinterpret_cast<uint4*>(a.out + at * a.dv)[rest % pieces] = make_uint4(0, 0, 0, 0);
-      if (a.lse && rest % pieces == 0) a.lse[at] = -INFINITY;
+    auto fill = [&](int64_t lo, int64_t hi) {
+      const int64_t all = (hi - lo) * a.H * pieces;
+      for (int64_t i = cta * kThreads + tid; i < all; i += ctas * kThreads) {
+        const int64_t at = lo * a.H + i / pieces;
+        const int piece = (int)(i % pieces);
+        if (a.fill_tail) reinterpret_cast<uint4*>(a.out + at * a.dv)[piece] = make_uint4(0, 0, 0, 0);
+        if (a.lse && piece == 0) a.lse[at] = -INFINITY;
+      }
+    };
+    if (!disorder) {
+      fill(0, a.B ? a.q_starts[0] : 0);
+      fill(a.B ? a.q_starts[a.B] : 0, a.Tq);
+    } else {
+      // what lies between the requests that keep their queries
+      int top = 0, done = 0;
+      for (int r0 = 0; r0 < a.B; r0 += 32) {
+        Bounds b{};
+        if (r0 + lane < a.B) b = bounds_of(a, r0 + lane);
+        const bool keeps = keeps_queries(a, b, top);
+        for (uint32_t left = __ballot_sync(0xffffffffu, keeps); left; left &= left - 1) {
+          const int src = __ffs(left) - 1;
+          const int q0 = __shfl_sync(0xffffffffu, (int)b.q0, src), nq = __shfl_sync(0xffffffffu, (int)b.nq, src);
+          fill(done, q0);
+          done = q0 + nq;
+        }
+      }
+      fill(done, a.Tq);
     }
   }
   if (tid == 0 && bars->abort_flag) report(a.status, a.status_host, kStatusWaitTimeout);

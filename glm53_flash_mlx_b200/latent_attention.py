@@ -379,7 +379,9 @@ def latent_attention_expanded(q_nope: torch.Tensor, q_rope: torch.Tensor | None,
     Returns ``out`` [queries, heads, value], whose flattened rows are the output
     projection's input, and with ``return_lse`` the FP32 log-sum-exp
     [queries, heads]; rows without keys and rows outside every request as in
-    ``latent_attention_absorbed``.
+    ``latent_attention_absorbed``.  Starts that descend or leave the rows set the
+    status word: a request between such key starts has no keys; one between such
+    query starts, or that begins before a start ahead of its own, has no queries.
     """
     code = _dtype(q_nope, "q_nope")
     if q_nope.dim() != 3 or q_nope.shape[1] < 1:

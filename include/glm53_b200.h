@@ -789,9 +789,10 @@ int glm53_latent_absorbed(const void* q_latent, int64_t ql_stride_t, int64_t ql_
  * it) and lse FP32 [query_tokens, heads], contiguous; rows that see no key and
  * rows outside every request as in glm53_latent_absorbed.  nope_dim, value_dim
  * multiples of 64, rope_dim 0 or 64, nope_dim + rope_dim and value_dim at most
- * 256.  Starts that descend or leave the rows set GLM53_STATUS_BAD_GEOMETRY:
- * such a request has no keys, or no queries (what its rows of out hold is not
- * defined). */
+ * 256.  Starts that descend or leave the rows set GLM53_STATUS_BAD_GEOMETRY.
+ * A request with such key starts has no keys.  One with such query starts, or
+ * that begins before a start ahead of its own, has no queries: rows of no other
+ * request are rows outside every request. */
 int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, int64_t qn_stride_h, const void* q_rope,
                           int64_t qr_stride_t, int64_t qr_stride_h, const void* k_nope, int64_t kn_stride_t,
                           int64_t kn_stride_h, const void* k_rope, int64_t kr_stride_t, const void* values,

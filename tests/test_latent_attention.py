@@ -819,6 +819,67 @@ def test_expanded_rows_outside_every_request():
     assert torch.equal(got[:40], want[:40]) and (got[40:] == 0).all()
 
 
+def rows_of_requests(starts, rows):
+    """Which request each row belongs to (-1: none), whatever the starts hold."""
+    owner, top = [-1] * rows, 0
+    for i, (a, b) in enumerate(zip(starts, starts[1:])):
+        if 0 <= a <= rows:
+            top = max(top, a)
+        if top <= a <= b <= rows:
+            owner[a:b] = [i] * (b - a)
+    return owner
+
+
+OUT_OF_ORDER = [  # starts, rows
+    ([0, 5, 8], 6), ([0, 50, 30], 50), ([0, 40, 0, 40], 40), ([0, 40, 0, 40, 0, 40], 40), ([0, 10, 50, 30, 35, 40], 40),
+    ([-1, 1, 2, 3, 4, 5], 40), ([0, 10, 20, 30, 40, 41], 40), ([40, 30, 20, 10, 5, 0], 40), ([0, 300, 100, 310, 305, 520], 530),
+    ([7, 20, 900, 15, 25, -4, 30, 300], 400), ([2 ** 31 - 1, -2 ** 31, 3, 9], 12), ([0, 2 ** 31 - 1, 0, 5], 9),
+    ([0, 500, 200, 600, 1000], 1100), ([3 * (i % 40) + i // 7 for i in range(260)], 150)]
+
+
+def test_rows_of_requests():
+    assert rows_of_requests([0, 2, 2, 5], 6) == [0, 0, 2, 2, 2, -1]
+    assert rows_of_requests([0, 5, 8], 6) == [0] * 5 + [-1]
+    assert rows_of_requests([0, 4, 0, 4], 4) == [0] * 4
+    assert rows_of_requests([3, 9, 1, 4, 6], 8) == [-1] * 3 + [2] * 0 + [-1] + [3] * 2 + [-1] * 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case,keys,H", [(c, k, 2) for c in range(len(OUT_OF_ORDER)) for k in (30, 300, 2300)] +
+                         [(0, 4000, 64), (2, 4000, 64)])
+def test_expanded_starts_out_of_order(case, keys, H):
+    """Every row is written by one request or counts as a row outside every request, with CTAs that walk, that take a
+    unit each and that work in pairs."""
+    import glm53_flash_mlx_b200 as G
+
+    starts, rows = OUT_OF_ORDER[case]
+    B, i32 = len(starts) - 1, torch.int32
+    if B > 100:
+        keys //= 10
+    qn, qr, kn, kr, v, _, ks = make_expanded([rows] + [0] * (B - 1), [keys] * B, H, 128, 64, 128, torch.bfloat16, case)
+    bad = torch.tensor(starts, dtype=torch.int64).to(i32).cuda()
+    owner = torch.tensor(rows_of_requests(starts, rows), device="cuda")
+    stale(rows, H)
+    out, lse = G.latent_attention_expanded(qn, qr, kn, kr, v, bad, ks, scale=0.07, return_lse=True)
+    with pytest.raises(RuntimeError):
+        G.check_latent_status()
+    none = owner < 0
+    assert (out[none] == 0).all() and (lse[none] == -math.inf).all()
+    kept = sorted(set(owner[~none].tolist()))
+    # the same requests in order, their rows gathered; each keeps its own keys
+    own = [int((owner == i).sum()) for i in kept]
+    if kept:
+        take = lambda x: x[~none]
+        got = expanded64(take(qn), take(qr), *(torch.cat([x[i * keys:(i + 1) * keys] for i in kept]) for x in (kn, kr, v)),
+                         own, [keys] * len(kept), 0.07, True, torch.bfloat16)
+        check(out[~none], lse[~none], *got)
+    given = torch.full_like(out, 3.0)
+    _, again = G.latent_attention_expanded(qn, qr, kn, kr, v, bad, ks, scale=0.07, out=given, return_lse=True)
+    with pytest.raises(RuntimeError):
+        G.check_latent_status()
+    assert (given[none] == 3).all() and torch.equal(given[~none], out[~none]) and torch.equal(again, lse)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("nk", [[60, 30], [4500, 30]])  # CTAs alone, CTA pairs
 def test_expanded_log_sums_behind_the_last_query_of_a_given_result(nk):
