@@ -696,12 +696,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float sub = m == -INFINITY ? 0.f : m;
       uint32_t w[32];
+      float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         const float p0 = ex2(fmaf(v[2 * i], a.c, -sub)), p1 = ex2(fmaf(v[2 * i + 1], a.c, -sub));
-        l += p0 + p1;
+        sum += p0 + p1;
         w[i] = Elem<E>::pack(p0, p1);
       }
+      // A tile's weights are added up before they meet the running sum: one by
+      // one, small ones would be rounded against a large one thousands of times
+      // (30,000 keys, all but one 17.5 nats below the first: 3.8e-4 off the log-sum).
+      l += sum;
       tmem_st32(tmem + lanes + kSCol + b * kTile + half * 32, w);
       tmem_wait_st();
       tmem_fence_before();

@@ -901,6 +901,29 @@ def test_expanded_log_sums_behind_the_last_query_of_a_given_result(nk):
     G.check_latent_status()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 130, 200])
+@pytest.mark.parametrize("nats", [17.5, 16.0, 14.0])
+def test_expanded_sums_many_small_weights(nats, nq):
+    """One key far above 30,000 others, which together make up to 2% of the sum.  The log-sum's error: a tile's 32
+    additions and those of 235 tiles, half a step of 2^-23 each, 1.6e-5; the score's and the exponential's steps, 2^-18;
+    one rounding."""
+    import glm53_flash_mlx_b200 as G
+
+    n, dt = 30000, torch.bfloat16
+    k = torch.zeros((n, 2, 64), dtype=dt, device="cuda")
+    k[0, :, 0] = nats
+    q = torch.zeros((nq, 2, 64), dtype=dt, device="cuda")
+    q[..., 0] = 1
+    starts = [torch.tensor([0, m], dtype=torch.int32, device="cuda") for m in (nq, n)]
+    for dv in (64, 128):  # CTAs alone, CTA pairs
+        v = torch.zeros((n, 2, dv), dtype=dt, device="cuda")
+        _, lse = G.latent_attention_expanded(q, None, k, None, v, *starts, scale=1.0, causal=False, return_lse=True)
+        G.check_latent_status()
+        want = nats + math.log1p((n - 1) * math.exp(-nats))
+        assert ((lse.double() - want).abs() <= 1.6e-5 + 2.0 ** -18 + want * 2.0 ** -24).all(), float((lse - want).abs().max())
+
+
 # --- streams, graphs, together ---------------------------------------------
 
 
