@@ -2,6 +2,8 @@
 // types, fail-closed status reports and shape limits.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace glm53 {
@@ -104,6 +106,12 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
 // the one in use by this much, in powers of two: weights stay below 2^8, which
 // every type here holds, and most tiles rescale nothing.
 constexpr float kMaxSlack = 8.0f;
+// FP16 weights are held times 2^7, that is relative to the maximum less 7: 2^15
+// at most, which FP16 holds, and what is below 2^-32 of the largest is lost, not
+// what is below 2^-25 (keys 17.5 nats under one of their tile all vanished from
+// the result, but not from its divisor).  BF16 has the exponents of FP32.
+template <typename E>
+constexpr float kWeightShift = std::is_same<E, __half>::value ? 7.0f : 0.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

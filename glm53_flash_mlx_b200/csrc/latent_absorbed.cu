@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)(strip * 32) << 16;
     bool stop = false;
     for (int segment = 0; !stop && next_segment(a, cur, sg); ++segment) {
-      float m[kOwn], l[kOwn];
+      float m[kOwn], l[kOwn];  // m: the maximum in use less kWeightShift, from which weights are counted
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
         m[i] = -INFINITY;
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < kOwn; ++i) {
             const int e = (i >> 1) * 4 + (i & 1);
-            grow |= fmaxf(v[e], v[e + 2]) > m[i] + kMaxSlack;
+            grow |= fmaxf(v[e], v[e + 2]) > m[i] + (kMaxSlack + kWeightShift<E>);
           }
           if (valid < kKeys) {
             // clear the value rows that the last MMA step takes beyond the end
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < kOwn; ++i) {
             const int h = 8 * (i >> 1) + h0 + (i & 1);
             const float top = fmaxf(m[i], fmaxf(fmaxf(bars->xchg[0][h], bars->xchg[1][h]),
-                                                fmaxf(bars->xchg[2][h], bars->xchg[3][h])));
+                                                fmaxf(bars->xchg[2][h], bars->xchg[3][h])) - kWeightShift<E>);
             const float f = top == m[i] ? 1.f : ex2(m[i] - top);
             m[i] = top;
             l[i] *= f;

@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       vis = j0 + r < u.nq ? u.seen(a, j0 + r) : 0;
       vis0 = u.seen(a, j0);
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;  // m: the maximum in use less kWeightShift, from which weights are counted
     if (tiles > 0) ++units;
     for (int t = 0; t < tiles; ++t) {
       const uint32_t v_ = g + t, b = v_ & 1;
@@ -667,13 +667,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 1; i < 64; ++i) top = fmaxf(top, v[i]);
       top *= a.c;
       // also orders every read of S before the stores of P into its columns
-      const bool grow = any_of(stop || top > m + kMaxSlack, 1, kSoftThreads);
+      const bool grow = any_of(stop || top > m + (kMaxSlack + kWeightShift<E>), 1, kSoftThreads);
       if (grow) {
         stop = any_of(stop, 1, kSoftThreads);
         if (stop) break;
         xchg[half * kTile + r] = top;
         bar_sync(1, kSoftThreads);
-        top = fmaxf(m, fmaxf(xchg[r], xchg[kTile + r]));
+        top = fmaxf(m, fmaxf(xchg[r], xchg[kTile + r]) - kWeightShift<E>);
         bar_sync(1, kSoftThreads);
         const float f = top == m ? 1.f : ex2(m - top);
         m = top;

@@ -924,6 +924,63 @@ def test_expanded_sums_many_small_weights(nats, nq):
         assert ((lse.double() - want).abs() <= 1.6e-5 + 2.0 ** -18 + want * 2.0 ** -24).all(), float((lse - want).abs().max())
 
 
+# --- weights far below the largest -----------------------------------------
+
+
+def small_weights(n, nats, width, dtype):
+    """n keys of `width` values: the first scores `nats` above all others (q = 1 in the first place, scale 1) and has
+    the values 0, the others 1 in places 8 and up; and what softmax gives there, with the tolerance of one rounding of
+    the result and of each weight.  An FP16 weight is held to 2^-25 where the largest is 2^7 or more: off by 2^-32 of
+    the largest."""
+    k = torch.zeros((n, width), dtype=dtype, device="cuda")
+    k[0, 0] = nats
+    k[1:, 8:] = 1
+    others = (n - 1) * math.exp(-nats)
+    want = others / (1 + others)
+    u = torch.finfo(dtype).eps / 2
+    tol = want * (2 * u + 2.0 ** -18) + (n * 2.0 ** -32 if dtype == torch.float16 else 0)
+    return k, want, math.log1p(others) + nats, tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,n,nats", [(1, 100003, 17.5), (160, 3000, 17.5), (160, 3000, 12.0), (160, 200, 14.0)])
+def test_absorbed_small_weights_count(dtype, B, n, nats):
+    """In parts that are joined, and with all of a request's keys in one unit."""
+    import glm53_flash_mlx_b200 as G
+
+    k, want, lse64, tol = small_weights(n, nats, 576, dtype)
+    pages = -(-n // 64)
+    cache = torch.full((pages, 64, 576), math.nan, dtype=dtype, device="cuda")
+    cache.view(-1, 576)[:n] = k
+    q = torch.zeros((B, 16, 576), dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    table = torch.arange(pages, device="cuda").int().repeat(B, 1)
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    out, lse = G.latent_attention_absorbed(q[..., :512], q[..., 512:], cache, table, lens, scale=1.0, return_lse=True)
+    G.check_latent_status()
+    assert ((out[..., 8:].double() - want).abs() <= tol).all(), (float(out[0, 0, 8]), want)
+    assert ((lse.double() - lse64).abs() <= 2.0 ** -18 * (1 + lse64)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nq", [1, 130, 200])
+@pytest.mark.parametrize("n,nats", [(30000, 17.5), (30000, 16.0), (3000, 12.0), (300, 14.0)])
+def test_expanded_small_weights_count(dtype, n, nats, nq):
+    import glm53_flash_mlx_b200 as G
+
+    k, want, lse64, tol = small_weights(n, nats, 128, dtype)
+    q = torch.zeros((nq, 2, 128), dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    v = k[:, None].expand(n, 2, 128)
+    starts = [torch.tensor([0, m], dtype=torch.int32, device="cuda") for m in (nq, n)]
+    out, lse = G.latent_attention_expanded(q, None, v, None, v, *starts, scale=1.0, causal=False, return_lse=True)
+    G.check_latent_status()
+    assert ((out[..., 8:].double() - want).abs() <= tol).all(), (float(out[0, 0, 8]), want)
+    assert ((lse.double() - lse64).abs() <= 2.0 ** -18 * (1 + lse64)).all()
+
+
 # --- streams, graphs, together ---------------------------------------------
 
 
