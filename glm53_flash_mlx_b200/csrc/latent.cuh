@@ -112,6 +112,9 @@ constexpr float kMaxSlack = 8.0f;
 // the result, but not from its divisor).  BF16 has the exponents of FP32.
 template <typename E>
 constexpr float kWeightShift = std::is_same<E, __half>::value ? 7.0f : 0.0f;
+// A row whose scores are all -inf has no weight anywhere: 0, as one that sees no key.
+__device__ __forceinline__ float inverse_sum(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (tid < N) {
         const float sum = (bars->xchg[0][tid] + bars->xchg[1][tid]) + (bars->xchg[2][tid] + bars->xchg[3][tid]);
         const float top = bars->top[tid];
-        bars->factor[tid] = 1.f / sum;
+        bars->factor[tid] = inverse_sum(sum);
         if (!whole) {
           a.pm[slot * N + tid] = top;
           a.pl[slot * N + tid] = sum;
@@ -754,7 +754,7 @@ __device__ __forceinline__ float2 part_weights(const Args& a, const Parts& q, in
     sum = fmaf(l[k], w, sum);
   }
   sum = warp_sum(sum);
-  return make_float2(1.f / sum, (base + log2f(sum)) * kLn2);
+  return make_float2(inverse_sum(sum), (base + log2f(sum)) * kLn2);
 }
 
 __device__ __forceinline__ void add_part(float4& o, float w, const float4& x) {

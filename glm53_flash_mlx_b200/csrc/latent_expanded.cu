@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_sync(1, kSoftThreads);
       l = xchg[r] + xchg[kTile + r];
       const bool poison = tiles > 0 && bars->poison[units & 1] == units;
-      const float inv = 1.f / l;
+      const float inv = inverse_sum(l);
       const bool mine = j0 + r < u.nq;
       const int64_t at = (int64_t)(u.q0 + j0 + r) * a.H + u.head;
       if (mine && a.lse && half == 0)

@@ -310,9 +310,10 @@ def latent_attention_absorbed(q_latent: torch.Tensor, q_rope: torch.Tensor | Non
     [requests].  ``query_starts`` int32 [requests + 1] bounds each request's
     tokens (None: one each); the last one sees every row, each earlier one a row
     less.  Returns ``out`` [tokens, heads, latent] and, with ``return_lse``, the
-    FP32 log-sum-exp [tokens, heads].  A token that sees no row gives 0 and
-    -inf.  Tokens behind ``query_starts[-1]`` give 0 in a new result, are left
-    as they were in a given ``out``, and have the log-sum-exp -inf.
+    FP32 log-sum-exp [tokens, heads].  A token that sees no row, or whose scores
+    are all -inf, gives 0 and -inf.  Tokens behind ``query_starts[-1]`` give 0 in
+    a new result, are left as they were in a given ``out``, and have the
+    log-sum-exp -inf.
     """
     code = _dtype(q_latent, "q_latent")
     if q_latent.dim() != 3 or q_latent.shape[1] < 1:

@@ -764,11 +764,11 @@ int glm53_latent_cache_write(const void* kv, int64_t tokens, int64_t kv_stride, 
  * 384 or 512; rope_dim 0 or 64; page_size a multiple of 8.  query_starts int32
  * [requests + 1] gives each request's tokens (NULL: one each); the last of a
  * request's tokens sees all seq_lens rows, each earlier one a row less.  A
- * token that sees no row gives 0 and lse -inf.  Tokens outside every request
- * (behind query_starts[requests]) give lse -inf; their rows of out are zeroed
- * when fill_tail is set, else left as they were.  out overlaps no input.  The
- * workspace (256-byte aligned, contents of no account) belongs to one call at a
- * time.  A page id outside the cache sets GLM53_STATUS_BAD_PAGE and its rows
+ * token that sees no row, or whose scores are all -inf, gives 0 and lse -inf.
+ * Tokens outside every request (behind query_starts[requests]) give lse -inf;
+ * their rows of out are zeroed when fill_tail is set, else left as they were.
+ * out overlaps no input.  The workspace (256-byte aligned, contents of no
+ * account) belongs to one call at a time.  A page id outside the cache sets GLM53_STATUS_BAD_PAGE and its rows
  * read as zeros; a length outside the table sets GLM53_STATUS_BAD_GEOMETRY and
  * counts as 0; starts that descend or leave the tokens set
  * GLM53_STATUS_BAD_GEOMETRY and bound no token of any request. */

@@ -981,6 +981,69 @@ def test_expanded_small_weights_count(dtype, n, nats, nq):
     assert ((lse.double() - lse64).abs() <= 2.0 ** -18 * (1 + lse64)).all()
 
 
+# --- rows without weight, rows that are not finite -------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 5000])  # one unit, parts that are joined
+def test_absorbed_scores_of_minus_infinity(n):
+    """A key whose score is -inf has no weight; a token whose keys all have such scores gives 0 and -inf, as one
+    that sees no key."""
+    import glm53_flash_mlx_b200 as G
+
+    for lost in (n, n - 1, 3):  # the first `lost` keys
+        ql, qr, cache, table, lens, _, rows = make_absorbed([n], [1], 16, 512, 64, 16, torch.bfloat16, n)
+        qr[..., 7] = 0.5
+        at = torch.arange(n, device="cuda")
+        rows[0][:lost, 512 + 7] = -math.inf
+        cache.view(-1, 576)[table[0].long()[at // 16] * 16 + at % 16] = rows[0]
+        out, lse = G.latent_attention_absorbed(ql, qr, cache, table, lens, scale=0.05, return_lse=True)
+        G.check_latent_status()
+        if lost == n:
+            assert (out == 0).all() and (lse == -math.inf).all()
+        else:
+            check(out, lse, *absorbed64(ql, qr, [rows[0][lost:]], [n - lost], [1], 0.05, torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,n", [(3, 5), (200, 300), (150, 4500)])
+def test_expanded_scores_of_minus_infinity(nq, n):
+    import glm53_flash_mlx_b200 as G
+
+    for lost in (n, 2, n - nq + 1):  # with the last, the first query sees keys without weight alone
+        qn, qr, kn, kr, v, qs, ks = make_expanded([nq], [n], 2, 128, 64, 128, torch.bfloat16, n)
+        qr, kr = qr.clone(), kr.clone()
+        qr[..., 7] = 0.5
+        kr[:lost, 7] = -math.inf
+        out, lse = G.latent_attention_expanded(qn, qr, kn, kr, v, qs, ks, scale=0.05, return_lse=True)
+        G.check_latent_status()
+        none = torch.arange(nq, device="cuda") + (n - nq) + 1 <= lost
+        assert (out[none] == 0).all() and (lse[none] == -math.inf).all()
+        if lost < n:
+            check(out, lse, *expanded64(qn, qr, kn[lost:], kr[lost:], v[lost:], [nq], [n - lost], 0.05, True, torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_absorbed_seen_rows_that_are_not_finite(what):
+    """Only the tokens that see such a row get it, through its score (NaN) or its value."""
+    import glm53_flash_mlx_b200 as G
+
+    lens, queries, H = [3000, 700, 40], [1, 3, 1], 16
+    ql, qr, cache, table, n, starts, rows = make_absorbed(lens, queries, H, 512, 64, 16, torch.bfloat16, 21)
+    ql.fill_(0.25)
+    call = lambda: G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05, query_starts=starts, return_lse=True)
+    clean, lse = call()
+    at = 698  # of the second request: its tokens see 698, 699 and 700 rows
+    cache.view(-1, 576)[int(table[1, at // 16]) * 16 + at % 16, 77] = what
+    got, again = call()
+    G.check_latent_status()
+    seen = torch.tensor([False, False, True, True, False], device="cuda")
+    # an infinite score takes all weight, and inf - inf in the exponent is NaN, in 64 bits as here
+    assert got[seen].isnan().all() and again[seen].isnan().all()
+    assert torch.equal(got[~seen], clean[~seen]) and torch.equal(again[~seen], lse[~seen])
+
+
 # --- streams, graphs, together ---------------------------------------------
 
 
