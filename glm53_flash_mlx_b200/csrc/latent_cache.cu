@@ -455,9 +455,10 @@ extern "C" int glm53_latent_cache_write(const void* kv, int64_t tokens, int64_t 
     set_last_error("%s: positions and inv_freq come together, with a rotary part", fn);
     return GLM53_ERR_INVALID;
   }
-  if (queries && (!positions || !queries_out || heads < 1 || heads > 4096 || q_stride_h < rope_dim ||
+  if (queries && (!positions || !queries_out || heads < 1 || heads > 4096 || q_stride_h < 0 ||
                   q_stride_t < 0 || q_stride_h % 8 != 0 || q_stride_t % 8 != 0)) {
-    set_last_error("%s: queries need positions, an output, 1 to 4096 heads and strides that are multiples of 8", fn);
+    set_last_error("%s: queries need positions, an output, 1 to 4096 heads and strides that are multiples of 8 from 0 on",
+                   fn);
     return GLM53_ERR_INVALID;
   }
   if (tokens == 0) return GLM53_OK;

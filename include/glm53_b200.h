@@ -749,7 +749,9 @@ int glm53_plan_pages(const int32_t* cached_lens, const int32_t* new_lens, int64_
  * skips the token, >= cache_rows sets GLM53_STATUS_BAD_PAGE and skips it.  Two
  * tokens with one slot leave either row.  kv and queries overlap neither the
  * cache nor queries_out.  queries (optional)
- * [tokens, heads, rope_dim]: turned likewise into queries_out (contiguous). */
+ * [tokens, heads, rope_dim], whose tokens and heads may overlap or repeat
+ * (strides are multiples of 8, 0 among them): turned likewise into queries_out
+ * (contiguous). */
 int glm53_latent_cache_write(const void* kv, int64_t tokens, int64_t kv_stride, int64_t latent_dim, int64_t rope_dim,
                              int dtype, const void* norm_weight, float eps, const int32_t* positions,
                              const double* inv_freq, int interleaved, const int64_t* slots, void* cache,

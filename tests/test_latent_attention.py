@@ -422,6 +422,23 @@ def test_write_refuses_rows_of_the_cache():
     G.check_latent_status()
 
 
+@pytest.mark.gpu
+def test_write_reads_queries_that_overlap():
+    import glm53_flash_mlx_b200 as G
+
+    dev, dt = "cuda", torch.bfloat16
+    run = torch.randn(1000, device=dev).to(dt)
+    pos = torch.arange(3, dtype=torch.int32, device=dev)
+    freq = torch.rand(32, dtype=torch.float64, device=dev)
+    for strides in ((200, 8, 1), (0, 64, 1), (200, 0, 1), (8, 16, 1), (7, 5, 1), (200, 64, 2)):
+        q = run.as_strided((3, 5, 64), strides)
+        cache = torch.zeros((1, 16, 576), dtype=dt, device=dev)
+        got = G.latent_cache_write(torch.ones((3, 576), dtype=dt, device=dev), cache, torch.arange(3, device=dev),
+                                   positions=pos, inv_freq=freq, queries=q)
+        G.check_latent_status()
+        rounded_close(got, turn64(q, pos, freq, False), 8.0)
+
+
 # --- absorbed form ---------------------------------------------------------
 
 
