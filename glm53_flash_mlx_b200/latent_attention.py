@@ -240,11 +240,10 @@ def latent_cache_write(kv: torch.Tensor, cache: torch.Tensor, slots: torch.Tenso
     as given), pairing value i with i + rope_dim / 2, or neighbours when
     ``interleaved``.  Unlike ``rms_norm`` the row is rounded once, at its store.
     ``cache`` [pages, page_size, latent + rope] is contiguous; ``slots`` int64
-    [tokens] (``PagePlan.slots``): a negative slot stores nothing; slots are
-    distinct (of two tokens with one slot either row stays).  ``kv`` and ``queries`` lie
-    outside the cache.  ``queries``
-    [tokens, heads, rope_dim] are rotated likewise into a new tensor, which is
-    returned (None without queries).
+    [tokens] (``PagePlan.slots``): a negative slot stores nothing, the others are
+    distinct (a row that two tokens name can end with pieces of both).  ``kv`` and
+    ``queries`` lie outside the cache.  ``queries`` [tokens, heads, rope_dim] are
+    rotated likewise into a new tensor, which is returned (None without queries).
     """
     code = _dtype(kv, "kv")
     if kv.dim() != 2 or not 0 <= rope_dim < kv.shape[1]:

@@ -746,9 +746,9 @@ int glm53_plan_pages(const int32_t* cached_lens, const int32_t* new_lens, int64_
  * given; inv_freq is FP64 [rope_dim / 2], pairs (i, i + rope_dim / 2), or
  * (2 i, 2 i + 1) when interleaved), computed in FP32 and rounded once.
  * kv [tokens, latent_dim + rope_dim], rows kv_stride apart; slots int64: < 0
- * skips the token, >= cache_rows sets GLM53_STATUS_BAD_PAGE and skips it.  Two
- * tokens with one slot leave either row.  kv and queries overlap neither the
- * cache nor queries_out.  queries (optional)
+ * skips the token, >= cache_rows sets GLM53_STATUS_BAD_PAGE and skips it.  The
+ * others are distinct: a row that two tokens name can end with pieces of both.
+ * kv and queries overlap neither the cache nor queries_out.  queries (optional)
  * [tokens, heads, rope_dim], whose tokens and heads may overlap or repeat
  * (strides are multiples of 8, 0 among them): turned likewise into queries_out
  * (contiguous). */

@@ -439,6 +439,25 @@ def test_write_reads_queries_that_overlap():
         rounded_close(got, turn64(q, pos, freq, False), 8.0)
 
 
+@pytest.mark.gpu
+def test_write_of_one_slot_twice_leaves_the_other_rows():
+    """What a row holds that two tokens name is not defined; equal tokens give their row, and all other rows are right."""
+    import glm53_flash_mlx_b200 as G
+
+    kv = torch.randn((300, 576), device="cuda").to(torch.bfloat16)
+    kv[200:250] = kv[100:150]
+    slots = torch.randperm(400, device="cuda")[:300]
+    slots[200:250] = slots[100:150]  # the same rows twice
+    slots[250:300] = slots[0]        # different rows in one slot
+    cache = torch.full((25, 16, 576), 5.0, dtype=torch.bfloat16, device="cuda")
+    G.latent_cache_write(kv, cache, slots)
+    G.check_latent_status()
+    want = torch.full((400, 576), 5.0, dtype=torch.bfloat16, device="cuda")
+    want[slots[1:200]] = kv[1:200]
+    rest = torch.arange(400, device="cuda") != slots[0]
+    assert torch.equal(cache.view(400, 576)[rest], want[rest])
+
+
 # --- absorbed form ---------------------------------------------------------
 
 
