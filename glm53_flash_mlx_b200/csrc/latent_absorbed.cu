@@ -167,18 +167,20 @@ __device__ __forceinline__ bool next_segment(const Args& a, Cursor& c, Segment& 
   return false;
 }
 
-struct __align__(8) Bars {
+struct Bars {
   uint64_t q_full, q_empty, full[2][2], empty[2][2], s_full[2], p_full[2], o_done, drain[2];
   uint32_t tmem_base;
   int abort_flag;
   Cursor cursor;
   int warp_sum[kThreads / 32];
-  float factor[kMaxHeads], top[kMaxHeads];
+  alignas(16) float factor[kMaxHeads];  // read four at a time
+  float top[kMaxHeads];
   float xchg[4][kMaxHeads];
 };
 // alignment slack, Q, two stages, P^T, barriers
 constexpr size_t kSmemBytes = 1024 + 3 * (size_t)kStageBytes + kChunkBytes + 2048;
 static_assert(sizeof(Bars) <= 2048, "barriers share two KB");
+static_assert((3 * kStageBytes + kChunkBytes) % alignof(Bars) == 0, "where the barriers lie, behind P^T");
 static_assert(kSmemBytes <= 232448, "227 KB a CTA");
 
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
