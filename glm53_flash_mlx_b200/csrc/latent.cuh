@@ -12,10 +12,6 @@ namespace latent {
 constexpr uint32_t kStatusBadPage = 1u << 3;  // a page id or slot outside the cache
 constexpr uint32_t kStatusNoPages = 1u << 4;  // a page plan that does not fit its pages, table or token capacity
 
-// Element type codes of the C ABI (GLM53_DTYPE_*).
-constexpr int kBf16 = 0;
-constexpr int kFp16 = 1;
-
 // OR a bit into the device status word and, where given, store the word in
 // the pinned host mirror: the success path needs no mirror launch.
 __device__ __forceinline__ void report(uint32_t* status, uint32_t* host, uint32_t bit) {
