@@ -1080,6 +1080,169 @@ def test_absorbed_seen_rows_that_are_not_finite(what):
     assert torch.equal(got[~seen], clean[~seen]) and torch.equal(again[~seen], lse[~seen])
 
 
+# --- how far results may be off on average, and counted keys ----------------
+
+
+def check_average(got, lse, q, k, v, visible, scale, dtype):
+    """One head's rows by their mean error.  q [n, d], k [m, d], v [m, dv], visible [n] keys each.
+
+    Each weight's rounding is at most u of it and independent of the others, so the mean square over a row's values is
+    at most u^2 sum p^2 v^2, and u^2 o^2 for the result's own (uniform errors make a third of that, which leaves room
+    for the mean over as few as 64 values).  Scores: a product of d values is added up in steps of 16, each cut off at
+    2^-23 of what has been added so far, below 4 standard deviations of the sum, sigma = scale sqrt(sum (q k)^2):
+    e = d / 16 2^-23 4 sigma, independent from key to key.  FP16: weights are held to 2^-32 of the largest, results to
+    2^-25.  Log-sums: at most the largest e, 2^-18 as above and one FP32 rounding of each of two factors."""
+    u = torch.finfo(dtype).eps / 2
+    q, k, v, got = q.double(), k.double(), v.double(), got.double()
+    seen = torch.arange(k.shape[0], device=q.device)[None, :] < visible[:, None]
+    s = torch.where(seen, (q @ k.T) * scale, -math.inf)
+    log = torch.logsumexp(s, -1)
+    p = torch.exp(s - log[:, None])
+    out = p @ v
+    e = torch.where(seen, (q.square() @ k.square().T).sqrt() * abs(scale), 0).amax(-1) * (q.shape[1] / 16 * 4 * 2.0 ** -23)
+    square = (u * u + e[:, None] ** 2) * (p.square() @ v.square()) + (u * u + 2.0 ** -36) * out.square() + 1e-30
+    if dtype == torch.float16:
+        square = square + 2.0 ** -64 * p.amax(-1, keepdim=True) ** 2 * (seen.double() @ v.square()) + 2.0 ** -50
+    err = (got - out).square().mean(-1).sqrt()
+    tol = square.mean(-1).sqrt()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{int(bad.sum())} rows off, worst {float((err / tol).nan_to_num(nan=1e9).max()):.3f} x tolerance"
+    assert ((lse.double() - log).abs() <= e + 2.0 ** -18 + 2.0 ** -22 * log.abs()).all(), float((lse - log).abs().max())
+
+
+def rounded_weights(q, k, v, visible, scale, dtype, bits, drop=None):
+    """Attention in 64 bits whose weights are rounded to `bits` of mantissa, rounded once to `dtype`; key `drop` left out."""
+    s = (q.double() @ k.double().T) * scale
+    s = s.masked_fill(torch.arange(k.shape[0])[None, :] >= visible[:, None], -math.inf)
+    if drop is not None:
+        s[:, drop] = -math.inf
+    p = torch.exp(s - s.amax(-1, keepdim=True))
+    m, x = torch.frexp(p)
+    r = torch.ldexp(torch.round(m * 2.0 ** bits) / 2.0 ** bits, x)
+    return ((r @ v.double()) / p.sum(-1, keepdim=True)).to(dtype), torch.logsumexp(s, -1).float()
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 8), (torch.float16, 11)])
+@pytest.mark.parametrize("n", [1, 7, 777, 9000])
+def test_mean_errors_tell_coarser_weights(dtype, bits, n):
+    g = torch.Generator().manual_seed(n)
+    q, k = (torch.randn((x, 576), generator=g).to(dtype) for x in (6, n))
+    v, visible, scale = k[:, :512], torch.full((6,), n), 1.5 / 24
+    check_average(*rounded_weights(q, k, v, visible, scale, dtype, bits), q, k, v, visible, scale, dtype)
+    if n == 1:
+        return
+    with pytest.raises(AssertionError):  # three bits less, as of FP16 weights that are held as BF16
+        check_average(*rounded_weights(q, k, v, visible, scale, dtype, bits - 3), q, k, v, visible, scale, dtype)
+    with pytest.raises(AssertionError):
+        check_average(*rounded_weights(q, k, v, visible, scale, dtype, bits, drop=n // 2), q, k, v, visible, scale, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,queries,H,latent,rope,page", [
+    ([777], [1], 64, 512, 64, 64), ([9000], [1], 64, 512, 64, 64), ([40, 1, 3000, 500], [2, 1, 3, 1], 16, 512, 64, 16),
+    ([900] * 200, [1] * 200, 16, 512, 64, 64), ([1500, 70], [1, 1], 130, 128, 0, 32)])
+def test_absorbed_errors_on_average(dtype, lens, queries, H, latent, rope, page):
+    import glm53_flash_mlx_b200 as G
+
+    ql, qr, cache, table, n, starts, rows = make_absorbed(lens, queries, H, latent, rope, page, dtype, 31)
+    scale = (latent + rope) ** -0.5 * 1.5
+    out, lse = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=scale, query_starts=starts, return_lse=True)
+    G.check_latent_status()
+    t = 0
+    for m, nq, x in zip(lens, queries, rows):
+        for j in range(nq):
+            q = ql[t] if qr is None else torch.cat([ql[t], qr[t]], -1)
+            vis = torch.full((H,), m - (nq - 1 - j), device="cuda")
+            check_average(out[t], lse[t], q, x, x[:, :latent], vis, scale, dtype)
+            t += 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nq,nk,H,dn,dr,dv,causal", [
+    ([256], [256], 8, 192, 64, 256, True), ([129, 1, 127], [129, 640, 300], 2, 128, 64, 128, True),
+    ([513], [4500], 2, 192, 64, 256, True), ([100], [3000], 2, 192, 64, 256, False), ([70] * 40, [90] * 40, 3, 64, 0, 64, True)])
+def test_expanded_errors_on_average(dtype, nq, nk, H, dn, dr, dv, causal):
+    import glm53_flash_mlx_b200 as G
+
+    t = make_expanded(nq, nk, H, dn, dr, dv, dtype, 32)
+    scale = (dn + dr) ** -0.5 * 1.5
+    out, lse = G.latent_attention_expanded(*t, scale=scale, causal=causal, return_lse=True)
+    G.check_latent_status()
+    qn, qr, kn, kr, v = t[:5]
+    a = b = 0
+    for n, m in zip(nq, nk):
+        vis = torch.arange(n, device="cuda") + (m - n) + 1 if causal else torch.full((n,), m, device="cuda")
+        for h in range(H):
+            q, k = qn[a:a + n, h], kn[b:b + m, h]
+            if dr:
+                q, k = torch.cat([q, qr[a:a + n, h]], -1), torch.cat([k, kr[b:b + m]], -1)
+            check_average(out[a:a + n, h], lse[a:a + n, h], q, k, v[b:b + m, h], vis, scale, dtype)
+        a, b = a + n, b + m
+
+
+def check_counts(out, lse, visible):
+    """Queries of 0 give every key the weight 1, so with values that mark key j in place j mod dv each value is the
+    number of a place's keys over the number of all, both exact, in three roundings; a key lost or taken twice changes
+    its place by one in a few dozen and the log of the number of all by more than FP32's steps there."""
+    dv = out.shape[-1]
+    u = torch.finfo(out.dtype).eps / 2
+    vis = visible.double()[:, None]
+    counts = torch.div(visible[:, None] - torch.arange(dv, device=out.device) + dv - 1, dv, rounding_mode="floor").clamp(min=0)
+    want = (counts / vis.clamp(min=1))[:, None]
+    assert ((out.double() - want).abs() <= (u + 2.0 ** -22) * want).all()
+    some = visible > 0
+    assert (lse[~some] == -math.inf).all()
+    assert ((lse[some].double() - vis[some].log()).abs() <= 2.0 ** -20 + 2.0 ** -22 * vis[some].log()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,queries,H,page", [
+    ([30011], [1], 16, 64), ([100003], [1], 64, 64), ([1, 63, 64, 65, 30011, 4097, 0, 777], [1] * 8, 64, 64),
+    ([1, 63, 64, 65, 9011, 4097, 0, 777], [3, 2, 1, 4, 3, 3, 2, 1], 16, 16), ([5000 - 31 * i for i in range(150)], [1] * 150, 70, 8)])
+def test_absorbed_counts_every_key_once(dtype, lens, queries, H, page):
+    import glm53_flash_mlx_b200 as G
+
+    ql, qr, cache, table, n, starts, _ = make_absorbed([min(x, 1) for x in lens], queries, H, 512, 64, page, dtype, 33)
+    width = -(-max(lens) // page)
+    # all requests read the same rows, in pages out of order
+    cache = torch.full((width + 3, page, 576), math.nan, dtype=dtype, device="cuda")
+    ids = torch.randperm(width + 3, device="cuda")[:width]
+    at = torch.arange(max(lens), device="cuda")
+    rows = torch.zeros((max(lens), 576), dtype=dtype, device="cuda")
+    rows[at, at % 512] = 1
+    cache.view(-1, 576)[ids[at // page] * page + at % page] = rows
+    table = ids.int().repeat(len(lens), 1)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, lse = G.latent_attention_absorbed(torch.zeros_like(ql), torch.zeros_like(qr), cache, table, n, scale=1.0,
+                                           query_starts=starts, return_lse=True)
+    G.check_latent_status()
+    visible = [max(0, m - (nq - 1 - j)) for m, nq in zip(lens, queries) for j in range(nq)]
+    check_counts(out, lse, torch.tensor(visible, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("nq,nk,H,dv", [
+    ([300, 1, 129, 0, 5], [300, 9000, 2500, 7, 2], 3, 256), ([513], [9001], 2, 128), ([1], [20003], 2, 256),
+    ([128, 100], [2561, 7000], 2, 256), ([40, 130] * 80, [60, 140] * 80, 2, 64), ([300, 200], [299, 150], 2, 192)])
+def test_expanded_counts_every_key_once(dtype, causal, nq, nk, H, dv):
+    import glm53_flash_mlx_b200 as G
+
+    qn, qr, kn, kr, v, qs, ks = make_expanded(nq, nk, H, 128 if dv < 256 else 192, 64, dv, dtype, 34)
+    v = torch.zeros_like(v)
+    at = torch.cat([torch.arange(m, device="cuda") for m in nk])
+    v[torch.arange(sum(nk), device="cuda"), :, at % dv] = 1
+    out, lse = G.latent_attention_expanded(torch.zeros_like(qn), torch.zeros_like(qr), kn, kr, v, qs, ks, scale=1.0,
+                                           causal=causal, return_lse=True)
+    G.check_latent_status()
+    visible = [max(0, m - n + 1 + j) if causal else m for n, m in zip(nq, nk) for j in range(n)]
+    check_counts(out, lse, torch.tensor(visible, device="cuda"))
+
+
 # --- streams, graphs, together ---------------------------------------------
 
 
