@@ -1330,6 +1330,60 @@ def test_calls_at_once_on_several_streams():
 
 
 @pytest.mark.gpu
+def test_a_second_chunk_over_the_rows_in_the_cache():
+    """A prompt's next chunk attends over what is in the cache already: the keys' slots follow from the block table and
+    the lengths, and the expanded form over those rows gives each query what one call over the whole prompt gives."""
+    import glm53_flash_mlx_b200 as G
+    from glm53_flash_mlx_b200 import synthetic as S
+
+    dev, dt = torch.device("cuda", torch.cuda.current_device()), torch.bfloat16
+    g = torch.Generator(device=dev).manual_seed(41)
+    H, dn, dv, page, B = 4, 192, 256, 16, 3
+    first, second = [150, 1, 64], [37, 130, 1]
+    i32 = dict(dtype=torch.int32, device=dev)
+    table, count = torch.full((B, 14), -1, **i32), torch.tensor([30], **i32)
+    free = torch.randperm(30, generator=g, device=dev).int()
+    cache = torch.full((30, page, 576), math.nan, dtype=dt, device=dev)
+    freq = 10000.0 ** (-torch.arange(0, r, 2, device=dev, dtype=torch.float64) / r)
+    kvb, kvb_s = S.random_block_fp8(H * (dn + dv), R, seed=5, device=dev)
+    scale = (dn + r) ** -0.5
+
+    kept, outs, cached = [[] for _ in range(B)], [], torch.zeros(B, **i32)
+    for chunk in (first, second):
+        T = sum(chunk)
+        plan = G.plan_pages(cached, torch.tensor(chunk, **i32), table, free, count, page_size=page, tokens=T)
+        kv = torch.randn((T, 576), generator=g, device=dev).to(dt)
+        q = torch.randn((T, H, dn + r), generator=g, device=dev).to(dt)
+        q_rope = G.latent_cache_write(kv, cache, plan.slots, positions=plan.positions, inv_freq=freq, queries=q[..., dn:])
+        # the slots of all keys, cached and new
+        lens = plan.seq_lens.long()
+        keys = int(sum(first)) if chunk is first else sum(first) + sum(second)
+        key_starts = torch.cat([lens.new_zeros(1), lens.cumsum(0)])
+        request = torch.repeat_interleave(torch.arange(B, device=dev), lens, output_size=keys)
+        position = torch.arange(keys, device=dev) - key_starts[request]
+        key_slots = table[request, position // page].long() * page + position % page
+        rows = cache.view(-1, 576)[key_slots]
+        up = G.block_fp8_linear(rows[:, :R].contiguous(), kvb, kvb_s).view(keys, H, dn + dv)
+        out = G.latent_attention_expanded(q[..., :dn], q_rope, up[..., :dn], rows[:, R:], up[..., dn:], plan.query_starts,
+                                          key_starts.int(), scale=scale)
+        check(out, None, *expanded64(q[..., :dn], q_rope, up[..., :dn], rows[:, R:], up[..., dn:], chunk, lens.tolist(),
+                                     scale, True, dt))
+        at = 0
+        for i, n in enumerate(chunk):
+            kept[i].append((q[at:at + n, :, :dn], q_rope[at:at + n], out[at:at + n]))
+            at += n
+        cached, count = plan.seq_lens, plan.free_count
+    G.check_latent_status()
+    qn, qr, want = (torch.cat([torch.cat([c[j] for c in k]) for k in kept]) for j in range(3))
+    whole = G.latent_attention_expanded(qn, qr, up[..., :dn], rows[:, R:], up[..., dn:], key_starts.int(), key_starts.int(),
+                                        scale=scale)
+    # the same sums in another order of tiles: a rounding of the weights and one of the result on each side
+    err = (whole.double() - want.double()).square().mean(-1).sqrt()
+    size = want.double().square().mean(-1).sqrt()
+    assert (err <= 2 * 2 * 2.0 ** -8 * size + 1e-6).all(), float((err / size).max())
+
+
+@pytest.mark.gpu
 def test_a_prompt_and_its_decode_together():
     """Plan, store, expand and attend a ragged prompt batch, then decode a token each: both forms give the
     layer's attention, and the output projection reads the result."""
