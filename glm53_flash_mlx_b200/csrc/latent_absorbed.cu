@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < kOwn; ++i) {
             const int e = (i >> 1) * 4 + (i & 1);
-            grow |= fmaxf(v[e], v[e + 2]) > m[i] + (kMaxSlack + kWeightShift<E>);
+            grow |= fmaxf(v[e], v[e + 2]) - m[i] > kMaxSlack + kWeightShift<E>;
           }
           if (valid < kKeys) {
             // clear the value rows that the last MMA step takes beyond the end

@@ -665,13 +665,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       float top = v[0];
 #pragma unroll
       for (int i = 1; i < 64; ++i) top = fmaxf(top, v[i]);
-      top *= a.c;
+      // the largest exponent as it is formed below, whatever FP32 makes of m + slack;
       // also orders every read of S before the stores of P into its columns
-      const bool grow = any_of(stop || top > m + (kMaxSlack + kWeightShift<E>), 1, kSoftThreads);
+      const bool grow = any_of(stop || fmaf(top, a.c, -m) > kMaxSlack + kWeightShift<E>, 1, kSoftThreads);
       if (grow) {
         stop = any_of(stop, 1, kSoftThreads);
         if (stop) break;
-        xchg[half * kTile + r] = top;
+        xchg[half * kTile + r] = top * a.c;
         bar_sync(1, kSoftThreads);
         top = fmaxf(m, fmaxf(xchg[r], xchg[kTile + r]) - kWeightShift<E>);
         bar_sync(1, kSoftThreads);

@@ -1017,6 +1017,37 @@ def test_expanded_small_weights_count(dtype, n, nats, nq):
     assert ((lse.double() - lse64).abs() <= 2.0 ** -18 * (1 + lse64)).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("power", [20, 23, 24, 25, 26])
+def test_weights_of_large_scores_stay_in_range(dtype, power):
+    """Scores near 2^power in powers of two, where FP32 has steps of up to 8, later ones some steps above the first: no
+    weight leaves its type's range.  All values are 1, and so is their mean whatever the weights: the sum of n weights
+    rounded by u each, over their sum, rounded."""
+    import glm53_flash_mlx_b200 as G
+
+    u = torch.finfo(dtype).eps / 2
+    i32 = dict(dtype=torch.int32, device="cuda")
+    n, rises = 256, list(range(0, 41))
+    k = torch.zeros((len(rises), n, 576), dtype=dtype, device="cuda")
+    k[..., 0] = 2.0 ** (power - power // 2)
+    k[..., 8:] = 1
+    for i, x in enumerate(rises):
+        k[i, 128:, 1] = x  # the second 128 keys of each request
+    q = torch.zeros((len(rises), 16, 576), dtype=dtype, device="cuda")
+    q[..., 0], q[..., 1] = 2.0 ** (power // 2), 1
+    table = torch.arange(4 * len(rises), **i32).view(-1, 4)
+    lens = torch.full((len(rises),), n, **i32)
+    out = G.latent_attention_absorbed(q[..., :512], q[..., 512:], k.view(-1, 64, 576), table, lens, scale=math.log(2))
+    assert ((out[..., 8:].double() - 1).abs() <= 2 * u + 2.0 ** -18).all()
+    starts = torch.arange(len(rises) + 1, **i32)
+    flat = k.view(-1, 1, 576)
+    out = G.latent_attention_expanded(q[:, :1, :128], None, flat[..., :128], None, flat[..., 64:192], starts, starts * n,
+                                      scale=math.log(2))
+    assert ((out.double() - 1).abs() <= 2 * u + 2.0 ** -18).all()
+    G.check_latent_status()
+
+
 # --- rows without weight, rows that are not finite -------------------------
 
 
