@@ -287,10 +287,11 @@ def latent_cache_write(kv: torch.Tensor, cache: torch.Tensor, slots: torch.Tenso
     if T and (kp < end and kp + 2 * ((T - 1) * kt + width) > first or heads and qp < end
               and qp + 2 * ((T - 1) * qt + (heads - 1) * qh + rope_dim) > first):
         raise ValueError("kv and queries must lie outside the cache")
-    if not slots.is_contiguous():
-        slots = slots.contiguous()
-    _CACHE_WRITE(index, kp, T, kt if kt > width else width, latent, rope_dim, code, wp, eps, pp, fp,
-          interleaved, slots.data_ptr(), first, cache.shape[0] * cache.shape[1], qp, heads, qt, qh, rp)
+    if T:
+        if not slots.is_contiguous():
+            slots = slots.contiguous()
+        _CACHE_WRITE(index, kp, T, kt if kt > width else width, latent, rope_dim, code, wp, eps, pp, fp,
+              interleaved, slots.data_ptr(), first, cache.shape[0] * cache.shape[1], qp, heads, qt, qh, rp)
     return rotated
 
 

@@ -1361,6 +1361,90 @@ def test_calls_at_once_on_several_streams():
 
 
 @pytest.mark.gpu
+def test_batches_of_nothing():
+    """No requests, no tokens, no keys, no pages: every row counts as one outside every request or that sees nothing."""
+    import glm53_flash_mlx_b200 as G
+
+    dev, dt = "cuda", torch.bfloat16
+    i32 = dict(dtype=torch.int32, device=dev)
+    new = lambda *shape: torch.full(shape, 2.0, dtype=dt, device=dev)
+    none, start = torch.zeros(0, **i32), torch.zeros(1, **i32)
+    for T in (0, 5):
+        stale(5, 3)
+        out, lse = G.latent_attention_absorbed(new(T, 3, 512), new(T, 3, 64), new(2, 16, 576), torch.zeros((0, 4), **i32),
+                                               none, scale=1.0, query_starts=start, return_lse=True)
+        assert out.shape == (T, 3, 512) and (out == 0).all() and (lse == -math.inf).all()
+        for dv in (64, 128):
+            for keys in (0, 7):
+                stale(5, 3)
+                out, lse = G.latent_attention_expanded(new(T, 3, 128), new(T, 3, 64), new(keys, 3, 128), new(keys, 64),
+                                                       new(keys, 3, dv), start, start, scale=1.0, return_lse=True)
+                assert out.shape == (T, 3, dv) and (out == 0).all() and (lse == -math.inf).all()
+    # requests that hold nothing: a table without pages, a cache without pages, requests without keys
+    zeros, starts = torch.zeros(5, **i32), torch.arange(6, **i32)
+    for cache, table in ((new(2, 16, 576), torch.zeros((5, 0), **i32)), (new(0, 16, 576), torch.zeros((5, 2), **i32))):
+        out, lse = G.latent_attention_absorbed(new(5, 3, 512), new(5, 3, 64), cache, table, zeros, scale=1.0, return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    for causal in (True, False):
+        out, lse = G.latent_attention_expanded(new(5, 3, 128), new(5, 3, 64), new(0, 3, 128), new(0, 64), new(0, 3, 128),
+                                               starts, zeros.new_zeros(6), scale=1.0, causal=causal, return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    G.check_latent_status()
+    q = G.latent_cache_write(new(0, 576), new(2, 16, 576), none.long(), positions=none, queries=new(0, 3, 64),
+                             inv_freq=torch.ones(32, dtype=torch.float64, device=dev))
+    assert q.shape == (0, 3, 64)
+    plan = G.plan_pages(none, none, torch.zeros((0, 4), **i32), none, start, page_size=16, tokens=0)
+    assert plan.slots.numel() == 0 and plan.query_starts.tolist() == [0] and plan.free_count.tolist() == [0]
+    G.check_latent_status()
+
+
+ONE_CALL_THEN_CAPTURE = """
+import torch
+import glm53_flash_mlx_b200 as G
+
+i32 = dict(dtype=torch.int32, device="cuda")
+one = torch.ones(2, **i32)
+table = torch.full((2, 4), -1, **i32)
+plan = lambda: G.plan_pages(one * 0, one, table, torch.arange(8, **i32), one[:1] * 8, page_size=16, tokens=3)
+plan()  # the one call on this device before captures
+results = []
+for dt in (torch.bfloat16, torch.float16):
+    new = lambda *shape: torch.ones(shape, dtype=dt, device="cuda")
+    for H in (16, 32, 64):
+        q, cache, t = new(2, H, 576), new(4, 16, 576), torch.zeros((2, 1), **i32)
+        n, e, k = one * 16, new(2, H, 256), new(32, H, 256)
+        starts = torch.arange(3, **i32)
+        kv, slots, pos, freq = new(2, 576), starts[:2].long(), one, torch.ones(32, dtype=torch.float64, device="cuda")
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            a = G.latent_attention_absorbed(q[..., :512], q[..., 512:], cache, t, n, scale=0.05)
+            b = G.latent_attention_expanded(e, None, k, None, k, starts, starts * 16, scale=0.05)
+            c = G.latent_cache_write(kv, cache, slots, positions=pos, inv_freq=freq, queries=q[..., 512:])
+        g.replay()
+        results.append((a, b, c))
+torch.cuda.synchronize()
+G.check_latent_status()
+assert all((a == 1).all() and (b == 1).all() for a, b, _ in results)
+print("captured")
+"""
+
+
+@pytest.mark.gpu
+def test_capture_after_one_call_of_another_operator():
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parents[1]
+    env = dict(os.environ, PYTHONPATH=str(root))
+    got = subprocess.run([sys.executable, "-c", ONE_CALL_THEN_CAPTURE], env=env, cwd=root, capture_output=True, text=True,
+                         timeout=300)
+    assert got.returncode == 0 and "captured" in got.stdout, got.stderr[-2000:]
+
+
+@pytest.mark.gpu
 def test_a_second_chunk_over_the_rows_in_the_cache():
     """A prompt's next chunk attends over what is in the cache already: the keys' slots follow from the block table and
     the lengths, and the expanded form over those rows gives each query what one call over the whole prompt gives."""
