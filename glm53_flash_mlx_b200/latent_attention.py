@@ -46,6 +46,7 @@ def _status(index: int) -> tuple:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("call a latent-attention operator once on this device before capturing it")
         sw = StatusWord(torch.device("cuda", index))
+        torch.cuda.current_stream(index).synchronize()  # cleared before a call on any stream sets it
         entry = _STATUS[index] = (sw, sw.word.data_ptr(), sw.host.data_ptr(), sw._host_word)
     return entry
 

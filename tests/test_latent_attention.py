@@ -1445,6 +1445,35 @@ def test_capture_after_one_call_of_another_operator():
 
 
 @pytest.mark.gpu
+def test_status_word_is_clear_before_any_stream_sets_it(monkeypatch):
+    """The first call on a device makes the status word on its own stream; a call on another stream may run first."""
+    import glm53_flash_mlx_b200 as G
+    from glm53_flash_mlx_b200 import latent_attention as L
+
+    ql, qr, cache, table, n, _, _ = make_absorbed([100, 30], [1, 1], 16, 512, 64, 16, torch.bfloat16, 9)
+    bad = table.clone()
+    bad[1, 1] = cache.shape[0]
+    G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05)
+    monkeypatch.setattr(L, "_STATUS", {})
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (first, second):
+        with torch.cuda.stream(s):  # blocks of the word's size that hold other bits, for the allocator
+            blocks = [torch.full((64,), -1, dtype=torch.int32, device="cuda") for _ in range(2000)]
+            del blocks
+    pinned = [torch.zeros(4, dtype=torch.int32).pin_memory() for _ in range(4)]
+    del pinned  # a pinned block at hand: to get a new one would wait for the device
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        torch.cuda._sleep(200_000_000)
+        G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05)
+    with torch.cuda.stream(second):
+        G.latent_attention_absorbed(ql, qr, cache, bad, n, scale=0.05)
+    with pytest.raises(IndexError, match="page"):
+        G.check_latent_status()
+    G.check_latent_status()
+
+
+@pytest.mark.gpu
 def test_a_second_chunk_over_the_rows_in_the_cache():
     """A prompt's next chunk attends over what is in the cache already: the keys' slots follow from the block table and
     the lengths, and the expanded form over those rows gives each query what one call over the whole prompt gives."""
