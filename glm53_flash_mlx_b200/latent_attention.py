@@ -20,6 +20,7 @@ the device.  Errors that only the device can see (a page id outside the cache,
 a plan that does not fit) set a status word: the call leaves its documented
 safe result and the next call of this module raises (``IndexError`` /
 ``RuntimeError``); ``check_latent_status()`` synchronises and raises at once.
+A call under capture raises too, but leaves the word to the next eager one.
 """
 
 from __future__ import annotations
@@ -31,7 +32,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as N
-from .packed import StatusWord, _SYNC_STATUS
+from .packed import StatusWord, _SYNC_STATUS, _raise_status
 
 _DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_FP16}
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
@@ -87,6 +88,8 @@ class _Entry:
         """Call on the device's current stream with its status word, whatever the current device is."""
         sw, word, host, mirror = _status(index)
         if mirror.value:
+            if torch.cuda.is_current_stream_capturing():
+                _raise_status(mirror.value & 0xFFFFFFFF)  # a capture can neither wait for the device nor clear the word
             sw.raise_pending()
         lib = N._lib or N.lib()
         stream = _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream

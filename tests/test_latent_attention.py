@@ -1474,6 +1474,31 @@ def test_status_word_is_clear_before_any_stream_sets_it(monkeypatch):
 
 
 @pytest.mark.gpu
+def test_an_error_before_a_capture_is_raised_in_it():
+    import glm53_flash_mlx_b200 as G
+
+    ql, qr, cache, table, n, _, _ = make_absorbed([100, 30], [1, 1], 16, 512, 64, 16, torch.bfloat16, 9)
+    call = lambda t: G.latent_attention_absorbed(ql, qr, cache, t, n, scale=0.05)
+    want = call(table)
+    bad = table.clone()
+    bad[1, 1] = cache.shape[0]
+    call(bad)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(IndexError, match="page"):
+        with torch.cuda.graph(g):
+            call(table)
+    with pytest.raises(IndexError, match="page"):  # a capture cannot clear the word
+        G.check_latent_status()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call(table)
+    g.replay()
+    G.check_latent_status()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
 def test_a_second_chunk_over_the_rows_in_the_cache():
     """A prompt's next chunk attends over what is in the cache already: the keys' slots follow from the block table and
     the lengths, and the expanded form over those rows gives each query what one call over the whole prompt gives."""
