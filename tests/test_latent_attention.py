@@ -1499,6 +1499,95 @@ def test_an_error_before_a_capture_is_raised_in_it():
 
 
 @pytest.mark.gpu
+def test_views_that_are_copied_first():
+    """Rows that 16-byte pieces cannot read, and integer tensors that are not contiguous, give what copies give."""
+    import glm53_flash_mlx_b200 as G
+
+    def views(x):
+        wide = torch.full((*x.shape[:-1], x.shape[-1] + 9), math.nan, dtype=x.dtype, device="cuda")
+        wide[..., 1:1 + x.shape[-1]] = x
+        spread = torch.full((*x.shape[:-1], 2 * x.shape[-1]), math.nan, dtype=x.dtype, device="cuda")
+        spread[..., ::2] = x
+        turned = x.transpose(0, -1).contiguous().transpose(0, -1)
+        yield from (wide[..., 1:1 + x.shape[-1]], spread[..., ::2], turned)
+
+    def gaps(x):
+        return torch.stack([x, x - 5], -1)[..., 0]
+
+    ql, qr, cache, table, n, starts, _ = make_absorbed([100, 30, 7], [2, 1, 1], 16, 512, 64, 16, torch.bfloat16, 9)
+    want = G.latent_attention_absorbed(ql, qr, cache, table, n, scale=0.05, query_starts=starts)
+    for a, b in zip(views(ql), views(qr)):
+        assert torch.equal(G.latent_attention_absorbed(a, b, cache, gaps(table), gaps(n), scale=0.05,
+                                                       query_starts=gaps(starts)), want)
+    t = make_expanded([140, 3], [200, 30], 2, 128, 64, 128, torch.bfloat16, 8)
+    want = G.latent_attention_expanded(*t, scale=0.07)
+    for x in zip(*(views(y) for y in t[:5])):
+        assert torch.equal(G.latent_attention_expanded(*x, gaps(t[5]), gaps(t[6]), scale=0.07), want)
+
+    kv, q = torch.randn((9, 576), device="cuda").bfloat16(), torch.randn((9, 3, 64), device="cuda").bfloat16()
+    w, freq = torch.rand(512, device="cuda").bfloat16(), torch.rand(32, device="cuda", dtype=torch.float64)
+    pos, slots = torch.arange(9, device="cuda").int() * 77, torch.randperm(32, device="cuda")[:9]
+    store = lambda kv, q, w, pos, slots, freq: (c := torch.zeros((2, 16, 576), dtype=torch.bfloat16, device="cuda"),
+                                                G.latent_cache_write(kv, c, slots, norm_weight=w, positions=pos,
+                                                                     inv_freq=freq, queries=q))
+    want = store(kv, q, w, pos, slots, freq)
+    for a, b, c in zip(views(kv), views(q), views(w)):
+        got = store(a, b, c, gaps(pos), gaps(slots), gaps(freq))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    G.check_latent_status()
+
+
+@pytest.mark.gpu
+def test_a_cache_past_32_bits():
+    """Rows stored and read beyond 2^31 values and 2^32 bytes of the cache."""
+    import glm53_flash_mlx_b200 as G
+
+    dt, page, pages = torch.bfloat16, 64, 70000  # 2.6 x 10^9 values, 5.2 x 10^9 bytes
+    cache = torch.full((pages, page, 576), math.nan, dtype=dt, device="cuda")
+    lens = [300, 70]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ids = torch.tensor([[pages - 1, 3, 58300, pages - 2, 30000], [58255, 65000, -1, -1, -1]], dtype=torch.int32, device="cuda")
+    rows = [torch.randn((m, 576), generator=g, device="cuda").to(dt) for m in lens]
+    slots = torch.cat([ids[i].long()[torch.arange(m, device="cuda") // page] * page + torch.arange(m, device="cuda") % page
+                       for i, m in enumerate(lens)])
+    G.latent_cache_write(torch.cat(rows), cache, slots)
+    assert torch.equal(cache.view(-1, 576)[slots], torch.cat(rows))
+    q = torch.randn((2, 64, 576), generator=g, device="cuda").to(dt)
+    out, lse = G.latent_attention_absorbed(q[..., :512], q[..., 512:], cache, ids,
+                                           torch.tensor(lens, dtype=torch.int32, device="cuda"), scale=0.06, return_lse=True)
+    G.check_latent_status()
+    check(out, lse, *absorbed64(q[..., :512], q[..., 512:], rows, lens, [1, 1], 0.06, dt))
+
+
+@pytest.mark.gpu
+def test_a_prompt_batch_past_32_bits():
+    """Queries, keys, values and results of more than 2^31 values each; the last requests' results against 64 bits."""
+    import glm53_flash_mlx_b200 as G
+
+    dt, H, dn, dv, B, n = torch.bfloat16, 64, 192, 256, 1100, 128  # 140,800 rows
+    T = B * n
+    q = torch.zeros((T, H, dn + r), dtype=dt, device="cuda")
+    kv = torch.full((T, H, dn + dv), math.nan, dtype=dt, device="cuda")
+    kr = torch.zeros((T, 64), dtype=dt, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    last = slice(T - 2 * n, T)
+    for x in (q, kv, kr):
+        x[last] = torch.randn(x[last].shape, generator=g, device="cuda").to(dt)
+    kv[T - n + 70, 5, dn + 17] = math.inf  # a value that its epilogue adds again
+    starts = torch.arange(B + 1, dtype=torch.int32, device="cuda") * n
+    out, lse = G.latent_attention_expanded(q[..., :dn], q[..., dn:], kv[..., :dn], kr, kv[..., dn:], starts, starts,
+                                           scale=0.06, return_lse=True)
+    G.check_latent_status()
+    got, hit = out[last].clone(), torch.zeros((2 * n, H, dv), dtype=torch.bool, device="cuda")
+    hit[n + 70:, 5, 17] = True
+    assert (got[hit] == math.inf).all() and out[: T - 2 * n].isnan().all()
+    want = expanded64(q[last][..., :dn], q[last][..., dn:], kv[last][..., :dn], kr[last], kv[last][..., dn:], [n, n], [n, n],
+                      0.06, True, dt)
+    got[hit] = want[0][hit].to(dt)  # (the 64-bit form leaves out values that are not finite)
+    check(got, lse[last], *want)
+
+
+@pytest.mark.gpu
 def test_a_second_chunk_over_the_rows_in_the_cache():
     """A prompt's next chunk attends over what is in the cache already: the keys' slots follow from the block table and
     the lengths, and the expanded form over those rows gives each query what one call over the whole prompt gives."""
