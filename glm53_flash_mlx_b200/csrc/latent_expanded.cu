@@ -881,8 +881,10 @@ int launch(const CUtensorMap& qn, const CUtensorMap& qr, const CUtensorMap& kn, 
   // tile come before the next tile, so one request's keys and values of all
   // heads should stay in L2 (126 MB): over 8,192 keys of 256 + 192 values
   // (402 MB) 947 / 772, of 192 + 64 (201 MB) 615 / 543.  Many short requests, one
-  // unit a CTA / walking: 300 of 100 queries and keys 2,230 / 1,026, 2,000 of 3 and
-  // 20 19,960 / 5,640.  A pair's units are long and stay one each.
+  // unit a CTA / walking: 300 of 100 queries and keys 2,230 / 1,051, 2,000 of 3 and
+  // 20 19,960 / 5,720.  A pair's units are long and stay one each.  Lengths are on
+  // the device: `held` and the rule for pairs go by averages, measured with equal
+  // requests, and one long request among many short ones gets what those get.
   const double held = 2.0 * a.Tk / a.B * a.H * (a.dn + a.dv);
   b.persistent = !PAIR && held <= 126e6;
   cudaLaunchConfig_t cfg = {};
@@ -991,9 +993,9 @@ extern "C" int glm53_latent_expanded(const void* q_nope, int64_t qn_stride_t, in
     return bf16 ? launch<__nv_bfloat16, true>(qn, qr, kn, kr, v, a, st) : launch<__half, true>(qn, qr, kn, kr, v, a, st);
   // Softmax warps whose search for a unit goes on where it stood, for many
   // requests: 64 heads, from the start / so, 200 requests of 20 queries and 40
-  // keys 658 / 605 us, 300 1,049 / 902, 2,000 of 3 and 20 16,400 / 5,640; but
-  // spilled registers cost 8 requests of 512 154 / 159, five ragged ones of 16
-  // heads 31.3 / 32.0.
+  // keys 682 / 640 us, 300 1,081 / 951, 2,000 of 3 and 20 17,050 / 5,720; but what
+  // is kept in shared memory costs 8 requests of 512 156 / 161, five ragged ones
+  // of 16 heads 31.1 / 31.6 (both spill: 164 / 176 bytes stored, 132 / 152 loaded).
   if (requests > 128)
     return bf16 ? launch<__nv_bfloat16, false, true>(qn, qr, kn, kr, v, a, st)
                 : launch<__half, false, true>(qn, qr, kn, kr, v, a, st);

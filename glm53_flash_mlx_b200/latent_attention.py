@@ -13,12 +13,15 @@ one rotary row in a paged cache, and all heads read them.
     out = latent_attention_expanded(q[..., :192], q_rope, kv_b[..., :192], cache_rope, kv_b[..., 192:],
                                     plan.query_starts, key_starts, scale=scale)   # prefill
 
-Tensors are BF16 or FP16; products, statistics and sums are FP32, rounded once
-into the result.  Lengths, tables and plans stay on the device: no call reads
-them back, so each can be captured into a CUDA graph after one eager call on
-the device.  Errors that only the device can see (a page id outside the cache,
-a plan that does not fit) set a status word: the call leaves its documented
-safe result and the next call of this module raises (``IndexError`` /
+Tensors are BF16 or FP16.  Scores, maxima, sums and results are FP32 until the
+result is rounded; in between the tensor cores take the softmax weights in the
+tensors' type, one rounding more each (their sum takes them unrounded), so the
+error against exact results is up to 1.4 times that of a 32-bit form.
+Lengths, tables and plans stay on the device: no call reads them back, so each
+can be captured into a CUDA graph after one eager call of any of them on the
+device.  Errors that only the device can see (a page id outside the cache, a
+plan that does not fit) set a status word: the call leaves its documented safe
+result and the next call of this module raises (``IndexError`` /
 ``RuntimeError``); ``check_latent_status()`` synchronises and raises at once.
 A call under capture raises too, but leaves the word to the next eager one.
 """

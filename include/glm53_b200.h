@@ -717,7 +717,9 @@ int glm53_head_major_to_rows(const void* head_major, int64_t heads, int64_t rows
  * of the cache is row slot % page_size of page slot / page_size.  A request's
  * block table row lists its pages in order.  `status_host`, where given, is a
  * pinned (device-mapped) word that a kernel which sets a status bit also
- * writes.  Strides count elements.
+ * writes.  Strides count elements.  Both attention forms keep scores, maxima,
+ * sums and results in FP32 and round the result once; each softmax weight is
+ * rounded to `dtype` where it meets its value (their sum is of unrounded ones).
  * --------------------------------------------------------------------- */
 
 /* Block tables and slot maps from request lengths, in one launch.
